@@ -1,0 +1,366 @@
+"""What the token operators (vision_assist_amd.tokens) are measured on, and their plain forms.
+
+The operators form one attention layer over the tokens of camera frames: a matrix product with bias, activation and
+residual (Linear), the norms of queries and keys for each head with a rotation over time, height and width, written
+into a stream's cache (QKNorm), and attention with a sliding window and first tokens that stay visible (attend).
+
+Sizes: 400 and 1600 tokens are the 20 x 20 and 40 x 40 maps of a 640 x 640 frame; 32 and 64 streams stand for
+cameras served together; channels and heads are generic.
+"""
+import math
+
+import torch
+
+own = False
+
+DT = {"bf16": torch.bfloat16, "w8a16": torch.bfloat16, "f32": torch.float32}
+
+
+# ------------------------------------------------------------------ cases
+def listed():
+    return [
+        # the up-projection of one stream's one new token: latency, and the weights read once
+        dict(name="linear one token", op="linear", dtype="bf16", M=1, K=1024, N=4096, act="gelu", bias=True, res=False),
+        # one new token of each of 32 streams on e4m3 weights: the bytes of the weights
+        dict(name="linear 32 streams w8a16", op="linear", dtype="w8a16", M=32, K=4096, N=4096, act="silu", bias=True,
+             res=False),
+        # the reference's precision on a ragged size: a down-projection onto the residual stream
+        dict(name="linear f32 odd", op="linear", dtype="f32", M=1603, K=520, N=1000, act=None, bias=True, res=True),
+        # a batch of clips: 64 frames of 400 tokens
+        dict(name="linear clip", op="linear", dtype="bf16", M=25600, K=1024, N=4096, act="gelu", bias=True, res=False),
+        # one new token of each of 64 streams into their caches (rings that have wrapped)
+        dict(name="qk step", op="qk", dtype="bf16", B=64, S=1, Hq=16, Hk=8, D=128, R=128, axes=1, layout="half",
+             cache=True, slots=516, sinks=4, kv=1500),
+        # eight 40 x 40 frames: positions of time, height and width
+        dict(name="qk frames", op="qk", dtype="bf16", B=8, S=1600, Hq=12, Hk=12, D=64, R=64, axes=3, layout="half",
+             cache=False, slots=0, sinks=0, kv=0),
+        # the reference's precision, a head size that is no power of two, rotated in part, a padded batch
+        dict(name="qk f32 odd", op="qk", dtype="f32", B=3, S=1201, Hq=12, Hk=4, D=80, R=64, axes=2, layout="pairs",
+             cache=True, slots=1300, sinks=0, kv=1201),
+        # one new token of each of 32 streams over a long cache whose ring has wrapped
+        dict(name="attention step", op="attn", dtype="bf16", B=32, S=1, Hq=32, Hk=8, D=128, Dv=128, slots=6800,
+             frame=1, window=6400, sinks=400, kv=9000, ragged=True),
+        # a new frame of 400 tokens of each of 8 streams: its own tokens, the six frames before, the first frame
+        dict(name="attention frame", op="attn", dtype="bf16", B=8, S=400, Hq=16, Hk=8, D=128, Dv=128, slots=3200,
+             frame=400, window=2800, sinks=400, kv=12000, ragged=False),
+        # two clips of 16 frames, padded to the longer one
+        dict(name="attention clips", op="attn", dtype="bf16", B=2, S=6400, Hq=12, Hk=12, D=64, Dv=64, slots=6400,
+             frame=400, window=2400, sinks=400, kv=6400, ragged=True),
+        # one long sequence, token by token: a window and four sinks
+        dict(name="attention long", op="attn", dtype="bf16", B=1, S=8192, Hq=16, Hk=2, D=128, Dv=128, slots=8192,
+             frame=1, window=4096, sinks=4, kv=8192, ragged=False),
+        # the attention block of a 20 x 20 map in the reference's precision: every token sees every token
+        dict(name="attention map f32", op="attn", dtype="f32", B=16, S=400, Hq=8, Hk=8, D=32, Dv=64, slots=400,
+             frame=0, window=0, sinks=0, kv=400, ragged=False),
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    op = rng.choice(["linear", "linear", "qk", "attn", "attn"])
+    if op == "linear":
+        dtype = rng.choice(["bf16", "bf16", "w8a16", "f32"])
+        while True:
+            M, K, N = _log(rng, 1, 25600), 8 * _log(rng, 8, 512), _log(rng, 40, 4096)
+            if M * K * N * (4 if dtype == "f32" else 1) <= 25600 * 1024 * 4096:
+                break
+        return dict(op=op, dtype=dtype, M=M, K=K, N=N, act=rng.choice([None, "silu", "gelu", "gelu_tanh", "relu"]),
+                    bias=rng.random() < 0.8, res=rng.random() < 0.5)
+    if op == "qk":
+        while True:
+            B, S, Hk, G = _log(rng, 1, 64), rng.choice([1, _log(rng, 2, 6400)]), rng.randint(1, 12), rng.choice([1, 2, 4])
+            D = rng.choice([32, 64, 72, 80, 96, 128])
+            if B * S * Hk * (G + 2) * D <= 8 * 1600 * 36 * 64:
+                break
+        R = D if D % 16 == 0 and rng.random() < 0.7 else 32
+        cache = rng.random() < 0.5
+        return dict(op=op, dtype=rng.choice(["bf16", "bf16", "f32"]), B=B, S=S, Hq=Hk * G, Hk=Hk, D=D, R=R,
+                    axes=rng.randint(1, 3), layout=rng.choice(["half", "pairs"]), cache=cache,
+                    slots=S + rng.randint(4, 200) if cache else 0, sinks=rng.randint(0, 4) if cache else 0,
+                    kv=S + rng.randint(0, 3000) if cache else 0)
+    dtype, form = rng.choice(["bf16", "bf16", "bf16", "f32"]), rng.choice(["step", "frame", "clip"])
+    while True:
+        Hk, G, D = rng.randint(1, 8), rng.choice([1, 2, 4, 8]), rng.choice([32, 64, 80, 128])
+        Dv = D if D != 32 or rng.random() < 0.5 else 64
+        if form == "step":
+            B, S, slots, frame = _log(rng, 1, 64), rng.choice([1, 1, 1, 2, 4]), _log(rng, 60, 9000), 1
+            sinks = rng.randint(0, 40)
+            window, kv = slots - sinks - S + 1, rng.choice([slots, slots + rng.randint(1, 5000)])
+        elif form == "frame":
+            frame = _log(rng, 50, 1600)
+            B, S, n = _log(rng, 1, 8), frame, rng.randint(1, 6)
+            sinks, window = rng.choice([0, 4, frame]), n * frame
+            slots = sinks + window + frame
+            kv = frame * rng.randint(1, 20)
+        else:
+            B, S = _log(rng, 1, 8), _log(rng, 100, 8192)
+            frame = rng.choice([0, 1, 1, rng.randint(20, 500)])
+            sinks, window = rng.choice([0, 4, 100]), 0 if rng.random() < 0.4 else _log(rng, 32, 4096)
+            slots = kv = S
+        if B * Hk * G * S * slots * (4 if dtype == "f32" else 1) <= 16 * 8192 * 8192 and B * slots * Hk * D <= 32 * 6800 * 1024:
+            break
+    return dict(op=op, dtype=dtype, B=B, S=S, Hq=Hk * G, Hk=Hk, D=D, Dv=Dv, slots=slots, frame=frame, window=window,
+                sinks=sinks, kv=kv, ragged=rng.random() < 0.5)
+
+
+# ------------------------------------------------------------------ inputs
+def _lens(c):
+    """(q_len, kv_len) of each sequence; a ragged batch has shorter ones among them."""
+    q, kv = [], []
+    for b in range(c["B"]):
+        cut = (b * 37 + b * b * 11) if c.get("ragged") else 0
+        if c["S"] <= 4:
+            q.append(c["S"])
+            kv.append(max(c["S"], c["kv"] - 5 * cut % max(1, c["kv"])))
+        else:
+            q.append(max(1, c["S"] - (cut * 26) % c["S"]))
+            kv.append(c["kv"] - (c["S"] - q[-1]))
+    return q, kv
+
+
+def _qk_lens(c):
+    q = [c["S"] - (b * 7) % c["S"] for b in range(c["B"])] if c["cache"] else [c["S"]] * c["B"]
+    return q, [c["kv"] - (c["S"] - n) for n in q]
+
+
+def _sections(c):
+    """Rotated pairs of each axis."""
+    pairs, a = c["R"] // 2, c["axes"]
+    each = pairs // a
+    return [pairs - each * (a - 1)] + [each] * (a - 1)
+
+
+def prepare(case, seed):
+    c, dev = case, "cuda"
+    g = torch.Generator(device=dev).manual_seed(seed)
+    dt = DT[c["dtype"]]
+
+    def rand(*shape, dtype=dt, by=1.0):
+        return (torch.randn(shape, generator=g, device=dev) * by).to(dtype)
+
+    s = {"case": c}
+    if c["op"] == "linear":
+        M, K, N = c["M"], c["K"], c["N"]
+        s["x"], s["w"], s["scale"] = rand(M, K), rand(N, K, dtype=torch.float32, by=K ** -0.5), None
+        if c["dtype"] == "w8a16":
+            s["scale"] = s["w"].abs().amax(1) / 448
+            s["w"] = (s["w"] / s["scale"][:, None]).to(torch.float8_e4m3fn)
+        else:
+            s["w"] = s["w"].to(dt)
+        s["bias"] = rand(N, dtype=torch.float32, by=0.1) if c["bias"] else None
+        s["res"] = rand(M, N) if c["res"] else None
+        if own:
+            from vision_assist_amd.tokens import Linear
+            s["linear"] = Linear(s["w"], s["bias"], act=c["act"], dtype=c["dtype"], scale=s["scale"])
+        return s
+    if c["op"] == "qk":
+        B, S, Hq, Hk, D = (c[k] for k in ("B", "S", "Hq", "Hk", "D"))
+        qkv = rand(B, S, Hq + 2 * Hk, D)  # one product's output, viewed as queries, keys and values
+        s["q"], s["k"], s["v"] = qkv[:, :, :Hq], qkv[:, :, Hq:Hq + Hk], qkv[:, :, Hq + Hk:]
+        s["wq"], s["wk"] = 1 + rand(D, dtype=torch.float32, by=0.1), 1 + rand(D, dtype=torch.float32, by=0.1)
+        q_len, kv_len = _qk_lens(c)
+        s["q_len"], s["kv_len"] = (torch.tensor(v, dtype=torch.int32, device=dev) for v in (q_len, kv_len))
+        t = torch.arange(S, device=dev)
+        t = (t + torch.randint(0, 100000, (B, 1), generator=g, device=dev)) if c["axes"] == 1 else t
+        pos = [t.expand(B, S)] if c["axes"] == 1 else [(t // 1600).expand(B, S), (t // 40 % 40).expand(B, S), (t % 40).expand(B, S)]
+        s["pos"] = torch.stack(pos[:c["axes"]], -1).to(torch.int32).contiguous()
+        s["q_out"] = torch.zeros(B, S, Hq, D, dtype=dt, device=dev)  # rows behind a sequence stay zero
+        if c["cache"]:
+            s["ck"], s["cv"] = rand(B, c["slots"], Hk, D), rand(B, c["slots"], Hk, D)
+        if own:
+            from vision_assist_amd.tokens import QKNorm, Rotary, TokenCache
+            rot = Rotary(c["R"], _sections(c), layout=c["layout"])
+            s["norm"] = QKNorm(D, rot, s["wq"], s["wk"], eps=1e-6)
+            if c["cache"]:
+                s["cache"] = TokenCache.of(s["ck"], s["cv"], sinks=c["sinks"], length=s["kv_len"])
+        return s
+    B, S, Hq, Hk, D, Dv, slots = (c[k] for k in ("B", "S", "Hq", "Hk", "D", "Dv", "slots"))
+    s["q"], s["k"], s["v"] = rand(B, S, Hq, D), rand(B, slots, Hk, D), rand(B, slots, Hk, Dv)
+    q_len, kv_len = _lens(c)
+    s["q_len"], s["kv_len"] = (torch.tensor(v, dtype=torch.int32, device=dev) for v in (q_len, kv_len))
+    s["out"] = torch.zeros(B, S, Hq, Dv, dtype=dt, device=dev)
+    return s
+
+
+# ------------------------------------------------------------------ one pass
+def _act(y, act):
+    if act == "silu":
+        return y / (1 + torch.exp(-y))
+    if act == "gelu":
+        return 0.5 * y * torch.erfc(y * -(0.5 ** 0.5))
+    if act == "gelu_tanh":
+        return 0.5 * y * (1 + torch.tanh((2 / math.pi) ** 0.5 * (y + 0.044715 * y * y * y)))
+    return torch.clamp(y, min=0) if act == "relu" else y
+
+
+def _linear(s):
+    c = s["case"]
+    w = s["w"].float() if s["scale"] is None else s["w"].float() * s["scale"][:, None]
+    y = s["x"].float() @ w.t()
+    y = _act(y if s["bias"] is None else y + s["bias"], c["act"])
+    return (y if s["res"] is None else y + s["res"].float()).to(DT[c["dtype"]])
+
+
+def _turn(x, w, angle, c):
+    """Norm of each head, weight, rotation by angle [B, S, R / 2] in the first R values."""
+    x = x.float()
+    x = x * torch.rsqrt((x * x).mean(-1, keepdim=True) + 1e-6) * w
+    R = c["R"]
+    cos, sin = torch.cos(angle).float()[:, :, None], torch.sin(angle).float()[:, :, None]
+    if c["layout"] == "half":
+        a, b = x[..., :R // 2], x[..., R // 2:R]
+        return torch.cat([a * cos - b * sin, b * cos + a * sin, x[..., R:]], -1).to(DT[c["dtype"]])
+    a, b = x[..., 0:R:2], x[..., 1:R:2]
+    return torch.cat([torch.stack([a * cos - b * sin, b * cos + a * sin], -1).flatten(-2), x[..., R:]], -1).to(DT[c["dtype"]])
+
+
+def _qk(s):
+    c = s["case"]
+    R, dev, n = c["R"], s["q"].device, _sections(c)
+    freq = 10000.0 ** (-torch.arange(R // 2, dtype=torch.float64, device=dev) * 2 / R)
+    axis = torch.repeat_interleave(torch.arange(len(n), device=dev), torch.tensor(n, device=dev), output_size=R // 2)
+    angle = s["pos"].double()[..., axis] * freq
+    q, k = _turn(s["q"], s["wq"], angle, c), _turn(s["k"], s["wk"], angle, c)
+    if not c["cache"]:
+        return q, k
+    i = torch.arange(c["S"], device=dev)
+    there = i < s["q_len"][:, None]
+    p = (s["kv_len"] - s["q_len"])[:, None] + i
+    ring = c["slots"] - c["sinks"]
+    keep = there & ((p < c["sinks"]) | (p >= s["kv_len"][:, None] - ring))
+    slot = torch.where(p < c["sinks"], p, c["sinks"] + (p - c["sinks"]) % ring)
+    b, j = torch.nonzero(keep, as_tuple=True)
+    s["ck"][b, slot[b, j]], s["cv"][b, slot[b, j]] = k[b, j], s["v"][b, j]
+    return q * there[:, :, None, None], s["ck"], s["cv"]
+
+
+def _attend(s):
+    c = s["case"]
+    B, S, Hq, Hk, D, slots, sinks, frame = (c[k] for k in ("B", "S", "Hq", "Hk", "D", "slots", "sinks", "frame"))
+    dev, G = s["q"].device, Hq // Hk
+    kv, i, j = s["kv_len"].long()[:, None, None], torch.arange(S, device=dev)[None, :, None], torch.arange(slots, device=dev)
+    at = kv - s["q_len"].long()[:, None, None] + i
+    ring = slots - sinks
+    p = torch.where(j < sinks, j, kv - 1 - (kv - 1 - j) % ring)  # the newest position that is held in slot j
+    end = (at // frame + 1) * frame if frame else torch.full_like(at, 1 << 40)
+    see = (p >= j) & (p < kv) & (p < end) & (at >= 0)
+    if c["window"]:
+        see = see & ((p < sinks) | (p >= end - c["window"]))
+    there = (i < s["q_len"][:, None, None])[:, :, :, None]
+    q = s["q"].float().reshape(B, S, Hk, G, D).permute(0, 2, 3, 1, 4).reshape(B, Hk, G * S, D)
+    a = (q @ s["k"].float().permute(0, 2, 3, 1).contiguous()).mul_(D ** -0.5).view(B, Hk, G, S, slots)
+    a.masked_fill_(~see[:, None, None], -math.inf)
+    a.sub_(a.amax(-1, keepdim=True).clamp_(min=-1e30)).exp_()
+    total = a.sum(-1, keepdim=True)
+    o = (a.view(B, Hk, G * S, slots) @ s["v"].float().permute(0, 2, 1, 3).contiguous()).view(B, Hk, G, S, -1)
+    o = (o / torch.where(total > 0, total, 1.0)).permute(0, 3, 1, 2, 4).reshape(B, S, Hq, -1)
+    return torch.where(there, o, 0.0).to(DT[c["dtype"]])
+
+
+def run(state):
+    s, c = state, state["case"]
+    if not own:
+        return {"linear": _linear, "qk": _qk, "attn": _attend}[c["op"]](s)
+    if c["op"] == "linear":
+        return s["linear"](s["x"], residual=s["res"])
+    if c["op"] == "qk":
+        if not c["cache"]:
+            return s["norm"](s["q"], s["k"], s["pos"])
+        s["norm"].store(s["q"], s["k"], s["v"], s["pos"], s["cache"], q_len=s["q_len"], q_out=s["q_out"])
+        return s["q_out"], s["ck"], s["cv"]
+    from vision_assist_amd.tokens import attend
+    return attend(s["q"], s["k"], s["v"], frame=c["frame"], window=c["window"], sinks=c["sinks"], q_len=s["q_len"],
+                  kv_len=s["kv_len"], out=s["out"])
+
+
+# ------------------------------------------------------------------ what a pass needs
+def _seen(c, q, kv):
+    """(query, key) pairs of one sequence and the keys that any of its queries sees."""
+    pairs, first, some = 0, 1 << 40, 0
+    held = max(c["sinks"], kv - (c["slots"] - c["sinks"]))  # the oldest position behind the sinks that is still there
+    for at in range(max(0, kv - q), kv):
+        end = (at // c["frame"] + 1) * c["frame"] if c["frame"] else 1 << 40
+        top = min(end, kv)
+        low = max(held, end - c["window"] if c["window"] else 0)
+        pinned = min(c["sinks"], top)
+        pairs += pinned + max(0, top - low)
+        first, some = min(first, low), max(some, pinned)
+    return pairs, some + max(0, kv - first)
+
+
+def work(case):
+    c, e = case, DT[case["dtype"]].itemsize
+    if c["op"] == "linear":
+        M, K, N = c["M"], c["K"], c["N"]
+        w = N * K * (1 if c["dtype"] == "w8a16" else e) + (4 * N if c["dtype"] == "w8a16" else 0)
+        return {"bytes": M * K * e + w + M * N * e * (2 if c["res"] else 1) + 4 * N * c["bias"], "flops": 2 * M * N * K}
+    if c["op"] == "qk":
+        tokens = sum(_qk_lens(c)[0])
+        heads = c["Hq"] + c["Hk"] * (2 if c["cache"] else 1)
+        return {"bytes": tokens * (2 * heads * c["D"] * e + 4 * c["axes"]), "flops": 8 * tokens * heads * c["D"]}
+    pairs, keys, rows = 0, 0, 0
+    for q, kv in zip(*_lens(c)):
+        n, m = _seen(c, q, kv)
+        pairs, keys, rows = pairs + n, keys + m, rows + q
+    return {"bytes": e * (keys * c["Hk"] + rows * c["Hq"]) * (c["D"] + c["Dv"]),
+            "flops": 2 * pairs * c["Hq"] * (c["D"] + c["Dv"])}
+
+
+# ------------------------------------------------------------------ the definitions in 64 bits
+def exact(case, seed):
+    c, s = case, prepare(case, seed)
+    if c["op"] == "linear":
+        w = s["w"].double()
+        if s["scale"] is not None:
+            w = s["scale"].double().diag_embed() @ w
+        y = torch.nn.functional.linear(s["x"].double(), w, None if s["bias"] is None else s["bias"].double())
+        name = {None: "none", "gelu_tanh": "gelu"}.get(c["act"], c["act"])
+        if name != "none":
+            f = getattr(torch.nn.functional, name)
+            y = f(y, approximate="tanh") if c["act"] == "gelu_tanh" else f(y)
+        return y if s["res"] is None else s["res"].double().add_(y)
+    if c["op"] == "qk":
+        R, lens = c["R"], _qk_lens(c)
+        axis = [a for a, n in enumerate(_sections(c)) for _ in range(n)]
+        theta = torch.stack([s["pos"][..., a].double() / 10000.0 ** (2 * f / R) for f, a in enumerate(axis)], -1)
+        turn = torch.polar(torch.ones_like(theta), theta)[:, :, None]
+
+        def one(x, w):
+            x = x.double()
+            x = torch.nn.functional.normalize(x, dim=-1, eps=0.0) * c["D"] ** 0.5 * w.double() / (1 + 1e-6 / x.square().mean(-1, keepdim=True)).sqrt()
+            head = x[..., :R]
+            z = torch.complex(*(head.unflatten(-1, (2, R // 2)).unbind(-2) if c["layout"] == "half" else head.unflatten(-1, (R // 2, 2)).unbind(-1))) * turn
+            x[..., :R] = torch.stack([z.real, z.imag], -2 if c["layout"] == "half" else -1).flatten(-2)
+            return x
+
+        q, k = one(s["q"], s["wq"]), one(s["k"], s["wk"])
+        if not c["cache"]:
+            return q, k
+        ck, cv, ring = s["ck"].double(), s["cv"].double(), c["slots"] - c["sinks"]
+        for b, (n, kv) in enumerate(zip(*lens)):
+            q[b, n:] = 0
+            where = {}
+            for i in range(n):  # a later token takes the slot of an earlier one
+                p = kv - n + i
+                where[p if p < c["sinks"] else c["sinks"] + (p - c["sinks"]) % ring] = i
+            to, of = (torch.tensor(list(v), device=q.device) for v in (where.keys(), where.values()))
+            ck[b, to], cv[b, to] = k[b, of], s["v"][b, of].double()
+        return q, ck, cv
+    out, G, ring = torch.zeros(s["out"].shape, dtype=torch.float64, device="cuda"), c["Hq"] // c["Hk"], c["slots"] - c["sinks"]
+    for b, (n, kv) in enumerate(zip(*_lens(c))):
+        held = torch.tensor([p for p in range(kv) if p < c["sinks"] or p >= kv - ring], device="cuda")  # in their order
+        slot = torch.where(held < c["sinks"], held, (held - c["sinks"]) % ring + c["sinks"])
+        at = torch.arange(kv - n, kv, device="cuda")[:, None]
+        end = torch.div(at, c["frame"], rounding_mode="floor") * c["frame"] + c["frame"] if c["frame"] else at + (1 << 40)
+        hide = held >= end
+        if c["window"]:
+            hide |= (held < end - c["window"]) & (held >= c["sinks"])
+        for h in range(c["Hk"]):
+            k, v = s["k"][b, slot, h].double(), s["v"][b, slot, h].double()
+            for m in range(h * G, (h + 1) * G):
+                a = torch.addmm(torch.zeros((), dtype=torch.float64, device="cuda"), s["q"][b, :n, m].double(), k.t()) / c["D"] ** 0.5
+                out[b, :n, m] = torch.softmax(a.masked_fill_(hide, -math.inf), -1).nan_to_num_(0.0) @ v
+    return out
