@@ -98,7 +98,7 @@ def draw(rng):
         else:
             B, S = _log(rng, 1, 8), _log(rng, 100, 8192)
             frame = rng.choice([0, 1, 1, rng.randint(20, 500)])
-            sinks, window = rng.choice([0, 4, 100]), 0 if rng.random() < 0.4 else _log(rng, 32, 4096)
+            sinks, window = rng.choice([0, 4, 100]) if frame else 0, 0 if not frame or rng.random() < 0.4 else _log(rng, 32, 4096)
             slots = kv = S
         if B * Hk * G * S * slots * (4 if dtype == "f32" else 1) <= 16 * 8192 * 8192 and B * slots * Hk * D <= 32 * 6800 * 1024:
             break
