@@ -19,9 +19,8 @@ constexpr int RSRC = 0x00020000;      // buffer descriptor word 3 (gfx9 raw buff
 // bf16 epilogues: hardware exp and reciprocal (~1 ulp f32, far below the bf16 rounding that follows),
 // the same expression as va_seg.hip's unfused layers
 __device__ __forceinline__ float silu(float x) { return x * __builtin_amdgcn_rcpf(1.0f + __expf(-x)); }
-// four SiLUs with the plain f32 steps packed in pairs (v_pk_mul_f32 / v_pk_add_f32 around the two
-// 8-cycle transcendentals): the same operations in the same order as silu(), so bit-identical.  (Briefly
-// blamed for va_pw.hip's sporadic non-finite outputs; the cause was that kernel's store hazard)
+// SiLUs in pairs around the two 8-cycle transcendentals: the same operations in the same order as silu(), so
+// bit-identical (the library is built without the packed-f32 instructions: Makefile)
 __device__ __forceinline__ f32x2 silu2(f32x2 x) {
     const f32x2 t = x * (f32x2){-1.4426950408889634f, -1.4426950408889634f};
     const f32x2 e = {__builtin_amdgcn_exp2f(t[0]), __builtin_amdgcn_exp2f(t[1])};

@@ -59,7 +59,7 @@ __device__ inline __bf16 from_f<__bf16>(float v) {
 // follows); the exact-f32 parity path uses silu_exact
 __device__ inline float silu(float x) { return x * __builtin_amdgcn_rcpf(1.0f + __expf(-x)); }
 __device__ inline float silu_exact(float x) { return x / (1.0f + expf(-x)); }
-// silu() over an array, the plain f32 steps packed in pairs (fz::silu2): bit-identical to silu() per element
+// silu() over an array in pairs (fz::silu2): bit-identical to silu() per element
 template <int N>
 __device__ __forceinline__ void silu_n(float (&v)[N]) {
     static_assert(N % 2 == 0, "pairs");
