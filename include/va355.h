@@ -405,6 +405,10 @@ int va_seg_upsample2x(void* stream, const void* src, int32_t ld_s, void* dst, in
 #define VA_OP_FORK 8
 #define VA_OP_JOIN 9
 #define VA_LANES 4
+/* Token operators (below) as ops: a.x = HOST pointer to the operator's argument struct, read during the call. */
+#define VA_OP_TOK_LINEAR 10
+#define VA_OP_TOK_QK 11
+#define VA_OP_TOK_ATTN 12
 typedef struct va_seg_op {
     int32_t kind;
     int32_t lane; /* 0 = the calling stream; 1 .. VA_LANES - 1 (see VA_OP_FORK) */
@@ -536,8 +540,94 @@ int va_post_select_masks(void* stream, const va_mask_select_args* m);
  * poly_n [B][max_det] points (truncated to poly_cap). */
 int va_post_polygons(void* stream, const va_post_args* p, float* polys, int32_t* poly_n, int32_t poly_cap);
 
+/* ---------------------------------------------------------------- token operators */
+/* One attention layer over the tokens of camera frames -- the layers a transformer block beside the convolutional
+ * network needs: a matrix product with its epilogue, the norms and the rotation of queries and keys, attention with a
+ * sliding window and first tokens that stay visible.  Forward only, as every layer of this library.  They take
+ * VA_DTYPE_BF16 or VA_DTYPE_F32 tensors; sums, norms and softmax statistics are float.  Every pointer is a device
+ * pointer of the stream's device; sizes of zero are allowed where noted and launch nothing.  A caller may put them
+ * into the op list of va_seg_run (VA_OP_TOK_*). */
+
+#define VA_ACT_NONE 0
+#define VA_ACT_SILU 1
+#define VA_ACT_GELU 2       /* x Phi(x) */
+#define VA_ACT_GELU_TANH 3  /* its tanh form */
+#define VA_ACT_RELU 4
+
+/* y[m][n] = act(sum_k x[m][k] w[n][k] + bias[n]) + res[m][n], m < M, n < N.  M = 0 writes nothing.
+ * y must not overlap x or w; it may be res itself (same pointer and stride). */
+typedef struct va_tok_linear_args {
+    const void* x;          /* [M][K] dtype, rows ldx elements apart */
+    const void* w;          /* packed weights, 16-byte aligned, zeros from row N and column K on, Kpad % 64 == 0,
+                               Npad % 64 == 0:
+                               BF16: bf16 [Npad][Kpad];  F32 (six exact term products each, float sums; values below bf16's largest, 3.38e38, in
+                               size): three exact bf16 terms [Npad][Kpad / 8][3][8] (the 8 h,
+                               then the 8 m, then the 8 l of a group: va_conv_args.w3 with K in its own order);
+                               w8 = 1 (BF16): e4m3 bytes [Npad][Kpad], in va_conv_args.w8's order inside a 64-block */
+    const float* wscale;    /* w8: [Npad] scale of each row, else NULL */
+    const float* bias;      /* [N] or NULL */
+    const void* res;        /* [M][N] dtype, rows ldr elements apart, or NULL */
+    void* y;                /* [M][N] dtype (float when out_f32), rows ldy elements apart */
+    int64_t ldx, ldr, ldy;
+    int32_t M, N, K, Npad, Kpad;
+    int32_t dtype, w8, act, out_f32;
+    int32_t pad;
+} va_tok_linear_args;
+int va_tok_linear(void* stream, const va_tok_linear_args* a);
+
+/* Norm of each head's vector, x / sqrt(mean(x^2) + eps) * weight, then the rotation of its first `rot` values by the
+ * token's position on one or more axes (time, height, width), for the Hq query heads and the Hk key heads of B x S
+ * tokens.  Pair f (f < rot / 2) is turned by 2 pi turns[f] pos[axis[f]]: values f and f + rot / 2 of the head
+ * (layout 0) or 2 f and 2 f + 1 (layout 1); the angle is formed in float64, so far positions keep their accuracy.
+ * Stored once, rounded once.
+ * With slots > 0 keys and values go into a stream's cache: token s of sequence b stands at position p = kv_len[b] -
+ * q_len[b] + s and is kept in slot p (p < sinks) or sinks + (p - sinks) % (slots - sinks); of tokens that share a slot
+ * the last one is kept.  Tokens s >= q_len[b] are not read, and nothing is written for them.
+ * q_out may be q itself and k_out k itself (same strides). */
+typedef struct va_tok_qk_args {
+    const void *q, *k, *v;      /* [B][S][Hq or Hk][D] dtype, D contiguous; v: [..][Hk][Dv], only with slots > 0 */
+    void *q_out, *k_out, *v_out; /* [B][S][Hq][D]; [B][S][Hk][D] or the cache [B][slots][Hk][D]; [B][slots][Hk][Dv] */
+    /* strides in elements: sequence, token (or slot), head */
+    int64_t q_sb, q_ss, q_sh, k_sb, k_ss, k_sh, v_sb, v_ss, v_sh;
+    int64_t qo_sb, qo_ss, qo_sh, ko_sb, ko_ss, ko_sh, vo_sb, vo_ss, vo_sh;
+    const float *q_weight, *k_weight; /* [D], or NULL: that norm is left out */
+    float eps;
+    int32_t rot;                /* rotated values of a head: even, <= D; 0: no rotation */
+    const double* turns;        /* [rot / 2] turns per position (frequency / 2 pi) */
+    const int32_t* axis;        /* [rot / 2] index of the position that turns the pair */
+    const int32_t* pos;         /* [B][S][axes] */
+    int64_t pos_sb, pos_ss;
+    const int32_t *q_len, *kv_len; /* [B] or NULL: q_len = S; kv_len (only with slots > 0) = q_len */
+    int32_t B, S, Hq, Hk, D, Dv, axes, layout, slots, sinks, dtype, pad;
+} va_tok_qk_args;
+int va_tok_qk(void* stream, const va_tok_qk_args* a);
+
+/* Attention of B x S queries (Hq heads) over `slots` cached keys and values (Hk heads, Hq % Hk == 0; query head h reads
+ * key head h / (Hq / Hk)).  Query s of sequence b stands at position i = kv_len[b] - q_len[b] + s; its frame ends at
+ * e = (i / frame + 1) * frame (frame 0, with window and sinks 0: no end), and it sees the keys at positions j < min(e, kv_len[b]) with j < sinks
+ * or j >= e - window (window 0: no limit): frame 1 is causal attention token by token, frame = tokens of an image lets
+ * the tokens of one image see each other.  Position j is held in slot j (j < sinks) or sinks + (j - sinks) %
+ * (slots - sinks); positions that later ones have overwritten are not seen.  A query that sees nothing gets zeros; for
+ * s >= q_len[b] nothing is written.  A key that a query does not see has no part in its result, whatever it holds.
+ * out = softmax(scale q k) v, the probabilities rounded to bf16 for the second product when dtype is BF16.
+ * ws: va_tok_attn_workspace_bytes(a) bytes, written and read within the call only (calls that may run at the same time
+ * need one each). */
+typedef struct va_tok_attn_args {
+    const void *q, *k, *v;      /* [B][S][Hq][D], [B][slots][Hk][D], [B][slots][Hk][Dv]: D, Dv contiguous, % 8 == 0, <= 128 */
+    void* o;                    /* [B][S][Hq][Dv] dtype */
+    int64_t q_sb, q_ss, q_sh, k_sb, k_ss, k_sh, v_sb, v_ss, v_sh, o_sb, o_ss, o_sh; /* strides in elements, % 8 == 0 */
+    const int32_t *q_len, *kv_len; /* [B] or NULL: S; slots */
+    float scale;
+    int32_t B, S, Hq, Hk, D, Dv, slots, frame, window, sinks, dtype;
+    void* ws;
+    int64_t ws_bytes;
+} va_tok_attn_args;
+int64_t va_tok_attn_workspace_bytes(const va_tok_attn_args* a);
+int va_tok_attn(void* stream, const va_tok_attn_args* a);
+
 /* ABI self-check: writes sizeof() of va_nav_dims, va_frame_hdr, va_query_hdr, va_conv_args, va_seg_op,
- * va_cand, va_det, va_mask_stat, va_post_args, va_contour_stat, va_mask_select_args (in that order) into
+ * va_cand, va_det, va_mask_stat, va_post_args, va_contour_stat, va_mask_select_args, va_tok_linear_args, va_tok_qk_args,
+ * va_tok_attn_args (in that order) into
  * out[0..n-1]; returns how many. */
 int va_abi_struct_sizes(int64_t* out, int32_t n);
 

@@ -86,6 +86,10 @@ SIGNATURES = [
     ("va_post_select_masks", I32, [P, P]),
     ("va_post_polygons", I32, [P, P, P, P, I32]),
     ("va_letterbox", I32, [P, P, I32, I32, I32, P, I32, I32, I32, I32, I32, I32]),
+    ("va_tok_linear", I32, [P, P]),
+    ("va_tok_qk", I32, [P, P]),
+    ("va_tok_attn_workspace_bytes", I64, [P]),
+    ("va_tok_attn", I32, [P, P]),
     ("va_abi_struct_sizes", I32, [P, I32]),
     ("va_diag", I32, [P, I32, I32]),
     ("va_switches_reload", I32, []),

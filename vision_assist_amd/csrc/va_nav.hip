@@ -1177,7 +1177,8 @@ int va_abi_struct_sizes(int64_t* out, int32_t n) {
     const int64_t sz[] = {(int64_t)sizeof(va_nav_dims), (int64_t)sizeof(va_frame_hdr), (int64_t)sizeof(va_query_hdr),
                           (int64_t)sizeof(va_conv_args), (int64_t)sizeof(va_seg_op),    (int64_t)sizeof(va_cand),
                           (int64_t)sizeof(va_det),       (int64_t)sizeof(va_mask_stat), (int64_t)sizeof(va_post_args),
-                          (int64_t)sizeof(va_contour_stat), (int64_t)sizeof(va_mask_select_args)};
+                          (int64_t)sizeof(va_contour_stat), (int64_t)sizeof(va_mask_select_args),
+                          (int64_t)sizeof(va_tok_linear_args), (int64_t)sizeof(va_tok_qk_args), (int64_t)sizeof(va_tok_attn_args)};
     int k = (int)(sizeof sz / sizeof sz[0]);
     if (!out) return k;
     for (int i = 0; i < n && i < k; ++i) out[i] = sz[i];

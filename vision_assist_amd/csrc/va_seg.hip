@@ -4418,6 +4418,15 @@ int va_seg_run(void* stream, const va_seg_op* ops, int32_t n) {
             case VA_OP_STEM:
                 rc = a.dtype == VA_DTYPE_F32 ? va_seg_stem_f32(st, &a) : va_seg_stem(st, &a);
                 break;
+            case VA_OP_TOK_LINEAR:
+                rc = va_tok_linear(st, (const va_tok_linear_args*)a.x);
+                break;
+            case VA_OP_TOK_QK:
+                rc = va_tok_qk(st, (const va_tok_qk_args*)a.x);
+                break;
+            case VA_OP_TOK_ATTN:
+                rc = va_tok_attn(st, (const va_tok_attn_args*)a.x);
+                break;
             default:
                 rc = VA_ERR_ARG;
         }

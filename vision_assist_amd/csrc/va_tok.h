@@ -1,0 +1,76 @@
+// va_tok.h -- shared device helpers of the token operators (va_tok_linear.hip, va_tok_qk.hip, va_tok_attn.hip): vector
+// types, bf16 conversions, the exact three-term split of a float, activations.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/va355.h"
+
+namespace tok {
+
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+typedef __attribute__((ext_vector_type(2))) float f32x2;
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(2))) unsigned int u32x2;
+typedef __attribute__((ext_vector_type(4))) unsigned int u32x4;
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+typedef __attribute__((address_space(1))) void gvoid_t;
+typedef __attribute__((address_space(3))) void lvoid_t;
+
+// consecutive workgroups go to the 8 XCDs in turn: the i-th workgroup of an XCD takes the i-th tile of a contiguous
+// run, so that neighbouring tiles (which read the same operand rows) share that XCD's L2
+__device__ __forceinline__ int xcd_tile(int bid, int ntiles) {
+    const int q = ntiles / 8, r = ntiles % 8, x = bid % 8, j = bid / 8;
+    return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + j;
+}
+
+// two floats -> packed bf16 (round to nearest even)
+__device__ __forceinline__ unsigned pk_bf16(float a, float b) {
+    return __builtin_bit_cast(unsigned, (bf16x2){(__bf16)a, (__bf16)b});
+}
+__device__ __forceinline__ float bf_lo(unsigned u) { return __uint_as_float(u << 16); }
+__device__ __forceinline__ float bf_hi(unsigned u) { return __uint_as_float(u & 0xffff0000u); }
+
+// e4m3 bytes -> bf16, exact (every e4m3 value is a bf16 value)
+__device__ __forceinline__ bf16x8 e4m3x8(uint2 q) {
+    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)q.x, 1.0f, false);
+    const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)q.x, 1.0f, true);
+    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)q.y, 1.0f, false);
+    const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)q.y, 1.0f, true);
+    return (bf16x8){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// x = h + m + l exactly, each the round-to-nearest bf16 of what remains (x - h and x - h - m are exact in float: the
+// remainders have at most 16 and 8 significant bits).  Six of the nine term products (hh, hm, mh, hl, mm, lh) keep a
+// float product to 2^-26 of |a b|: |m| <= 2^-9 |x|, |l| <= 2^-18 |x|.
+__device__ __forceinline__ void split3(const float (&x)[8], bf16x8 (&t)[3]) {
+    unsigned w[3][4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        float a = x[2 * e], b = x[2 * e + 1];
+        w[0][e] = pk_bf16(a, b);
+        a -= bf_lo(w[0][e]), b -= bf_hi(w[0][e]);
+        w[1][e] = pk_bf16(a, b);
+        a -= bf_lo(w[1][e]), b -= bf_hi(w[1][e]);
+        w[2][e] = pk_bf16(a, b);
+    }
+#pragma unroll
+    for (int k = 0; k < 3; ++k) t[k] = __builtin_bit_cast(bf16x8, (u32x4){w[k][0], w[k][1], w[k][2], w[k][3]});
+}
+
+// x Phi(x) = x erfc(-x / sqrt 2) / 2 (the erfc form keeps the left tail's relative accuracy); the tanh form as
+// x / (1 + exp(-2 u)), the same function
+__device__ __forceinline__ float activate(float x, int act) {
+    switch (act) {
+        case VA_ACT_SILU: return x / (1.0f + expf(-x));
+        case VA_ACT_GELU: return 0.5f * x * erfcf(-0.70710678118654752f * x);
+        case VA_ACT_GELU_TANH: return x / (1.0f + expf(-1.5957691216057308f * (x + 0.044715f * x * x * x)));
+        case VA_ACT_RELU: return x < 0.0f ? 0.0f : x;
+        default: return x;
+    }
+}
+
+}  // namespace tok
