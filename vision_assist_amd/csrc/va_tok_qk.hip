@@ -10,6 +10,7 @@ namespace {
 using namespace tok;
 
 constexpr int QK_WAVES = 4, QK_PAIRS = 128;  // D <= 256
+constexpr int QK_U = 4;
 
 template <typename T, int P>
 __device__ __forceinline__ void load_p(const T* p, float (&v)[P]) {
@@ -104,6 +105,7 @@ __global__ __launch_bounds__(64 * QK_WAVES) void qk_kernel(va_tok_qk_args a, int
     __syncthreads();
     if (!live) return;
     const int hpw = 64 / lph, sub = lane / lph, c0 = lane - sub * lph, npair = (a.D + 1) / 2;
+    constexpr int U = P == 1 ? 1 : QK_U;
     const int heads = a.Hq + a.Hk, groups = (heads + hpw - 1) / hpw;
     const float inv_d = 1.0f / (float)a.D;
     int lo[IT], hi[IT];
@@ -129,61 +131,72 @@ __global__ __launch_bounds__(64 * QK_WAVES) void qk_kernel(va_tok_qk_args a, int
             }
         }
     }
-    for (int g = part; g < groups; g += parts) {
-        const int h = g * hpw + sub;
-        const bool isq = h < a.Hq, mine = h < heads;
-        const T* src = isq ? (const T*)a.q + b * a.q_sb + s * a.q_ss + h * a.q_sh
-                           : (const T*)a.k + b * a.k_sb + s * a.k_ss + (h - a.Hq) * a.k_sh;
-        float x[IT][P], y[IT][P], sum = 0.0f;
+    for (int g0 = part; g0 < groups; g0 += parts * U) {
+        // U groups of heads are read before the first is stored: a wave's loads in flight, not its latency, set the rate
+        float x[U][IT][P], y[U][IT][P];
 #pragma unroll
-        for (int i = 0; i < IT; ++i) {
+        for (int u = 0; u < U; ++u) {
+            const int h = (g0 + u * parts) * hpw + sub;
+            const bool isq = h < a.Hq, mine = h < heads;
+            const T* src = isq ? (const T*)a.q + b * a.q_sb + s * a.q_ss + h * a.q_sh
+                               : (const T*)a.k + b * a.k_sb + s * a.k_ss + (h - a.Hq) * a.k_sh;
 #pragma unroll
-            for (int p = 0; p < P; ++p) x[i][p] = y[i][p] = 0.0f;
-            if (mine && on[i]) {
+            for (int i = 0; i < IT; ++i) {
+#pragma unroll
+                for (int p = 0; p < P; ++p) x[u][i][p] = y[u][i][p] = 0.0f;
+                if (!mine || !on[i]) continue;
                 if constexpr (P == 1) {
-                    load_p<T, 1>(src + lo[i], x[i]);
-                    if (hi[i] >= 0) load_p<T, 1>(src + hi[i], y[i]);
+                    load_p<T, 1>(src + lo[i], x[u][i]);
+                    if (hi[i] >= 0) load_p<T, 1>(src + hi[i], y[u][i]);
                 } else if (a.layout) {
                     float t[2 * P];
                     load_p<T, 2 * P>(src + lo[i], t);
 #pragma unroll
-                    for (int p = 0; p < P; ++p) x[i][p] = t[2 * p], y[i][p] = t[2 * p + 1];
+                    for (int p = 0; p < P; ++p) x[u][i][p] = t[2 * p], y[u][i][p] = t[2 * p + 1];
                 } else {
-                    load_p<T, P>(src + lo[i], x[i]);
-                    load_p<T, P>(src + hi[i], y[i]);
+                    load_p<T, P>(src + lo[i], x[u][i]);
+                    load_p<T, P>(src + hi[i], y[u][i]);
                 }
             }
-#pragma unroll
-            for (int p = 0; p < P; ++p) sum += x[i][p] * x[i][p] + y[i][p] * y[i][p];
         }
-        for (int d = 1; d < lph; d <<= 1) sum += __shfl_xor(sum, d);
-        const bool normed = isq ? a.q_weight != nullptr : a.k_weight != nullptr;
-        const float inv = normed ? 1.0f / sqrtf(sum * inv_d + a.eps) : 1.0f;
-        if (!mine || (!isq && !keep)) continue;
-        T* dst = isq ? (T*)a.q_out + b * a.qo_sb + s * a.qo_ss + h * a.qo_sh
-                     : (T*)a.k_out + b * a.ko_sb + (int64_t)slot * a.ko_ss + (h - a.Hq) * a.ko_sh;
 #pragma unroll
-        for (int i = 0; i < IT; ++i) {
-            if (!on[i]) continue;
-            float u[P], v[P];
+        for (int u = 0; u < U; ++u) {
+            const int h = (g0 + u * parts) * hpw + sub;
+            const bool isq = h < a.Hq, mine = h < heads;
+            float sum = 0.0f;
 #pragma unroll
-            for (int p = 0; p < P; ++p) {
-                const float l = x[i][p] * inv * (isq ? wl[0][i][p] : wl[1][i][p]);
-                const float r = y[i][p] * inv * (isq ? wh[0][i][p] : wh[1][i][p]);
-                u[p] = l * cc[i][p] - r * ss[i][p];
-                v[p] = r * cc[i][p] + l * ss[i][p];
-            }
-            if constexpr (P == 1) {
-                store_p<T, 1>(dst + lo[i], u);
-                if (hi[i] >= 0) store_p<T, 1>(dst + hi[i], v);
-            } else if (a.layout) {
-                float t[2 * P];
+            for (int i = 0; i < IT; ++i)
 #pragma unroll
-                for (int p = 0; p < P; ++p) t[2 * p] = u[p], t[2 * p + 1] = v[p];
-                store_p<T, 2 * P>(dst + lo[i], t);
-            } else {
-                store_p<T, P>(dst + lo[i], u);
-                store_p<T, P>(dst + hi[i], v);
+                for (int p = 0; p < P; ++p) sum += x[u][i][p] * x[u][i][p] + y[u][i][p] * y[u][i][p];
+            for (int d = 1; d < lph; d <<= 1) sum += __shfl_xor(sum, d);
+            const bool normed = isq ? a.q_weight != nullptr : a.k_weight != nullptr;
+            const float inv = normed ? 1.0f / sqrtf(sum * inv_d + a.eps) : 1.0f;
+            if (!mine || (!isq && !keep)) continue;
+            T* dst = isq ? (T*)a.q_out + b * a.qo_sb + s * a.qo_ss + h * a.qo_sh
+                         : (T*)a.k_out + b * a.ko_sb + (int64_t)slot * a.ko_ss + (h - a.Hq) * a.ko_sh;
+#pragma unroll
+            for (int i = 0; i < IT; ++i) {
+                if (!on[i]) continue;
+                float l[P], r[P];
+#pragma unroll
+                for (int p = 0; p < P; ++p) {
+                    const float m = x[u][i][p] * inv * (isq ? wl[0][i][p] : wl[1][i][p]);
+                    const float n = y[u][i][p] * inv * (isq ? wh[0][i][p] : wh[1][i][p]);
+                    l[p] = m * cc[i][p] - n * ss[i][p];
+                    r[p] = n * cc[i][p] + m * ss[i][p];
+                }
+                if constexpr (P == 1) {
+                    store_p<T, 1>(dst + lo[i], l);
+                    if (hi[i] >= 0) store_p<T, 1>(dst + hi[i], r);
+                } else if (a.layout) {
+                    float t[2 * P];
+#pragma unroll
+                    for (int p = 0; p < P; ++p) t[2 * p] = l[p], t[2 * p + 1] = r[p];
+                    store_p<T, 2 * P>(dst + lo[i], t);
+                } else {
+                    store_p<T, P>(dst + lo[i], l);
+                    store_p<T, P>(dst + hi[i], r);
+                }
             }
         }
     }
@@ -216,6 +229,18 @@ bool qk_ok(const va_tok_qk_args& a) {
     return true;
 }
 
+// whether every lane's P pairs can be read and written as vectors: 8 bytes of each half (layout 0) or 16 bytes (1); the
+// values of a cached token in 16 bytes
+bool qk_wide(const va_tok_qk_args& a) {
+    const int e = a.dtype == VA_DTYPE_F32 ? 4 : 2, P = 8 / e, n = a.layout ? 2 * P : P;
+    if (a.D % (2 * P) || (a.rot / 2) % P || ((a.D - a.rot) / 2) % P) return false;
+    int64_t st = a.q_sb | a.q_ss | a.q_sh | a.k_sb | a.k_ss | a.k_sh | a.qo_sb | a.qo_ss | a.qo_sh | a.ko_sb | a.ko_ss | a.ko_sh;
+    if (st % n || (((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.q_out | (uintptr_t)a.k_out) & (uintptr_t)(n * e - 1))) return false;
+    if (!a.slots) return true;
+    st = a.v_sb | a.v_ss | a.v_sh | a.vo_sb | a.vo_ss | a.vo_sh | a.Dv;
+    return st % (16 / e) == 0 && !(((uintptr_t)a.v | (uintptr_t)a.v_out) & 15);
+}
+
 }  // namespace
 
 extern "C" int va_tok_qk(void* stream, const va_tok_qk_args* ap) {
@@ -224,13 +249,24 @@ extern "C" int va_tok_qk(void* stream, const va_tok_qk_args* ap) {
     if (a.B == 0 || a.S == 0 || a.Hq + a.Hk == 0) return VA_OK;
     const bool f32 = a.dtype == VA_DTYPE_F32;
     const int64_t tokens = (int64_t)a.B * a.S;
-    const int64_t blocks = (tokens + QK_WAVES - 1) / QK_WAVES;
+    const bool wide = qk_wide(a);
+    const int P = wide ? (f32 ? 2 : 4) : 1;
+    int lph = 64;  // lanes of a head: a power of two that holds its pairs
+    while (wide && lph > 1 && (lph / 2) * P >= a.D / 2) lph /= 2;
+    // few tokens: a token's heads over several waves, up to eight waves for each of the 256 CUs
+    const int groups = (a.Hq + a.Hk + 64 / lph - 1) / (64 / lph);
+    const int parts = (int)max((int64_t)1, min((int64_t)groups, 2048 / tokens));
+    const int64_t blocks = (tokens * parts + QK_WAVES - 1) / QK_WAVES;
     if (blocks > INT32_MAX) return VA_ERR_RANGE;
     const dim3 grid((unsigned)blocks), block(64 * QK_WAVES);
     hipStream_t st = (hipStream_t)stream;
-    if (f32)
-        hipLaunchKernelGGL((qk_kernel<float, 1, 2>), grid, block, 0, st, a, 64, 1);
+    if (f32 && wide)
+        hipLaunchKernelGGL((qk_kernel<float, 2, 1>), grid, block, 0, st, a, lph, parts);
+    else if (f32)
+        hipLaunchKernelGGL((qk_kernel<float, 1, 2>), grid, block, 0, st, a, lph, parts);
+    else if (wide)
+        hipLaunchKernelGGL((qk_kernel<__bf16, 4, 1>), grid, block, 0, st, a, lph, parts);
     else
-        hipLaunchKernelGGL((qk_kernel<__bf16, 1, 2>), grid, block, 0, st, a, 64, 1);
+        hipLaunchKernelGGL((qk_kernel<__bf16, 1, 2>), grid, block, 0, st, a, lph, parts);
     return hipGetLastError() == hipSuccess ? VA_OK : VA_ERR_HIP;
 }

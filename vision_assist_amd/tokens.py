@@ -17,6 +17,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import math
+import struct
 
 import torch
 
@@ -52,6 +53,14 @@ class AttnArgs(ctypes.Structure):  # va_tok_attn_args
                [("ws", VOIDP), ("ws_bytes", I64)]
 
 
+# the same layouts for a call's own use: one pack() of plain numbers is a fraction of a ctypes structure's fields, and
+# small calls are bound by the host
+LINEAR_PACK = struct.Struct("@6P3q10i")
+QK_PACK = struct.Struct("@6P18q2Pfi3P2q2P12i")
+ATTN_PACK = struct.Struct("@4P12q2Pf11iPq")
+assert (LINEAR_PACK.size, QK_PACK.size, ATTN_PACK.size) == tuple(ctypes.sizeof(t) for t in (LinearArgs, QKArgs, AttnArgs))
+
+
 # ------------------------------------------------------------------ what every call checks
 def _need(ok: bool, what: str) -> None:
     if not ok:
@@ -67,6 +76,9 @@ def _on(t: torch.Tensor, dev: torch.device, dtype, name: str) -> None:
 
 def _range(t: torch.Tensor) -> tuple[int, int]:
     """The bytes between a tensor's first and last element (0, 0: it has none)."""
+    if t.is_contiguous():
+        at = t.data_ptr()
+        return at, at + t.numel() * t.element_size()
     if t.numel() == 0:
         return 0, 0
     last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
@@ -91,12 +103,15 @@ def _interleaved(x: torch.Tensor, y: torch.Tensor) -> bool:
     return False
 
 
+def _meet(x: tuple[int, int], y: tuple[int, int]) -> bool:
+    return x[0] < y[1] and y[0] < x[1]
+
+
 def _apart(out: torch.Tensor, t: torch.Tensor | None, name: str, same_ok: bool = False) -> None:
     """Refuses an output that overlaps an input (same_ok: unless it is that very tensor)."""
     if t is None:
         return
-    (a, b), (c, d) = _range(out), _range(t)
-    if a < d and c < b and not (same_ok and out.data_ptr() == t.data_ptr() and out.shape == t.shape and
+    if _meet(_range(out), _range(t)) and not (same_ok and out.data_ptr() == t.data_ptr() and out.shape == t.shape and
                                 out.stride() == t.stride() and out.dtype == t.dtype) \
             and not _interleaved(out, t):
         raise _lib.VaError(f"the output overlaps {name}")
@@ -104,40 +119,35 @@ def _apart(out: torch.Tensor, t: torch.Tensor | None, name: str, same_ok: bool =
 
 def _own_elements(out: torch.Tensor) -> None:
     """Refuses an output whose elements share memory (an expanded tensor)."""
+    if out.is_contiguous():
+        return
     at = 1
     for s, n in sorted((s, n) for n, s in zip(out.shape, out.stride()) if n > 1):
         _need(s >= at, "the output's elements overlap")
         at = s * n
 
 
-class _Launch:
-    """The device and stream of one call; what it allocates inside belongs to that stream."""
+_raw_stream, _device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
-    def __init__(self, dev: torch.device, stream, inputs):
-        self.scope = None
-        if dev.type != "cuda":
-            raise _lib.VaError(f"the token operators need tensors on the GPU, not on {dev}")
-        if stream is None:
-            if dev.index != torch.cuda.current_device():
-                self.scope = torch.cuda.device(dev)
-                self.scope.__enter__()
-            self.ptr = torch.cuda.current_stream(dev).cuda_stream
-            return
-        self.ptr = _lib.stream_ptr(stream, dev)
-        self.scope = contextlib.ExitStack()
-        self.scope.enter_context(torch.cuda.device(dev))
-        self.scope.enter_context(torch.cuda.stream(stream))
-        for t in inputs:
-            if t is not None:
-                t.record_stream(stream)
 
-    def __enter__(self):
-        return self
+def _elsewhere(dev: torch.device, stream, inputs, go):
+    """go() on a device that is not the current one, or on a stream of the caller's: what it allocates belongs to that
+    stream, and its inputs are recorded on it."""
+    if dev.type != "cuda":
+        raise _lib.VaError(f"the token operators need tensors on the GPU, not on {dev}")
+    with contextlib.ExitStack() as scope:
+        scope.enter_context(torch.cuda.device(dev))
+        if stream is not None:
+            _lib.stream_ptr(stream, dev)  # refuses a stream of another device
+            scope.enter_context(torch.cuda.stream(stream))
+            for t in inputs:
+                if t is not None:
+                    t.record_stream(stream)
+        return go()
 
-    def __exit__(self, *exc):
-        if self.scope is not None:
-            self.scope.__exit__(*exc)
-        return False
+
+def _here(dev: torch.device, stream) -> bool:
+    return stream is None and dev.type == "cuda" and dev.index == _device()
 
 
 # ------------------------------------------------------------------ matrix product
@@ -192,57 +202,68 @@ class Linear:
         else:
             self.w = padded(w.to(torch.bfloat16))
         self.bias = None if bias is None else bias.detach().to(self.device, torch.float32).contiguous()
-        self._args = LinearArgs(w=self.w.data_ptr(), wscale=self.wscale.data_ptr() if self.wscale is not None else None,
-                                bias=self.bias.data_ptr() if bias is not None else None, N=N, K=K, Npad=Np, Kpad=Kp,
-                                dtype=VA_DTYPE_F32 if dtype == "f32" else VA_DTYPE_BF16, w8=int(dtype == "w8a16"),
-                                act=ACTS[act])
+        self._ptrs = (self.w.data_ptr(), self.wscale.data_ptr() if self.wscale is not None else 0,
+                      self.bias.data_ptr() if bias is not None else 0)
+        self._ints = (N, K, Np, Kp, VA_DTYPE_F32 if dtype == "f32" else VA_DTYPE_BF16, int(dtype == "w8a16"), ACTS[act])
 
     def args(self, x: torch.Tensor, out: torch.Tensor, residual: torch.Tensor | None = None) -> LinearArgs:
         """The va_tok_linear_args of a call on [M, K] rows (for an op list: VA_OP_TOK_LINEAR); they point into these
         tensors, which the caller keeps."""
-        a = LinearArgs.from_buffer_copy(self._args)
-        a.x, a.y, a.M = x.data_ptr(), out.data_ptr(), x.shape[0]
-        one = a.M <= 1  # a single row's stride says nothing
-        a.ldx, a.ldy = self.K if one else x.stride(0), self.N if one else out.stride(0)
-        if residual is not None:
-            a.res, a.ldr = residual.data_ptr(), self.N if one else residual.stride(0)
-        a.out_f32 = int(out.dtype == torch.float32 and self.tdtype != torch.float32)
-        return a
+        return LinearArgs.from_buffer_copy(self._pack(x, out, residual))
+
+    def _pack(self, x, out, residual) -> bytes:
+        M, N = x.shape[0], self.N
+        one = M <= 1  # a single row's stride says nothing
+        return LINEAR_PACK.pack(x.data_ptr(), *self._ptrs, 0 if residual is None else residual.data_ptr(), out.data_ptr(),
+                                self.K if one else x.stride(0), N if one or residual is None else residual.stride(0),
+                                N if one else out.stride(0), M, *self._ints, out.dtype != self.tdtype, 0)
 
     def __call__(self, x: torch.Tensor, residual: torch.Tensor | None = None, out: torch.Tensor | None = None,
                  stream=None) -> torch.Tensor:
         """x [..., K] -> [..., N].  residual [..., N] is added after the activation.  out: bf16 or (for the bf16 forms)
         float; it may be the residual itself, and must not overlap x."""
         _on(x, self.device, self.tdtype, "x")
-        lead = x.shape[:-1]
-        _need(x.dim() >= 1 and x.shape[-1] == self.K, f"x {tuple(x.shape)}: [..., {self.K}]")
-        with _Launch(self.device, stream, (x, residual, out, self.w)) as at:
-            x2 = self._rows(x, self.K)
-            _need(x2.shape[0] <= I32_MAX, "more rows than 32 bits count")
-            r2 = None
-            if residual is not None:
-                _on(residual, self.device, self.tdtype, "residual")
-                _need(residual.shape == (*lead, self.N), f"residual {tuple(residual.shape)}: {(*lead, self.N)}")
-                r2 = self._rows(residual, self.N)
-            if out is None:
-                out = torch.empty((*lead, self.N), dtype=self.tdtype, device=self.device)
-                o2 = out.view(-1, self.N)
-            else:
-                _need(out.dtype in (self.tdtype, torch.float32), f"out is {out.dtype}")
-                _on(out, self.device, out.dtype, "out")
-                _need(out.shape == (*lead, self.N), f"out {tuple(out.shape)}: {(*lead, self.N)}")
-                _own_elements(out)
-                try:
-                    o2 = out.view(-1, self.N) if out.numel() else out.reshape(-1, self.N)
-                except RuntimeError:
-                    o2 = None
-                _need(o2 is not None and (self.N == 1 or o2.numel() == 0 or o2.stride(1) == 1),
-                      "out: rows of a common stride with contiguous values")
-                _apart(o2, x, "x")
-                _apart(o2, r2, "the residual", same_ok=True)
-            if x2.shape[0]:
-                _lib.check(self.lib.va_tok_linear(at.ptr, ctypes.byref(self.args(x2, o2, r2))), "va_tok_linear")
+        if not _here(self.device, stream):
+            return _elsewhere(self.device, stream, (x, residual, out, self.w), lambda: self(x, residual, out))
+        shape = x.shape
+        if len(shape) == 0 or shape[-1] != self.K:
+            raise _lib.VaError(f"x {tuple(shape)}: [..., {self.K}]")
+        want = (*shape[:-1], self.N)
+        x2 = self._rows(x, self.K)
+        if x2.shape[0] > I32_MAX:
+            raise _lib.VaError("more rows than 32 bits count")
+        r2 = None
+        if residual is not None:
+            _on(residual, self.device, self.tdtype, "residual")
+            if residual.shape != want:
+                raise _lib.VaError(f"residual {tuple(residual.shape)}: {want}")
+            r2 = self._rows(residual, self.N)
+        if out is None:
+            out = x.new_empty(want)
+            o2 = out if len(want) == 2 else out.view(-1, self.N) if x2.shape[0] else out
+        else:
+            o2 = self._given(out, want, x, r2)
+        if x2.shape[0]:
+            rc = self.lib.va_tok_linear(_raw_stream(self.device.index), self._pack(x2, o2, r2))
+            if rc:
+                _lib.check(rc, "va_tok_linear")
         return out
+
+    def _given(self, out, want, x, r2):
+        """The caller's output as rows."""
+        _need(out.dtype in (self.tdtype, torch.float32), f"out is {out.dtype}")
+        _on(out, self.device, out.dtype, "out")
+        _need(out.shape == want, f"out {tuple(out.shape)}: {want}")
+        _own_elements(out)
+        try:
+            o2 = out.view(-1, self.N) if out.numel() else out.reshape(0, self.N)
+        except RuntimeError:
+            o2 = None
+        _need(o2 is not None and (self.N == 1 or o2.numel() == 0 or o2.stride(1) == 1),
+              "out: rows of a common stride with contiguous values")
+        _apart(o2, x, "x")
+        _apart(o2, r2, "the residual", same_ok=True)
+        return o2
 
     @staticmethod
     def _rows(x: torch.Tensor, n: int) -> torch.Tensor:
@@ -304,8 +325,13 @@ class TokenCache:
         _need(0 <= sinks < k.shape[1], f"sinks {sinks}: fewer than the {k.shape[1]} slots")
         _on(length, k.device, torch.int32, "length")
         _need(length.shape == (k.shape[0],) and length.is_contiguous(), "length: [B]")
+        _need(k.stride(3) == 1 and v.stride(3) == 1, "k, v: contiguous values")
+        _own_elements(k)
+        _own_elements(v)
+        _apart(k, v, "the values")
         self.k, self.v, self.sinks, self.len = k, v, int(sinks), length
         self.slots = k.shape[1]
+        self._k_range, self._v_range = _range(k), _range(v)
 
     @classmethod
     def of(cls, k: torch.Tensor, v: torch.Tensor, sinks: int = 0, length: torch.Tensor | None = None) -> "TokenCache":
@@ -341,93 +367,93 @@ class QKNorm:
         self.D, self.rotary = head_dim, rotary
         self.wq, self.wk = (None if w is None else w.detach().to(self.device, torch.float32).contiguous()
                             for w in (q_weight, k_weight))
-        a = self._args = QKArgs(D=head_dim, eps=eps)
-        if self.wq is not None:
-            a.q_weight = self.wq.data_ptr()
-        if self.wk is not None:
-            a.k_weight = self.wk.data_ptr()
-        if rotary is not None:
-            a.rot, a.layout, a.turns, a.axis = rotary.dim, LAYOUTS[rotary.layout], rotary.turns.data_ptr(), rotary.axis.data_ptr()
+        self.eps = float(eps)
+        self._norm = (self.wq.data_ptr() if self.wq is not None else 0, self.wk.data_ptr() if self.wk is not None else 0,
+                      self.eps)
+        self._rot = (0, 0, 0) if rotary is None else (rotary.dim, rotary.turns.data_ptr(), rotary.axis.data_ptr())
 
     def __call__(self, q: torch.Tensor, k: torch.Tensor, pos: torch.Tensor | None = None,
                  q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None, stream=None):
         """q [B, S, Hq, D], k [B, S, Hk, D] (any strides with contiguous values, e.g. views of one product's output)
         -> (q', k').  pos: int32 [B, S, axes] ([B, S] for one axis; expanded views are fine).  q_out / k_out may be
         q / k themselves."""
-        with _Launch(self.device, stream, (q, k, pos, q_out, k_out)) as at:
-            a, q, k = self._begin(q, k, pos)
+        if not _here(self.device, stream):
+            return _elsewhere(self.device, stream, (q, k, pos, q_out, k_out), lambda: self(q, k, pos, q_out, k_out))
+        q, k, pos = self._begin(q, k, pos)
+        if q_out is None and k_out is None:
+            q_out, k_out = q.new_empty(q.shape), k.new_empty(k.shape)
+        else:
             q_out, k_out = (self._out(t, like, n) for t, like, n in ((q_out, q, "q_out"), (k_out, k, "k_out")))
-            self._tell(a, q, k, None, q_out, k_out, None)
             _apart(q_out, k, "k")
             _apart(k_out, q, "q")
             _apart(q_out, k_out, "k_out")
-            if q.shape[0] * q.shape[1]:
-                _lib.check(self.lib.va_tok_qk(at.ptr, ctypes.byref(a)), "va_tok_qk")
+        self._launch(q, k, None, pos, q_out, k_out, None, 0, 0, 0, 0)
         return q_out, k_out
 
     def store(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor | None, cache: TokenCache,
               q_len: torch.Tensor | None = None, q_out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
         """The same for the last q_len[b] tokens (default S) of cache.len[b]: -> q', with the keys and values in the
-        cache.  Rows s >= q_len[b] of q_out are left as they were; a token whose slot a later one of the call takes,
-        or whose position is negative, is not kept."""
-        with _Launch(self.device, stream, (q, k, v, pos, q_len, q_out, cache.k, cache.v, cache.len)) as at:
-            a, q, k = self._begin(q, k, pos)
-            B, S, Hk = k.shape[:3]
-            _on(v, self.device, q.dtype, "v")
-            Dv = cache.v.shape[3]
-            _need(v.shape == (B, S, Hk, Dv), f"v {tuple(v.shape)}: {(B, S, Hk, Dv)}")
-            v = v if v.stride(3) == 1 or Dv == 1 else v.contiguous()
-            _on(cache.k, self.device, q.dtype, "the cache")
-            _need(cache.k.shape[0] == B and cache.k.shape[2:] == (Hk, self.D), f"the cache holds {tuple(cache.k.shape)}")
-            _need(cache.k.stride(3) == 1 and cache.v.stride(3) == 1, "the cache's values are not contiguous")
-            _own_elements(cache.k)
-            _own_elements(cache.v)
-            q_out = self._out(q_out, q, "q_out", torch.zeros if q_len is not None else torch.empty)
-            if q_len is not None:
-                _lens(q_len, B, self.device, "q_len")
-                a.q_len = q_len.data_ptr()
-            a.kv_len, a.slots, a.sinks = cache.len.data_ptr(), cache.slots, cache.sinks
-            self._tell(a, q, k, v, q_out, cache.k, cache.v)
-            for t, n in ((cache.k, "the cache's keys"), (cache.v, "the cache's values")):
-                _apart(q_out, t, n)
-                for u, m in ((q, "q"), (k, "k"), (v, "v")):
-                    _apart(t, u, m)
-            _apart(q_out, k, "k")
-            _apart(q_out, v, "v")
-            _apart(cache.k, cache.v, "the cache's values")
-            if B * S:
-                _lib.check(self.lib.va_tok_qk(at.ptr, ctypes.byref(a)), "va_tok_qk")
+        cache.  Rows s >= q_len[b] of q_out are left as they were (zeros where the call makes it); a token whose slot a
+        later one of the call takes, or whose position is negative, is not kept."""
+        if not _here(self.device, stream):
+            return _elsewhere(self.device, stream, (q, k, v, pos, q_len, q_out, cache.k, cache.v, cache.len),
+                              lambda: self.store(q, k, v, pos, cache, q_len, q_out))
+        q, k, pos = self._begin(q, k, pos)
+        B, S, Hk, D = k.shape
+        ck, cv = cache.k, cache.v
+        _on(v, self.device, q.dtype, "v")
+        _on(ck, self.device, q.dtype, "the cache")
+        if v.shape != (B, S, Hk, cv.shape[3]):
+            raise _lib.VaError(f"v {tuple(v.shape)}: {(B, S, Hk, cv.shape[3])}")
+        if ck.shape[0] != B or ck.shape[2] != Hk or ck.shape[3] != D:
+            raise _lib.VaError(f"the cache holds {tuple(ck.shape)}")
+        v = v if v.stride(3) == 1 or v.shape[3] == 1 else v.contiguous()
+        if q_len is not None:
+            _lens(q_len, B, self.device, "q_len")
+        if q_out is None:
+            q_out = (torch.empty if q_len is None else torch.zeros)(q.shape, dtype=q.dtype, device=self.device)
+        else:
+            q_out = self._out(q_out, q, "q_out")
+            out = _range(q_out)
+            for t, n in ((k, "k"), (v, "v"), (ck, "the cache's keys"), (cv, "the cache's values")):
+                if _meet(out, _range(t)):
+                    _apart(q_out, t, n)
+        for t, n in ((q, "q"), (k, "k"), (v, "v")):
+            at = _range(t)
+            for c, r in ((ck, cache._k_range), (cv, cache._v_range)):
+                if _meet(r, at):
+                    _apart(c, t, n)
+        self._launch(q, k, v, pos, q_out, ck, cv, 0 if q_len is None else q_len.data_ptr(), cache.len.data_ptr(),
+                     cache.slots, cache.sinks)
         return q_out
 
     def _begin(self, q, k, pos):
-        a = QKArgs.from_buffer_copy(self._args)
-        _need(q.dim() == 4 and k.dim() == 4 and q.shape[:2] == k.shape[:2] and q.shape[3] == k.shape[3] == self.D,
-              f"q {tuple(q.shape)}, k {tuple(k.shape)}: [B, S, heads, {self.D}]")
-        _need(q.dtype in DTYPES, f"q is {q.dtype}: bfloat16 or float32")
+        if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != self.D or k.shape[3] != self.D:
+            raise _lib.VaError(f"q {tuple(q.shape)}, k {tuple(k.shape)}: [B, S, heads, {self.D}]")
+        if q.dtype not in DTYPES:
+            raise _lib.VaError(f"q is {q.dtype}: bfloat16 or float32")
         _on(q, self.device, q.dtype, "q")
         _on(k, self.device, q.dtype, "k")
-        B, S = q.shape[:2]
-        _need(max(B, S) <= I32_MAX and max(q.shape[2], k.shape[2]) <= 1 << 20, "a side beyond what the kernel counts")
-        q, k = (t if t.stride(3) == 1 or self.D == 1 else t.contiguous() for t in (q, k))
-        a.B, a.S, a.Hq, a.Hk, a.dtype = B, S, q.shape[2], k.shape[2], DTYPES[q.dtype]
-        if self.rotary is not None:
-            n = self.rotary.axes
-            _need(pos is not None, "pos: a rotation needs positions")
-            _on(pos, self.device, torch.int32, "pos")
-            pos = pos.unsqueeze(-1) if pos.dim() == 2 and n == 1 else pos
-            _need(pos.shape == (B, S, n), f"pos {tuple(pos.shape)}: {(B, S, n)}")
-            if n > 1 and pos.stride(2) != 1:
-                pos = pos.contiguous()
-            a.pos, a.pos_sb, a.pos_ss, a.axes = pos.data_ptr(), pos.stride(0), pos.stride(1), n
-            self._hold = None
-        else:
+        if max(q.shape) > I32_MAX or max(q.shape[2], k.shape[2]) > 1 << 20:
+            raise _lib.VaError("a side beyond what the kernel counts")
+        if self.D > 1:
+            q = q if q.stride(3) == 1 else q.contiguous()
+            k = k if k.stride(3) == 1 else k.contiguous()
+        if self.rotary is None:
             _need(pos is None, "pos: there is no rotation")
-        a._keep = (q, k, pos)  # copies live as long as the arguments
-        return a, q, k
+            return q, k, None
+        if pos is None:
+            raise _lib.VaError("pos: a rotation needs positions")
+        _on(pos, self.device, torch.int32, "pos")
+        n = self.rotary.axes
+        pos = pos.unsqueeze(-1) if pos.dim() == 2 and n == 1 else pos
+        if pos.shape != (q.shape[0], q.shape[1], n):
+            raise _lib.VaError(f"pos {tuple(pos.shape)}: {(q.shape[0], q.shape[1], n)}")
+        return q, k, pos if n == 1 or pos.stride(2) == 1 else pos.contiguous()
 
-    def _out(self, t, like, name, new=torch.empty):
+    def _out(self, t, like, name):
         if t is None:
-            return new(like.shape, dtype=like.dtype, device=like.device)
+            return like.new_empty(like.shape)
         _on(t, self.device, like.dtype, name)
         _need(t.shape == like.shape and (t.stride(3) == 1 or self.D == 1),
               f"{name} {tuple(t.shape)}: {tuple(like.shape)} with contiguous values")
@@ -435,30 +461,35 @@ class QKNorm:
         _apart(t, like, "its input", same_ok=True)
         return t
 
-    def _tell(self, a, q, k, v, q_out, k_out, v_out):
-        for n, t in (("q", q), ("k", k), ("v", v)):
-            if t is not None:
-                setattr(a, n, t.data_ptr())
-                for i, d in enumerate(("sb", "ss", "sh")):
-                    setattr(a, f"{n}_{d}", t.stride(i))
-        for n, t in (("q", q_out), ("k", k_out), ("v", v_out)):
-            if t is not None:
-                setattr(a, n + "_out", t.data_ptr())
-                for i, d in enumerate(("sb", "ss", "sh")):
-                    setattr(a, f"{n}o_{d}", t.stride(i))
-        if v is not None:
-            a.Dv = v.shape[3]
+    def _launch(self, q, k, v, pos, q_out, k_out, v_out, q_len, kv_len, slots, sinks):
+        B, S, Hq, D = q.shape
+        if B * S == 0:
+            return
+        rot, turns, axis = self._rot
+        none = (0, 0, 0)
+        a = QK_PACK.pack(
+            q.data_ptr(), k.data_ptr(), 0 if v is None else v.data_ptr(), q_out.data_ptr(), k_out.data_ptr(),
+            0 if v is None else v_out.data_ptr(), *q.stride()[:3], *k.stride()[:3], *(none if v is None else v.stride()[:3]),
+            *q_out.stride()[:3], *k_out.stride()[:3], *(none if v is None else v_out.stride()[:3]), *self._norm, rot, turns, axis,
+            *((0, 0, 0) if pos is None else (pos.data_ptr(), pos.stride(0), pos.stride(1))), q_len, kv_len, B, S, Hq, k.shape[2],
+            D, 0 if v is None else v.shape[3], 0 if pos is None else pos.shape[2],
+            0 if self.rotary is None else LAYOUTS[self.rotary.layout], slots, sinks, DTYPES[q.dtype], 0)
+        rc = self.lib.va_tok_qk(_raw_stream(self.device.index), a)
+        if rc:
+            _lib.check(rc, "va_tok_qk")
 
 
 # ------------------------------------------------------------------ attention
 def _lens(t, B, dev, name):
     _on(t, dev, torch.int32, name)
-    _need(t.shape == (B,) and (B <= 1 or t.stride(0) == 1), f"{name} {tuple(t.shape)}: int32 [{B}]")
+    if t.dim() != 1 or t.shape[0] != B or (B > 1 and t.stride(0) != 1):
+        raise _lib.VaError(f"{name} {tuple(t.shape)}: int32 [{B}]")
 
 
-def _aligned(t: torch.Tensor) -> bool:
-    """Contiguous values, every row 16-byte aligned."""
-    return t.stride(3) == 1 and not (t.stride(0) | t.stride(1) | t.stride(2)) % 8 and not t.data_ptr() & 15
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """t, or a copy of it, with contiguous values and every row 16-byte aligned."""
+    a, b, c, d = t.stride()
+    return t if d == 1 and not (a | b | c) % 8 and not t.data_ptr() & 15 else t.clone(memory_format=torch.contiguous_format)
 
 
 def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float | None = None, frame: int = 1,
@@ -475,53 +506,68 @@ def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float | 
     all of it, slots >= sinks + window + S - 1.  A query that sees nothing gets zeros; rows s >= q_len[b] of out are left
     as they were (zeros where the call makes it).  scale: D ** -0.5 by default, positive.  D and Dv: multiples of 8 up
     to 128."""
-    _need(q.dim() == 4 and k.dim() == 4 and v.dim() == 4, "q [B, S, Hq, D], k [B, slots, Hk, D], v [B, slots, Hk, Dv]")
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+        raise _lib.VaError("q [B, S, Hq, D], k [B, slots, Hk, D], v [B, slots, Hk, Dv]")
     B, S, Hq, D = q.shape
-    slots, Hk, Dv = k.shape[1], k.shape[2], v.shape[3]
-    _need(k.shape == (B, slots, Hk, D) and v.shape == (B, slots, Hk, Dv),
-          f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not fit")
-    _need(Hk > 0 and Hq > 0 and Hq % Hk == 0, f"{Hq} query heads over {Hk} key heads")
-    _need(D % 8 == 0 and 8 <= D <= 128 and Dv % 8 == 0 and 8 <= Dv <= 128, f"D {D}, Dv {Dv}: multiples of 8 up to 128")
-    _need(frame >= 0 and window >= 0 and sinks >= 0 and max(frame, window, sinks) <= I32_MAX,
-          "frame, window and sinks are not negative")
-    _need(frame > 0 or window == sinks == 0, "frame 0 sees everything: no window, no sinks")
-    _need(slots == 0 or sinks < slots, f"sinks {sinks}: fewer than the {slots} slots")
-    _need(max(B, S, slots) <= I32_MAX and S * (Hq // Hk) <= I32_MAX - 256, "a side beyond what the kernel counts")
+    Bk, slots, Hk, Dk = k.shape
+    Bv, vslots, vh, Dv = v.shape
+    if Bk != B or Dk != D or (Bv, vslots, vh) != (Bk, slots, Hk):
+        raise _lib.VaError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not fit")
+    if Hk == 0 or Hq == 0 or Hq % Hk:
+        raise _lib.VaError(f"{Hq} query heads over {Hk} key heads")
+    if D % 8 or not 8 <= D <= 128 or Dv % 8 or not 8 <= Dv <= 128:
+        raise _lib.VaError(f"D {D}, Dv {Dv}: multiples of 8 up to 128")
+    if min(frame, window, sinks) < 0 or max(frame, window, sinks) > I32_MAX:
+        raise _lib.VaError("frame, window and sinks are not negative")
+    if frame == 0 and (window or sinks):
+        raise _lib.VaError("frame 0 sees everything: no window, no sinks")
+    if slots and sinks >= slots:
+        raise _lib.VaError(f"sinks {sinks}: fewer than the {slots} slots")
+    if max(B, S, slots) > I32_MAX or S * (Hq // Hk) > I32_MAX - 256:
+        raise _lib.VaError("a side beyond what the kernel counts")
     scale = D ** -0.5 if scale is None else float(scale)
-    _need(0 < scale < math.inf, f"scale {scale}: positive")
-    _need(q.dtype in DTYPES, f"q is {q.dtype}: bfloat16 or float32")
-    dev = q.device
-    _on(k, dev, q.dtype, "k")
-    _on(v, dev, q.dtype, "v")
+    if not 0 < scale < math.inf:
+        raise _lib.VaError(f"scale {scale}: positive")
+    dev, dtype = q.device, q.dtype
+    if dtype not in DTYPES:
+        raise _lib.VaError(f"q is {dtype}: bfloat16 or float32")
+    _on(k, dev, dtype, "k")
+    _on(v, dev, dtype, "v")
     if q_len is not None:
         _lens(q_len, B, dev, "q_len")
     if kv_len is not None:
         _lens(kv_len, B, dev, "kv_len")
-    lib = _lib.load()
-    with _Launch(dev, stream, (q, k, v, q_len, kv_len, out)) as at:
-        if out is None:
-            out = (torch.empty if q_len is None else torch.zeros)((B, S, Hq, Dv), dtype=q.dtype, device=dev)
-        else:
-            _on(out, dev, q.dtype, "out")
-            _need(out.shape == (B, S, Hq, Dv), f"out {tuple(out.shape)}: {(B, S, Hq, Dv)}")
-            _own_elements(out)
-            for t, n in ((q, "q"), (k, "k"), (v, "v")):
+    if not _here(dev, stream):
+        return _elsewhere(dev, stream, (q, k, v, q_len, kv_len, out),
+                          lambda: attend(q, k, v, scale=scale, frame=frame, window=window, sinks=sinks, q_len=q_len,
+                                         kv_len=kv_len, out=out))
+    if out is None:
+        out = (torch.empty if q_len is None else torch.zeros)((B, S, Hq, Dv), dtype=dtype, device=dev)
+    else:
+        _on(out, dev, dtype, "out")
+        _need(out.shape == (B, S, Hq, Dv), "out: [B, S, Hq, Dv]")
+        _own_elements(out)
+        at = _range(out)
+        for t, n in ((q, "q"), (k, "k"), (v, "v")):
+            if _meet(at, _range(t)):
                 _apart(out, t, n)
-        if out.numel() == 0:
-            return out
-        q, k, v = (t if _aligned(t) else t.contiguous() for t in (q, k, v))
-        q, k, v = (t if _aligned(t) else t.clone(memory_format=torch.contiguous_format) for t in (q, k, v))
-        o = out if _aligned(out) else out.clone(memory_format=torch.contiguous_format)
-        a = AttnArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), *q.stride()[:3], *k.stride()[:3],
-                     *v.stride()[:3], *o.stride()[:3], None if q_len is None else q_len.data_ptr(),
-                     None if kv_len is None else kv_len.data_ptr(), scale, B, S, Hq, Hk, D, Dv, slots, frame, window, sinks,
-                     DTYPES[q.dtype], None, 0)
-        n = lib.va_tok_attn_workspace_bytes(ctypes.byref(a))
-        if n:
-            _need(n > 0, f"va_tok_attn_workspace_bytes failed with status {n}")
-            ws = torch.empty(n, dtype=torch.uint8, device=dev)
-            a.ws, a.ws_bytes = ws.data_ptr(), n
-        _lib.check(lib.va_tok_attn(at.ptr, ctypes.byref(a)), "va_tok_attn")
-        if o is not out:
-            out.copy_(o)
+    if B == 0 or S == 0:
+        return out
+    q, k, v = _aligned(q), _aligned(k), _aligned(v)
+    o = _aligned(out)
+    lib = _lib.load()
+    ints = (B, S, Hq, Hk, D, Dv, slots, frame, window, sinks, DTYPES[dtype])
+    most = (q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
+            *o.stride()[:3], 0 if q_len is None else q_len.data_ptr(), 0 if kv_len is None else kv_len.data_ptr(), scale, *ints)
+    a = ATTN_PACK.pack(*most, 0, 0)
+    n = lib.va_tok_attn_workspace_bytes(a)
+    if n:
+        _need(n > 0, f"va_tok_attn_workspace_bytes failed with status {n}")
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        a = ATTN_PACK.pack(*most, ws.data_ptr(), n)
+    rc = lib.va_tok_attn(_raw_stream(dev.index), a)
+    if rc:
+        _lib.check(rc, "va_tok_attn")
+    if o is not out:
+        out.copy_(o)
     return out
