@@ -10,6 +10,7 @@
 // One pass over the keys with the running maximum and sum of the softmax (base 2: the scale is folded with log2 e).
 #include <math.h>
 
+#include "va_dev.h"
 #include "va_tok.h"
 
 namespace {
@@ -49,15 +50,24 @@ struct Tr;
 template <>
 struct Tr<__bf16> {
     static constexpr int VE = 8;   // values of a 16-byte piece
-    static constexpr int KT = 64;  // keys of a tile
+    static constexpr int KT = 64;  // keys of a staged tile
 };
 template <>
 struct Tr<float> {
     static constexpr int VE = 4;
     static constexpr int KT = 32;
 };
+template <typename T, int DP>
+struct Dims {
+    static constexpr int VE = Tr<T>::VE, NC = DP / VE;                      // pieces of a row
+    static constexpr int CS = NC <= 4 ? 4 : NC <= 8 ? 8 : NC <= 16 ? 16 : 32;  // ... as laid out in LDS
+    static constexpr int NV = DP / 32;
+    // attn_split: waves of a workgroup (two buffers of K and V tiles each within the LDS), and its bytes
+    static constexpr int SW = CS == 32 ? 2 : 4, SLDS = SW * 4 * 32 * CS * 16;
+    static_assert(SLDS <= 128 * 1024 && SW / 2 * NV * 16 * 64 * 4 <= SLDS, "");
+};
 
-// LDS image of a tile: KT rows of CS 16-byte pieces, piece c of row r in place c ^ swz(r).  K is read by 8 lanes of
+// LDS image of a tile: rows of CS 16-byte pieces, piece c of row r in place c ^ swz(r).  K is read by 8 lanes of
 // consecutive rows at one piece, V by 4 rows at 4 pieces: both spread over the banks.
 template <int CS>
 __device__ __forceinline__ int swz(int r) {
@@ -69,224 +79,486 @@ __device__ __forceinline__ int swz(int r) {
         return (r >> 1) & 3;
 }
 
-// Tile walk: keys [t0, t0 + KT) of [lo, hi), positions -> slots
 __device__ __forceinline__ int slot_of(const va_tok_attn_args& a, int p) {
     if (p < a.slots) return p;
     return a.sinks + (p - a.sinks) % (a.slots - a.sinks);
 }
 
-template <typename T, int DP>
-__global__ __launch_bounds__(256) void attn_kernel(va_tok_attn_args a, int ntiles) {
-    constexpr int VE = Tr<T>::VE, KT = Tr<T>::KT;
-    constexpr bool BF = sizeof(T) == 2;
-    constexpr int NC = DP / VE;                                       // pieces of a row
-    constexpr int CS = NC <= 4 ? 4 : NC <= 8 ? 8 : NC <= 16 ? 16 : 32;  // ... as laid out (a power of two)
-    constexpr int KB = KT / 32, NV = DP / 32;
-    __shared__ __align__(16) unsigned char ks[KT * CS * 16], vs[KT * CS * 16];
-    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, lc = lane & 31, lh = lane >> 5;
-    const int G = a.Hq / a.Hk;
-    int bid = blockIdx.x;
-    const int tile = bid % ntiles;
-    bid /= ntiles;
-    const int hk = bid % a.Hk, b = bid / a.Hk;
-    const AttnSeq sq = attn_seq(a, b);
-    const int rows = sq.ql * G, r0 = tile * 128;
-    if (r0 >= rows) return;
-    // this lane's row
-    const int row = r0 + 32 * wid + lc, s = row / G, g = row - s * G;
-    const bool there = row < rows;
-    const Span sp = there ? attn_span(a, sq, sq.first + s) : Span{a.sinks, 0};
-    // the workgroup's keys: spans grow with the position
-    const int s0 = r0 / G, s1 = (min(r0 + 128, rows) - 1) / G;
-    const Span w0 = attn_span(a, sq, max(sq.first + s0, 0)), w1 = attn_span(a, sq, sq.first + s1);
-    const int top = w1.top, low = max(w0.low, a.sinks), ntop = min(a.sinks, top);
+// sc += K Q^T of 32 keys x 32 rows; kf(c): piece 2 c + lh of this lane's key
+template <typename T, int DP, typename F>
+__device__ __forceinline__ void scores(f32x16& sc, const u32x4 (&qf)[DP / (2 * Tr<T>::VE)], F kf) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sc[i] = 0.0f;
+#pragma unroll
+    for (int c = 0; c < DP / (2 * Tr<T>::VE); ++c) {
+        const u32x4 k = kf(c);
+        if constexpr (sizeof(T) == 2) {
+            sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16((bf16x8)k, (bf16x8)qf[c], sc, 0, 0, 0);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                sc = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k[e]), __uint_as_float(qf[c][e]), sc, 0, 0, 0);
+        }
+    }
+}
 
-    // Q^T fragments
-    const T* qp = (const T*)a.q + b * a.q_sb + s * a.q_ss + (int64_t)(hk * G + g) * a.q_sh;
-    u32x4 qf[DP / (2 * VE)];
+// the key of register i of a block of 32 scores
+__device__ __forceinline__ int key_of(int i, int lh) { return 8 * (i / 4) + 4 * lh + i % 4; }
+
+// The running softmax of one row (a lane and its partner lane ^ 32): mx is the reference of the exponents in units of
+// the raw scores, kept while the maximum grows by less than 2^8 in the result (the sums are float, and a probability
+// rounded to bf16 has the same relative error at any size).  Exponents: 2^((s - mx) c).
+template <int NV>
+struct Row {
+    float mx = -INFINITY, sum = 0.0f;
+    f32x16 acc[NV];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[v][i] = 0.0f;
+    }
+};
+
+template <int KB, int NV>
+__device__ __forceinline__ void softmax(Row<NV>& r, f32x16 (&sc)[KB], float c) {
+    float nm = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < KB; ++k)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) nm = fmaxf(nm, sc[k][i]);
+    nm = fmaxf(nm, __shfl_xor(nm, 32));
+    const bool up = nm > r.mx && !((nm - r.mx) * c <= 8.0f);
+    if (__any(up)) {  // (each row by its own maximum alone: a row's result does not depend on the others')
+        const float alpha = up ? __builtin_amdgcn_exp2f((r.mx - nm) * c) : 1.0f;
+        r.mx = up ? nm : r.mx;
+        r.sum *= alpha;
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) r.acc[v][i] *= alpha;
+    }
+    const float off = r.mx == -INFINITY ? 0.0f : -r.mx * c;
+    float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < KB; ++k)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            sc[k][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[k][i], c, off));
+            part[i % 4] += sc[k][i];
+        }
+    r.sum += (part[0] + part[1]) + (part[2] + part[3]);
+}
+
+// lane group (lh, column half): 4 keys of column 32 v + (lane & 31) from rows row0 + 4 lh .., for the two 8-key groups
+template <int CS>
+__device__ __forceinline__ u32x4 values_bf16(const unsigned char* vs, int row0, int v, int lane) {
+    const int lh = lane >> 5, q = lane & 15, ch = (lane >> 4) & 1;
+    u32x4 vf;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        // 16 lanes read 4 rows of 16 columns: lane q gets column q's 4 keys
+        const int row = row0 + 8 * u + 4 * lh + (q >> 2), pc = 4 * v + 2 * ch + ((q & 3) >> 1);
+        const unsigned char* at = vs + (row * CS + (pc ^ swz<CS>(row))) * 16 + 8 * (q & 1);
+        const u32x2 t = __builtin_bit_cast(
+            u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at));
+        vf[2 * u] = t[0], vf[2 * u + 1] = t[1];
+    }
+    return vf;
+}
+
+// O^T += V^T P^T over 32 keys whose values lie in LDS rows r0 .. r0 + 31 of vs.  FIN: values that are not finite count as
+// zeros (add_nonfinite adds them)
+// -> whether this lane met any
+template <typename T, int DP, bool FIN = false>
+__device__ __forceinline__ bool add_values(Row<DP / 32>& r, const f32x16& p, const unsigned char* vs, int r0, int lane) {
+    constexpr int CS = Dims<T, DP>::CS, NV = DP / 32;
+    bool bad = false;
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int c = 0; c < 16; c += 8) {
+            u32x4 pf;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) pf[e] = pk_bf16(p[c + 2 * e], p[c + 2 * e + 1]);
+            if constexpr (DP > 64) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                u32x4 vf = values_bf16<CS>(vs, r0 + 2 * c, v, lane);
+                if constexpr (FIN) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const bool lo = (vf[e] & 0x7f80u) == 0x7f80u, hi = (vf[e] & 0x7f800000u) == 0x7f800000u;
+                        vf[e] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
+                        bad |= lo || hi;
+                    }
+                }
+                r.acc[v] = __builtin_amdgcn_mfma_f32_32x32x16_bf16((bf16x8)vf, (bf16x8)pf, r.acc[v], 0, 0, 0);
+            }
+        }
+    } else {
+        const int lc = lane & 31, lh = lane >> 5;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int row = r0 + key_of(i, lh);
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                const int d = 32 * v + lc;
+                float x = *(const float*)(vs + (row * CS + ((d / 4) ^ swz<CS>(row))) * 16 + 4 * (d % 4));
+                if constexpr (FIN) {
+                    const bool nf = !(fabsf(x) < INFINITY);
+                    x = nf ? 0.0f : x;
+                    bad |= nf;
+                }
+                r.acc[v] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, p[i], r.acc[v], 0, 0, 0);
+            }
+        }
+    }
+    return bad;
+}
+
+// A tile that some row does not see whole and that holds values which are not finite: the product would carry them, as
+// 0 x inf, into rows that do not see their key.  They are left out of it, and each row adds those of the keys it sees
+// (positions from .. to - 1 of the tile's n keys).
+template <typename T, int DP>
+__device__ void add_nonfinite(Row<DP / 32>& r, const unsigned char* vs, int from, int to, int n, int lh) {
+    constexpr int CS = Dims<T, DP>::CS, NV = DP / 32, VE = Tr<T>::VE;
+#pragma unroll 1
+    for (int k = 0; k < n; ++k) {
+        const bool see = k >= from && k < to;
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int d = 32 * v + key_of(i, lh);
+                const float x = (float)*(const T*)(vs + (k * CS + ((d / VE) ^ swz<CS>(k))) * 16 + (d % VE) * sizeof(T));
+                if (see && !(fabsf(x) < INFINITY)) r.acc[v][i] += x;
+                if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // few registers, not speed
+            }
+    }
+}
+
+// 16 registers of block v -> columns 32 v + key_of(i, lh) of this lane's row
+template <typename T>
+__device__ __forceinline__ void store_block(T* op, const f32x16& x, float by, int v, int lh, int Dv) {
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+        const int d = 32 * v + key_of(i, lh);
+        if (d >= Dv) continue;
+        if constexpr (sizeof(T) == 2)
+            *(u32x2*)(op + d) = (u32x2){pk_bf16(x[i] * by, x[i + 1] * by), pk_bf16(x[i + 2] * by, x[i + 3] * by)};
+        else
+            *(f32x4*)(op + d) = (f32x4){x[i] * by, x[i + 1] * by, x[i + 2] * by, x[i + 3] * by};
+    }
+}
+
+template <typename T, int DP>
+__device__ __forceinline__ void load_q(const va_tok_attn_args& a, const T* qp, bool there, int lh,
+                                       u32x4 (&qf)[DP / (2 * Tr<T>::VE)]) {
+    constexpr int VE = Tr<T>::VE;
 #pragma unroll
     for (int c = 0; c < DP / (2 * VE); ++c) {
         const int d = (2 * c + lh) * VE;
         qf[c] = there && d < a.D ? *(const u32x4*)(qp + d) : (u32x4){0, 0, 0, 0};
     }
+}
+
+// The walk over a row block's keys: positions [0, ntop), [low, mid) and [mid, top) -- the sinks, and what its rows see
+// behind them, cut where the ring begins anew so that a tile's slots are consecutive -- in tiles of KT.
+template <int KT>
+struct Walk {
+    int ntop, low, mid, top, n0, n1, nt;
+    __device__ __forceinline__ Walk(const va_tok_attn_args& a, Span first, Span last) {
+        top = last.top, low = max(first.low, a.sinks), ntop = min(a.sinks, top), mid = top;
+        if (top > a.slots && top > low) {
+            const int ring = a.slots - a.sinks;
+            const int64_t m = a.sinks + ((int64_t)(low - a.sinks) + ring - 1) / ring * ring;
+            mid = m < top ? (int)m : top;
+        }
+        n0 = (ntop + KT - 1) / KT;
+        n1 = n0 + (mid > low ? (mid - low + KT - 1) / KT : 0);
+        nt = n1 + (top > mid && top > low ? (top - max(mid, low) + KT - 1) / KT : 0);
+    }
+    // tile t holds positions t0 .. min(t0 + KT, end) - 1
+    __device__ __forceinline__ void tile(int t, int* t0, int* end) const {
+        *t0 = t < n0 ? t * KT : t < n1 ? low + (t - n0) * KT : mid + (t - n1) * KT;
+        *end = t < n0 ? ntop : t < n1 ? mid : top;
+    }
+};
+
+// ------------------------------------------------------------------ many rows: 128 a workgroup, keys through LDS
+// Tiles of KT keys in two LDS buffers: the next tile is on its way into one by LDS-DMA while the other is worked on, and
+// one wait and barrier a tile publish it.  A tile's slots are consecutive (the walk is cut at the ring's end), so its
+// rows are offsets from one address; rows and pieces that are not there take an offset out of range and load zeros.
+constexpr int TILE_OOB = 0x7ffffff0;
+
+// (a plain function: the host pass drops the stub of a kernel template that names the builtin)
+__device__ __forceinline__ void dma16(const void* base, void* lds, int off) {
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, TILE_OOB, 0x00020000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lvoid_t*)lds, 16, off, 0, 0, 0);
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_kernel(va_tok_attn_args a, int ntiles) {
+    constexpr int VE = Tr<T>::VE, KT = Tr<T>::KT, CS = Dims<T, DP>::CS, KB = KT / 32, NV = DP / 32;
+    constexpr int NP = KT * CS / 256, BUF = KT * CS * 16;  // DMAs of a wave for K; bytes of a tile of K
+    extern __shared__ __align__(16) unsigned char sm[];    // [2][K | V]
+    const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), lc = lane & 31, lh = lane >> 5;
+    const int G = a.Hq / a.Hk;
+    int bid = xcd_tile(blockIdx.x, gridDim.x);
+    const int tile = ntiles - 1 - bid % ntiles;  // the rows that see most first
+    bid /= ntiles;
+    const int hk = bid % a.Hk, b = bid / a.Hk;
+    const AttnSeq sq = attn_seq(a, b);
+    const int rows = sq.ql * G, r0 = tile * 128;
+    if (r0 >= rows) return;
+    const int row = r0 + 32 * wid + lc, s = row / G, g = row - s * G;  // this lane's row
+    const bool there = row < rows;
+    const Span sp = there ? attn_span(a, sq, sq.first + s) : Span{a.sinks, 0};
+    // spans grow with the position: the workgroup's keys, and this wave's
+    const Walk<KT> w(a, attn_span(a, sq, max(sq.first + r0 / G, 0)), attn_span(a, sq, sq.first + (min(r0 + 128, rows) - 1) / G));
+    const Span f0 = attn_span(a, sq, sq.first + min(r0 + 32 * wid, rows - 1) / G);
+    const Span f1 = attn_span(a, sq, sq.first + min(r0 + 32 * wid + 31, rows - 1) / G);
+    const bool idle = r0 + 32 * wid >= rows;
+
+    u32x4 qf[DP / (2 * VE)];
+    load_q<T, DP>(a, (const T*)a.q + b * a.q_sb + s * a.q_ss + (int64_t)(hk * G + g) * a.q_sh, there, lh, qf);
     const float cexp = a.scale * 1.4426950408889634f;
-    float mx = -INFINITY, sum = 0.0f;
-    f32x16 acc[NV];
-#pragma unroll
-    for (int v = 0; v < NV; ++v)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[v][i] = 0.0f;
+    Row<NV> r;
+    r.clear();
 
     const T* kb = (const T*)a.k + b * a.k_sb + hk * a.k_sh;
     const T* vb = (const T*)a.v + b * a.v_sb + hk * a.v_sh;
-    for (int part = 0; part < 2; ++part) {
-        const int beg = part ? low : 0, end = part ? top : ntop;
-        for (int t0 = beg; t0 < end; t0 += KT) {
-            __syncthreads();
-            for (int i = tid; i < KT * NC; i += 256) {
-                const int r = i / NC, c = i % NC, p = t0 + r;
-                const int slot = p < end ? slot_of(a, p) : 0;
-                const bool kin = p < end && c * VE < a.D, vin = p < end && c * VE < a.Dv;
-                const int at = (r * CS + (c ^ swz<CS>(r))) * 16;
-                *(u32x4*)(ks + at) = kin ? *(const u32x4*)(kb + slot * a.k_ss + c * VE) : (u32x4){0, 0, 0, 0};
-                *(u32x4*)(vs + at) = vin ? *(const u32x4*)(vb + slot * a.v_ss + c * VE) : (u32x4){0, 0, 0, 0};
-            }
-            __syncthreads();
+    // this lane's DMAs: piece i = (wid * NP + j) * 64 + lane of the tile's image
+    int rr[NP], ko[NP], vo[NP];
+#pragma unroll
+    for (int j = 0; j < NP; ++j) {
+        const int i = (wid * NP + j) * 64 + lane, c = (i % CS) ^ swz<CS>(i / CS);
+        rr[j] = i / CS;
+        ko[j] = c * VE < a.D ? (int)(rr[j] * a.k_ss + c * VE) * (int)sizeof(T) : TILE_OOB;
+        vo[j] = c * VE < a.Dv ? (int)(rr[j] * a.v_ss + c * VE) * (int)sizeof(T) : TILE_OOB;
+    }
+    auto fetch = [&](int t, int buf) {
+        int t0, end;
+        w.tile(t, &t0, &end);
+        const int64_t slot = slot_of(a, t0);
+        const T *kt = kb + slot * a.k_ss, *vt = vb + slot * a.v_ss;
+        unsigned char* ks = sm + buf * 2 * BUF + wid * NP * 1024;
+#pragma unroll
+        for (int j = 0; j < NP; ++j) dma16(kt, ks + j * 1024, t0 + rr[j] < end ? ko[j] : TILE_OOB);
+#pragma unroll
+        for (int j = 0; j < NP; ++j) dma16(vt, ks + BUF + j * 1024, t0 + rr[j] < end ? vo[j] : TILE_OOB);
+    };
+    if (w.nt > 0) fetch(0, 0);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    for (int t = 0; t < w.nt; ++t) {
+        const int buf = t & 1;
+        if (t + 1 < w.nt) fetch(t + 1, buf ^ 1);
+        const unsigned char* ks = sm + buf * 2 * BUF;
+        const unsigned char* vs = ks + BUF;
+        int t0, end;
+        w.tile(t, &t0, &end);
+        const bool sink = t < w.n0;
+        if (!idle && t0 < f1.top && (sink || t0 + KT > f0.low)) {
             f32x16 sc[KB];
 #pragma unroll
-            for (int kb_ = 0; kb_ < KB; ++kb_) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) sc[kb_][i] = 0.0f;
-                const int r = 32 * kb_ + lc;
-#pragma unroll
-                for (int c = 0; c < NC / 2; ++c) {
-                    const u32x4 kf = *(const u32x4*)(ks + (r * CS + ((2 * c + lh) ^ swz<CS>(r))) * 16);
-                    if constexpr (BF) {
-                        sc[kb_] = __builtin_amdgcn_mfma_f32_32x32x16_bf16((bf16x8)kf, (bf16x8)qf[c], sc[kb_], 0, 0, 0);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            sc[kb_] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(kf[e]), __uint_as_float(qf[c][e]),
-                                                                          sc[kb_], 0, 0, 0);
-                    }
-                }
+            for (int k = 0; k < KB; ++k) {
+                scores<T, DP>(sc[k], qf, [&](int c) {
+                    const int kr = 32 * k + lc;
+                    return *(const u32x4*)(ks + (kr * CS + ((2 * c + lh) ^ swz<CS>(kr))) * 16);
+                });
+                __builtin_amdgcn_sched_barrier(0);  // (one block's fragments in registers at a time)
             }
-            // register i of block kb: key 32 kb + 8 (i / 4) + 4 lh + i % 4
-            float nm = mx;
+            if (t0 + KT <= min(f0.top, end) && (sink || t0 >= f1.low)) {  // every row of the wave sees every key
+                softmax<KB, NV>(r, sc, cexp);
 #pragma unroll
-            for (int kb_ = 0; kb_ < KB; ++kb_)
+                for (int k = 0; k < KB; ++k) add_values<T, DP>(r, sc[k], vs, 32 * k, lane);
+            } else {
+                const int from = (sink ? 0 : sp.low) - t0, upto = min(sp.top, end) - t0;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int p = t0 + 32 * kb_ + 8 * (i / 4) + 4 * lh + i % 4;
-                    const bool see = p < sp.top && p < end && (part ? p >= sp.low : true);
-                    sc[kb_][i] = see ? sc[kb_][i] * cexp : -INFINITY;
-                    nm = fmaxf(nm, sc[kb_][i]);
-                }
-            nm = fmaxf(nm, __shfl_xor(nm, 32));
-            const float base = nm == -INFINITY ? 0.0f : nm;
-            const float alpha = __builtin_amdgcn_exp2f(mx - base);
-            mx = nm;
-            sum *= alpha;
+                for (int k = 0; k < KB; ++k)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int p = 32 * k + key_of(i, lh);
+                        sc[k][i] = p >= from && p < upto ? sc[k][i] : -INFINITY;
+                    }
+                softmax<KB, NV>(r, sc, cexp);
+                bool bad = false;
+#pragma unroll
+                for (int k = 0; k < KB; ++k) bad |= add_values<T, DP, true>(r, sc[k], vs, 32 * k, lane);
+                if (__any(bad)) add_nonfinite<T, DP>(r, vs, from, upto, KT, lh);
+            }
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+    }
+    const float total = r.sum + __shfl_xor(r.sum, 32);
+    if (!there) return;
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    T* op = (T*)a.o + b * a.o_sb + s * a.o_ss + (int64_t)(hk * G + g) * a.o_sh;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) store_block<T>(op, r.acc[v], inv, v, lh, a.Dv);
+}
+
+// ------------------------------------------------------------------ few rows: the keys split over waves and workgroups
+// A workgroup takes 32 rows and one of nsplit shares of their tiles of 32 keys; its waves walk the share's tiles in
+// turn, each through two buffers of its own in LDS and without a barrier, until their sums are joined.  A tile comes by
+// LDS-DMA while the one before is worked on, whole rows at a time (a load covers complete cache lines: reading each key's
+// row by its own lane instead, 32 lines at a time, ran at 1.7 TB/s).
+// A share's result: [NV * 16][64] registers as they lie in the wave, then the 32 rows' maxima and sums.
+__device__ __forceinline__ int64_t part_floats(int NV) { return NV * 16 * 64 + 64; }
+
+template <typename T, int DP>
+__global__ __launch_bounds__((64 * Dims<T, DP>::SW), 1) void attn_split(va_tok_attn_args a, int nrb, int nsplit) {
+    constexpr int VE = Tr<T>::VE, CS = Dims<T, DP>::CS, NV = DP / 32;
+    constexpr int NP = 32 * CS / 64, BUF = 32 * CS * 16, ACC = NV * 16 * 64 * 4, SW = Dims<T, DP>::SW;
+    extern __shared__ __align__(16) unsigned char sm[];  // a wave: [2][K | V]; then the waves' registers
+    __shared__ float sms[2][2][64];
+    const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), lc = lane & 31, lh = lane >> 5;
+    const int G = a.Hq / a.Hk;
+    int bid = xcd_tile(blockIdx.x, gridDim.x);
+    const int split = bid % nsplit;
+    bid /= nsplit;
+    const int rb = bid % nrb;
+    const int unit = bid / nrb, hk = unit % a.Hk, b = unit / a.Hk;
+    const AttnSeq sq = attn_seq(a, b);
+    const int rows = sq.ql * G, r0 = rb * 32;
+    if (r0 >= rows) return;
+    const int row = r0 + lc, s = row / G, g = row - s * G;
+    const bool there = row < rows;
+    const Span sp = there ? attn_span(a, sq, sq.first + s) : Span{a.sinks, 0};
+    const Span f0 = attn_span(a, sq, sq.first + r0 / G), f1 = attn_span(a, sq, sq.first + (min(r0 + 32, rows) - 1) / G);
+    const Walk<32> w(a, attn_span(a, sq, max(sq.first + r0 / G, 0)), f1);
+    const int per = (w.nt + nsplit - 1) / nsplit, t1 = min((split + 1) * per, w.nt);
+
+    u32x4 qf[DP / (2 * VE)];
+    load_q<T, DP>(a, (const T*)a.q + b * a.q_sb + s * a.q_ss + (int64_t)(hk * G + g) * a.q_sh, there, lh, qf);
+    const float cexp = a.scale * 1.4426950408889634f;
+    Row<NV> r;
+    r.clear();
+    const T* kb = (const T*)a.k + b * a.k_sb + hk * a.k_sh;
+    const T* vb = (const T*)a.v + b * a.v_sb + hk * a.v_sh;
+    int ko[NP], vo[NP];  // this lane's DMAs: piece j * 64 + lane of the tile's image
+#pragma unroll
+    for (int j = 0; j < NP; ++j) {
+        const int rr = (j * 64 + lane) / CS, c = (lane % CS) ^ swz<CS>(rr);
+        ko[j] = c * VE < a.D ? (int)(rr * a.k_ss + c * VE) * (int)sizeof(T) : TILE_OOB;
+        vo[j] = c * VE < a.Dv ? (int)(rr * a.v_ss + c * VE) * (int)sizeof(T) : TILE_OOB;
+    }
+    unsigned char* mine = sm + wid * 4 * BUF;
+    auto fetch = [&](int t, int buf) {
+        int t0, end;
+        w.tile(t, &t0, &end);
+        const int64_t slot = slot_of(a, t0);
+        const T *k = kb + slot * a.k_ss, *v = vb + slot * a.v_ss;
+        unsigned char* to = mine + buf * 2 * BUF;
+        const int n = end - t0 - lane / CS;  // rows of the tile from this lane's first on
+#pragma unroll
+        for (int j = 0; j < NP; ++j) dma16(k, to + j * 1024, j * (64 / CS) < n ? ko[j] : TILE_OOB);
+#pragma unroll
+        for (int j = 0; j < NP; ++j) dma16(v, to + BUF + j * 1024, j * (64 / CS) < n ? vo[j] : TILE_OOB);
+    };
+    int t = split * per + wid, buf = 0;
+    if (t < t1) fetch(t, 0);
+    for (; t < t1; t += SW, buf ^= 1) {
+        // this tile is there (the wave's own loads, and its reads of the other buffer are done: their values were used)
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (t + SW < t1) fetch(t + SW, buf ^ 1);
+        const unsigned char *ks = mine + buf * 2 * BUF, *vs = ks + BUF;
+        int t0, end;
+        w.tile(t, &t0, &end);
+        const bool sink = t < w.n0;
+        f32x16 sc[1];
+        scores<T, DP>(sc[0], qf, [&](int c) { return *(const u32x4*)(ks + (lc * CS + ((2 * c + lh) ^ swz<CS>(lc))) * 16); });
+        if (t0 + 32 <= min(f0.top, end) && (sink || t0 >= f1.low)) {  // every row sees every key
+            softmax<1, NV>(r, sc, cexp);
+            add_values<T, DP>(r, sc[0], vs, 0, lane);
+        } else {
+            const int from = (sink ? 0 : sp.low) - t0, upto = min(sp.top, end) - t0;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sc[0][i] = key_of(i, lh) >= from && key_of(i, lh) < upto ? sc[0][i] : -INFINITY;
+            softmax<1, NV>(r, sc, cexp);
+            if (__any(add_values<T, DP, true>(r, sc[0], vs, 0, lane))) add_nonfinite<T, DP>(r, vs, from, upto, 32, lh);
+        }
+    }
+    // the upper half of the waves into the lower, until one is left
+    r.sum += __shfl_xor(r.sum, 32);
+    float* regs = (float*)sm;
+#pragma unroll
+    for (int half = SW / 2; half >= 1; half /= 2) {
+        __syncthreads();
+        if (wid >= half && wid < 2 * half) {
+            float* to = regs + (wid - half) * (ACC / 4);
 #pragma unroll
             for (int v = 0; v < NV; ++v)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) acc[v][i] *= alpha;
-            bool seen[KB][16];
+                for (int i = 0; i < 16; ++i) to[(v * 16 + i) * 64 + lane] = r.acc[v][i];
+            sms[wid - half][0][lane] = r.mx;
+            sms[wid - half][1][lane] = r.sum;
+        }
+        __syncthreads();
+        if (wid < half) {
+            const float* of = regs + wid * (ACC / 4);
+            const float m2 = sms[wid][0][lane], s2 = sms[wid][1][lane], mx = fmaxf(r.mx, m2);
+            const float base = mx == -INFINITY ? 0.0f : mx;
+            const float x = __builtin_amdgcn_exp2f((r.mx - base) * cexp), y = __builtin_amdgcn_exp2f((m2 - base) * cexp);
+            r.mx = mx;
+            r.sum = r.sum * x + s2 * y;
 #pragma unroll
-            for (int kb_ = 0; kb_ < KB; ++kb_)
+            for (int v = 0; v < NV; ++v)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    seen[kb_][i] = sc[kb_][i] != -INFINITY;
-                    sc[kb_][i] = __builtin_amdgcn_exp2f(sc[kb_][i] - base);
-                    sum += sc[kb_][i];
-                }
-            // O^T += V^T P^T: a step takes the keys of 8 (bf16) or 1 (f32) registers
-            constexpr int PR = BF ? 8 : 1;
-#pragma unroll
-            for (int kb_ = 0; kb_ < KB; ++kb_)
-#pragma unroll
-                for (int c = 0; c < 16; c += PR) {
-                    u32x4 pf, one;
-                    if constexpr (BF) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            pf[e] = pk_bf16(sc[kb_][c + 2 * e], sc[kb_][c + 2 * e + 1]);
-                            one[e] = (seen[kb_][c + 2 * e] ? 0x3f80u : 0u) | (seen[kb_][c + 2 * e + 1] ? 0x3f800000u : 0u);
-                        }
-                    }
-#pragma unroll
-                    for (int v = 0; v < NV; ++v) {
-                        if constexpr (BF) {
-                            // lane group (lh, column half): rows 4 lh + (i / 4) of the step's two 8-key groups
-                            const int q = lane & 15, ch = (lane >> 4) & 1;
-                            u32x4 vf;
-#pragma unroll
-                            for (int u = 0; u < 2; ++u) {
-                                const int r = 32 * kb_ + 2 * c + 8 * u + 4 * lh + (q >> 2);
-                                const int pc = 4 * v + 2 * ch + ((q & 3) >> 1);
-                                const unsigned char* at = vs + (r * CS + (pc ^ swz<CS>(r))) * 16 + 8 * (q & 1);
-                                const s16x4 t = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                    (__attribute__((address_space(3))) s16x4*)at);
-                                const u32x2 tt = __builtin_bit_cast(u32x2, t);
-                                vf[2 * u] = tt[0], vf[2 * u + 1] = tt[1];
-                            }
-                            // values that are not finite would reach rows that do not see their key (0 x inf): they
-                            // are taken out, and added where they are seen
-                            unsigned bad = 0;
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                bad |= (vf[e] & 0x7f80u) == 0x7f80u;
-                                bad |= (vf[e] & 0x7f800000u) == 0x7f800000u;
-                            }
-                            if (__any(bad)) {
-                                u32x4 fin, up, dn;
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) {
-                                    fin[e] = up[e] = dn[e] = 0;
-#pragma unroll
-                                    for (int w = 0; w < 32; w += 16) {
-                                        const unsigned x = vf[e] >> w & 0xffffu;
-                                        const bool nf = (x & 0x7f80u) == 0x7f80u, nan = nf && (x & 0x7fu);
-                                        fin[e] |= (nf ? 0u : x) << w;
-                                        up[e] |= (nf && (nan || !(x >> 15)) ? 0x3f80u : 0u) << w;
-                                        dn[e] |= (nf && (nan || x >> 15) ? 0x3f80u : 0u) << w;
-                                    }
-                                }
-                                f32x16 nu, nd;
-#pragma unroll
-                                for (int i = 0; i < 16; ++i) nu[i] = nd[i] = 0.0f;
-                                acc[v] = __builtin_amdgcn_mfma_f32_32x32x16_bf16((bf16x8)fin, (bf16x8)pf, acc[v], 0, 0, 0);
-                                nu = __builtin_amdgcn_mfma_f32_32x32x16_bf16((bf16x8)up, (bf16x8)one, nu, 0, 0, 0);
-                                nd = __builtin_amdgcn_mfma_f32_32x32x16_bf16((bf16x8)dn, (bf16x8)one, nd, 0, 0, 0);
-#pragma unroll
-                                for (int i = 0; i < 16; ++i) {
-                                    if (nu[i] > 0.0f) acc[v][i] += INFINITY;
-                                    if (nd[i] > 0.0f) acc[v][i] -= INFINITY;
-                                }
-                            } else {
-                                acc[v] = __builtin_amdgcn_mfma_f32_32x32x16_bf16((bf16x8)vf, (bf16x8)pf, acc[v], 0, 0, 0);
-                            }
-                        } else {
-                            const int r = 32 * kb_ + 8 * (c / 4) + 4 * lh + c % 4, d = 32 * v + lc;
-                            const float x = *(const float*)(vs + (r * CS + ((d / 4) ^ swz<CS>(r))) * 16 + 4 * (d % 4));
-                            const bool nf = !(fabsf(x) < INFINITY);
-                            acc[v] = __builtin_amdgcn_mfma_f32_32x32x2f32(nf ? 0.0f : x, sc[kb_][c], acc[v], 0, 0, 0);
-                            if (__any(nf)) {
-                                f32x16 nu, nd;
-#pragma unroll
-                                for (int i = 0; i < 16; ++i) nu[i] = nd[i] = 0.0f;
-                                const float w = seen[kb_][c] ? 1.0f : 0.0f;
-                                nu = __builtin_amdgcn_mfma_f32_32x32x2f32(nf && !(x < 0.0f) ? 1.0f : 0.0f, w, nu, 0, 0, 0);
-                                nd = __builtin_amdgcn_mfma_f32_32x32x2f32(nf && !(x > 0.0f) ? 1.0f : 0.0f, w, nd, 0, 0, 0);
-#pragma unroll
-                                for (int i = 0; i < 16; ++i) {
-                                    if (nu[i] > 0.0f) acc[v][i] += INFINITY;
-                                    if (nd[i] > 0.0f) acc[v][i] -= INFINITY;
-                                }
-                            }
-                        }
-                    }
-                }
+                for (int i = 0; i < 16; ++i) r.acc[v][i] = r.acc[v][i] * x + of[(v * 16 + i) * 64 + lane] * y;
         }
     }
-    if (!there) return;
-    const float total = sum + __shfl_xor(sum, 32);
-    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-    // register i of block v: column 32 v + 8 (i / 4) + 4 lh + i % 4 of this lane's row
-    T* op = (T*)a.o + b * a.o_sb + s * a.o_ss + (int64_t)(hk * G + g) * a.o_sh;
+    if (wid || !there) return;
+    if (nsplit == 1) {
+        const float inv = r.sum == 0.0f ? 0.0f : 1.0f / r.sum;
+        T* op = (T*)a.o + b * a.o_sb + s * a.o_ss + (int64_t)(hk * G + g) * a.o_sh;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) store_block<T>(op, r.acc[v], inv, v, lh, a.Dv);
+        return;
+    }
+    float* ws = (float*)a.ws + ((int64_t)(unit * nrb + rb) * nsplit + split) * part_floats(NV);
 #pragma unroll
     for (int v = 0; v < NV; ++v)
 #pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-            const int d = 32 * v + 2 * i + 4 * lh;
-            if (d >= a.Dv) continue;
-            const float x[4] = {acc[v][i] * inv, acc[v][i + 1] * inv, acc[v][i + 2] * inv, acc[v][i + 3] * inv};
-            if constexpr (BF)
-                *(u32x2*)(op + d) = (u32x2){pk_bf16(x[0], x[1]), pk_bf16(x[2], x[3])};
-            else
-                *(f32x4*)(op + d) = (f32x4){x[0], x[1], x[2], x[3]};
-        }
+        for (int i = 0; i < 16; ++i) ws[(v * 16 + i) * 64 + lane] = r.acc[v][i];
+    if (lh == 0) {
+        ws[NV * 16 * 64 + lc] = r.mx;
+        ws[NV * 16 * 64 + 32 + lc] = r.sum;
+    }
 }
+
+// the shares of 32 rows, in their order: a wave per block of 32 columns
+template <typename T, int DP>
+__global__ __launch_bounds__(64 * (DP / 32)) void attn_join(va_tok_attn_args a, int nrb, int nsplit) {
+    constexpr int NV = DP / 32;
+    const int lane = threadIdx.x & 63, v = threadIdx.x >> 6, lc = lane & 31, lh = lane >> 5, G = a.Hq / a.Hk;
+    const int rb = blockIdx.x % nrb, unit = blockIdx.x / nrb, hk = unit % a.Hk, b = unit / a.Hk;
+    const AttnSeq sq = attn_seq(a, b);
+    const int row = rb * 32 + lc, s = row / G, g = row - s * G;
+    if (row >= sq.ql * G) return;
+    const float cexp = a.scale * 1.4426950408889634f;
+    const float* ws = (const float*)a.ws + (int64_t)(unit * nrb + rb) * nsplit * part_floats(NV);
+    float mx = -INFINITY;
+    for (int i = 0; i < nsplit; ++i) mx = fmaxf(mx, ws[i * part_floats(NV) + NV * 16 * 64 + lc]);
+    const float base = mx == -INFINITY ? 0.0f : mx;
+    float sum = 0.0f;
+    f32x16 acc;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) acc[j] = 0.0f;
+    for (int i = 0; i < nsplit; ++i) {
+        const float* p = ws + i * part_floats(NV);
+        const float y = __builtin_amdgcn_exp2f((p[NV * 16 * 64 + lc] - base) * cexp);
+        sum += p[NV * 16 * 64 + 32 + lc] * y;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) acc[j] += p[(v * 16 + j) * 64 + lane] * y;
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    store_block<T>((T*)a.o + b * a.o_sb + s * a.o_ss + (int64_t)(hk * G + g) * a.o_sh, acc, inv, v, lh, a.Dv);
+}
+
+constexpr int64_t ROW_MAX = 1 << 22;  // elements between slots: a tile's offsets stay within 31 bits
 
 bool attn_ok(const va_tok_attn_args& a) {
     if (a.B < 0 || a.S < 0 || a.Hk < 1 || a.Hq < a.Hk || a.Hq % a.Hk || a.slots < 0) return false;
@@ -297,38 +569,93 @@ bool attn_ok(const va_tok_attn_args& a) {
     if (!(a.scale > 0.0f) || !(a.scale < INFINITY)) return false;
     if ((int64_t)a.S * (a.Hq / a.Hk) > INT32_MAX - 256) return false;
     const int64_t st = a.q_sb | a.q_ss | a.q_sh | a.k_sb | a.k_ss | a.k_sh | a.v_sb | a.v_ss | a.v_sh | a.o_sb | a.o_ss | a.o_sh;
-    if (st % 8) return false;
+    if (st % 8 || a.k_ss >= ROW_MAX || a.v_ss >= ROW_MAX) return false;
     const bool some = a.B > 0 && a.S > 0;
     if (some && (!a.q || !a.o || (a.slots && (!a.k || !a.v)))) return false;
     return !(((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.o) & 15);
 }
 
-template <typename T>
-hipError_t attn_go(const va_tok_attn_args& a, hipStream_t st, dim3 grid, int ntiles) {
-    switch ((max(a.D, a.Dv) + 31) / 32) {
-        case 1: hipLaunchKernelGGL((attn_kernel<T, 32>), grid, dim3(256), 0, st, a, ntiles); break;
-        case 2: hipLaunchKernelGGL((attn_kernel<T, 64>), grid, dim3(256), 0, st, a, ntiles); break;
-        case 3: hipLaunchKernelGGL((attn_kernel<T, 96>), grid, dim3(256), 0, st, a, ntiles); break;
-        default: hipLaunchKernelGGL((attn_kernel<T, 128>), grid, dim3(256), 0, st, a, ntiles);
+// How a call is split: rows of 128 through LDS (nsplit 0), or 32 rows a workgroup with the keys in nsplit shares.
+struct Plan {
+    int nrb, nsplit;
+};
+
+Plan attn_plan(const va_tok_attn_args& a) {
+    const int64_t rows = (int64_t)a.S * (a.Hq / a.Hk), units = (int64_t)a.B * a.Hk;
+    if (rows > 32) return {(int)((rows + 127) / 128), 0};
+    int64_t keys = a.slots;  // the most that a row block can see
+    if (a.window) keys = min(keys, (int64_t)a.sinks + a.window + a.S + a.frame);
+    const int64_t nrb = (rows + 31) / 32;
+    // two workgroups for each of the 256 CUs, and 256 keys at least to a share
+    const int64_t want = (512 + units * nrb - 1) / (units * nrb), most = (keys + 255) / 256;
+    return {(int)nrb, (int)max((int64_t)1, min(want, most))};
+}
+
+int64_t part_bytes(const va_tok_attn_args& a) { return (((max(a.D, a.Dv) + 31) / 32) * 16 * 64 + 64) * 4; }
+
+// a kernel's dynamic LDS beyond 64 KiB, once a device
+template <int LDS, typename K>
+hipError_t big_lds(K kernel) {
+    static DevFlag attr;
+    if (LDS <= 65536 || attr()) return hipSuccess;
+    const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+    if (e == hipSuccess) attr() = true;
+    return e;
+}
+
+template <typename T, int DP>
+hipError_t attn_go(const va_tok_attn_args& a, hipStream_t st, Plan p) {
+    const unsigned units = (unsigned)(a.B * a.Hk);
+    if (p.nsplit == 0) {
+        constexpr int lds = 4 * Tr<T>::KT * Dims<T, DP>::CS * 16;
+        if (hipError_t e = big_lds<lds>(attn_kernel<T, DP>)) return e;
+        hipLaunchKernelGGL((attn_kernel<T, DP>), dim3(units * p.nrb), dim3(256), lds, st, a, p.nrb);
+        return hipGetLastError();
     }
-    return hipGetLastError();
+    constexpr int lds = Dims<T, DP>::SLDS;
+    hipError_t e = big_lds<lds>(attn_split<T, DP>);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((attn_split<T, DP>), dim3(units * p.nrb * p.nsplit), dim3(64 * Dims<T, DP>::SW), lds, st, a, p.nrb,
+                       p.nsplit);
+    e = hipGetLastError();
+    if (e == hipSuccess && p.nsplit > 1) {
+        hipLaunchKernelGGL((attn_join<T, DP>), dim3(units * p.nrb), dim3(64 * (DP / 32)), 0, st, a, p.nrb, p.nsplit);
+        e = hipGetLastError();
+    }
+    return e;
+}
+
+template <typename T>
+hipError_t attn_type(const va_tok_attn_args& a, hipStream_t st, Plan p) {
+    switch ((max(a.D, a.Dv) + 31) / 32) {
+        case 1: return attn_go<T, 32>(a, st, p);
+        case 2: return attn_go<T, 64>(a, st, p);
+        case 3: return attn_go<T, 96>(a, st, p);
+        default: return attn_go<T, 128>(a, st, p);
+    }
 }
 
 }  // namespace
 
 extern "C" {
 
-int64_t va_tok_attn_workspace_bytes(const va_tok_attn_args* a) { return a && attn_ok(*a) ? 0 : VA_ERR_ARG; }
+int64_t va_tok_attn_workspace_bytes(const va_tok_attn_args* a) {
+    if (!a || !attn_ok(*a)) return VA_ERR_ARG;
+    if (a->B == 0 || a->S == 0) return 0;
+    const Plan p = attn_plan(*a);
+    return p.nsplit > 1 ? (int64_t)a->B * a->Hk * p.nrb * p.nsplit * part_bytes(*a) : 0;
+}
 
 int va_tok_attn(void* stream, const va_tok_attn_args* ap) {
     if (!ap || !attn_ok(*ap)) return VA_ERR_ARG;
     const va_tok_attn_args& a = *ap;
     if (a.B == 0 || a.S == 0) return VA_OK;
-    const int64_t ntiles = ((int64_t)a.S * (a.Hq / a.Hk) + 127) / 128, blocks = ntiles * a.Hk * a.B;
-    if (blocks > INT32_MAX) return VA_ERR_RANGE;
-    const dim3 grid((unsigned)blocks);
-    const hipError_t e = a.dtype == VA_DTYPE_F32 ? attn_go<float>(a, (hipStream_t)stream, grid, (int)ntiles)
-                                                 : attn_go<__bf16>(a, (hipStream_t)stream, grid, (int)ntiles);
+    const Plan p = attn_plan(a);
+    if ((int64_t)a.B * a.Hk * p.nrb * max(p.nsplit, 1) > INT32_MAX) return VA_ERR_RANGE;
+    const int64_t need = va_tok_attn_workspace_bytes(ap);
+    if (need > 0 && (!a.ws || a.ws_bytes < need || ((uintptr_t)a.ws & 15))) return VA_ERR_ARG;
+    const hipError_t e = a.dtype == VA_DTYPE_F32 ? attn_type<float>(a, (hipStream_t)stream, p)
+                                                 : attn_type<__bf16>(a, (hipStream_t)stream, p);
     return e == hipSuccess ? VA_OK : VA_ERR_HIP;
 }
 
