@@ -561,8 +561,8 @@ typedef struct va_tok_linear_args {
     const void* w;          /* packed weights, 16-byte aligned, zeros from row N and column K on, Kpad % 64 == 0,
                                Npad % 64 == 0:
                                BF16: bf16 [Npad][Kpad];  F32 (six exact term products each, float sums; values below bf16's largest, 3.38e38, in
-                               size): three exact bf16 terms [Npad][Kpad / 8][3][8] (the 8 h,
-                               then the 8 m, then the 8 l of a group: va_conv_args.w3 with K in its own order);
+                               size): bf16 [3][Npad][Kpad], the weights' exact terms h, m, l (w = h + m + l, each
+                               the round-to-nearest bf16 of what remains);
                                w8 = 1 (BF16): e4m3 bytes [Npad][Kpad], in va_conv_args.w8's order inside a 64-block */
     const float* wscale;    /* w8: [Npad] scale of each row, else NULL */
     const float* bias;      /* [N] or NULL */

@@ -73,4 +73,25 @@ __device__ __forceinline__ float activate(float x, int act) {
     }
 }
 
+// The same for a result that is rounded to bf16 (2^-9): hardware reciprocal and exponential, and for the Gaussian tail
+// Abramowitz and Stegun 7.1.26 (absolute error 7.5e-8): x Phi(x) = max(x, 0) - |x| erfc(|x| / sqrt 2) / 2, the tail as a
+// polynomial in t = 1 / (1 + 0.3275911 |x| / sqrt 2) times exp(-x^2 / 2).  20 issue slots against erfcf's 60: in a product
+// with K = 1024 the activations of a tile would take longer than its MFMAs.
+__device__ __forceinline__ float activate_bf16(float x, int act) {
+    switch (act) {
+        case VA_ACT_SILU:
+            return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * x));
+        case VA_ACT_GELU: {
+            const float z = fminf(fabsf(x), 1e4f), t = __builtin_amdgcn_rcpf(__builtin_fmaf(z, 0.23164189f, 1.0f));
+            const float p = t * __builtin_fmaf(t, __builtin_fmaf(t, __builtin_fmaf(t, __builtin_fmaf(t, 0.530702715f,
+                            -0.7265760135f), 0.7107068705f), -0.142248368f), 0.127414796f);
+            return __builtin_fmaf(-z, p * __builtin_amdgcn_exp2f(-0.72134752f * x * x), fmaxf(x, 0.0f));
+        }
+        case VA_ACT_GELU_TANH:
+            return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-2.3022081987f * __builtin_fmaf(0.044715f * x * x, x, x)));
+        case VA_ACT_RELU: return x < 0.0f ? 0.0f : x;
+        default: return x;
+    }
+}
+
 }  // namespace tok

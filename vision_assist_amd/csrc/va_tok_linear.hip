@@ -2,13 +2,14 @@
 //
 // The weights are the MFMA's A operand (its rows are output channels) and the tokens its B operand, so a lane's
 // accumulator registers are consecutive channels of one token: the epilogue stores them as vectors.
+#include "va_dev.h"
 #include "va_tok.h"
 
 namespace {
 using namespace tok;
 
 // four consecutive channels n .. n + 3 of token m from the accumulator: scale, bias, activation, residual, store.
-// vec: y, res rows are aligned for four values and n + 3 < N
+// vec: y and res rows are aligned for four values (1), for eight (2)
 struct Out {
     const float *wscale, *bias;
     const void* res;
@@ -26,7 +27,7 @@ __device__ __forceinline__ void finish4(const Out& o, int m, int n, f32x4 v) {
         float t = v[i];
         if (o.wscale) t *= o.wscale[c];
         if (o.bias) t += o.bias[c];
-        r[i] = activate(t, o.act);
+        r[i] = o.f32out ? activate(t, o.act) : activate_bf16(t, o.act);
     }
     if (o.vec && n + 3 < o.N) {
         if (o.res) {
@@ -80,9 +81,9 @@ __global__ __launch_bounds__(256) void linear_any(va_tok_linear_args a, Out o, i
         const int k = k0 + 8 * ch;
         bf16x8 wt[T], xt[T];
         if constexpr (FORM == F32) {
-            const bf16x8* p = (const bf16x8*)a.w + ((int64_t)(n0 + row) * (a.Kpad / 8) + k / 8) * 3;
 #pragma unroll
-            for (int t = 0; t < 3; ++t) wt[t] = p[t];
+            for (int t = 0; t < 3; ++t)
+                wt[t] = *(const bf16x8*)((const __bf16*)a.w + ((int64_t)t * a.Npad + n0 + row) * a.Kpad + k);
         } else if constexpr (FORM == W8) {
             const int c = k / 8, pos = (c & ~7) | ((c & 3) << 1) | ((c >> 2) & 1);
             wt[0] = e4m3x8(*(const uint2*)((const uint8_t*)a.w + (int64_t)(n0 + row) * a.Kpad + 8 * pos));
@@ -135,6 +136,339 @@ __global__ __launch_bounds__(256) void linear_any(va_tok_linear_args a, Out o, i
             finish4(o, m0 + 32 * wm + 16 * j + fr, n0 + 32 * wn + 16 * i + 4 * fq, acc[i][j]);
 }
 
+// the six term products that are kept of (h + m + l)(h + m + l)
+constexpr int NTERM = 6, TERM_W[6] = {0, 0, 1, 0, 1, 2}, TERM_X[6] = {0, 1, 0, 2, 1, 0};
+
+// ------------------------------------------------------------------ many tiles: LDS-DMA ring, counted waits
+// 64 WN channels x 64 WM tokens per workgroup, four waves of 32 WN x 32 WM on v_mfma_f32_32x32x16_bf16, K in steps of 32
+// through a ring of NS stages.  A step is two slices of 16; the fragments of a slice are read while the MFMAs of the slice
+// before run.  One barrier a step, after its first slice: by then every wave has read the whole step (its second slice's
+// fragments have arrived), so its stage is free and step t + NS is sent into it; and the wait before the barrier has
+// retired step t + 1's DMAs, whose fragments are read next, while those of t + 2 .. t + NS - 1 stay in flight.
+// Two workgroups share a CU: the epilogue of one (activations: VALU) runs beside the MFMAs of the other.
+//   rows of a stage: 64 bytes (bf16: 32 values), piece p of row r in place p ^ ((r >> 1) & 3); F32's x 128 bytes, place
+//   p ^ (r & 7); e4m3 weights 32 bytes, piece p in place p ^ ((r >> 2) & 1): eight lanes' 16 bytes cover the banks
+//   weight rows are staged in an order that leaves a lane 16 consecutive channels of its token in its registers
+constexpr int LIN_OOB = 0x7ffffff0;      // an offset that a descriptor of that many bytes answers with zeros
+constexpr int LIN_ROW = 1 << 21;         // longest rows in values: the offsets of 256 of them stay within 31 bits
+
+__device__ __forceinline__ void dma16(const void* base, void* lds, int off, int uniform) {
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, LIN_OOB, 0x00020000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lvoid_t*)lds, 16, off, uniform, 0, 0);
+}
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// eight consecutive channels of a token, through every type and alignment
+__device__ __forceinline__ void finish8(const Out& o, int m, int n, float (&r)[8], const float (&scale)[8], const float (&bias)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = __builtin_fmaf(r[i], scale[i], bias[i]);
+    if (o.f32out) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r[i] = activate(r[i], o.act);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r[i] = activate_bf16(r[i], o.act);
+    }
+    if (o.vec == 2 && n + 7 < o.N) {
+        if (o.res) {
+            if (o.f32in) {
+                const f32x4* q = (const f32x4*)((const float*)o.res + (int64_t)m * o.ldr + n);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) r[i] += q[i / 4][i % 4];
+            } else {
+                const u32x4 q = *(const u32x4*)((const __bf16*)o.res + (int64_t)m * o.ldr + n);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) r[2 * e] += bf_lo(q[e]), r[2 * e + 1] += bf_hi(q[e]);
+            }
+        }
+        if (o.f32out) {
+            f32x4* y = (f32x4*)((float*)o.y + (int64_t)m * o.ldy + n);
+            y[0] = (f32x4){r[0], r[1], r[2], r[3]}, y[1] = (f32x4){r[4], r[5], r[6], r[7]};
+        } else {
+            *(u32x4*)((__bf16*)o.y + (int64_t)m * o.ldy + n) =
+                (u32x4){pk_bf16(r[0], r[1]), pk_bf16(r[2], r[3]), pk_bf16(r[4], r[5]), pk_bf16(r[6], r[7])};
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if (n + i >= o.N) return;
+        const int64_t at = (int64_t)m * o.ldy + n + i;
+        if (o.res) r[i] += o.f32in ? ((const float*)o.res)[(int64_t)m * o.ldr + n + i]
+                                   : (float)((const __bf16*)o.res)[(int64_t)m * o.ldr + n + i];
+        if (o.f32out)
+            ((float*)o.y)[at] = r[i];
+        else
+            ((__bf16*)o.y)[at] = (__bf16)r[i];
+    }
+}
+
+template <Form F, int WN, int WM>
+struct TileCfg {
+    static constexpr int BN = 64 * WN, BM = 64 * WM, T = F == F32 ? 3 : 1;
+    static constexpr int WROW = F == W8 ? 32 : 64, XROW = F == F32 ? 128 : 64;   // bytes of a staged row
+    static constexpr int WPL = BN * WROW, WB = T * WPL, XB = BM * XROW, STAGE = WB + XB;
+    static constexpr int ND = STAGE / 4096;                                       // DMAs of a wave and step
+    static constexpr int NS = 3 * STAGE <= 80 * 1024 ? 3 : 2;
+    // the epilogue's blocks: a wave's 32 tokens x 32 WN channels of float, rows padded by 16 bytes
+    static constexpr int EROW = (32 * WN + 4) * 4, EPI = 4 * 32 * EROW, LDS = NS * STAGE > EPI ? NS * STAGE : EPI;
+    static_assert(STAGE % 4096 == 0 && LDS <= 80 * 1024, "two workgroups a CU");
+};
+
+template <Form F, int WN, int WM>
+__global__ __launch_bounds__(256, 2) void linear_tile(va_tok_linear_args a, Out o, int ntn) {
+    using C = TileCfg<F, WN, WM>;
+    constexpr int NS = C::NS, ND = C::ND, T = C::T;
+    extern __shared__ __align__(16) unsigned char sm[];
+    const int tile = xcd_tile(blockIdx.x, gridDim.x);
+    const int n0 = tile % ntn * C::BN, m0 = tile / ntn * C::BM;
+    const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lc = lane & 31, lh = lane >> 5;
+    const int wn = wid & 1, wm = wid >> 1;
+    constexpr int XE = F == F32 ? 4 : 2;
+    // this lane's DMAs: instruction d = wid * ND + j fills bytes [1024 d, 1024 d + 1024) of a stage
+    int off[ND], kc[ND];  // byte offset of the piece from its operand's tile; for x its first k of a step
+#pragma unroll
+    for (int j = 0; j < ND; ++j) {
+        const int at = (wid * ND + j) * 1024 + lane * 16;
+        if (at < C::WB) {
+            const int in = at % C::WPL, r = in / C::WROW, q = in % C::WROW / 16;
+            const int p = F == W8 ? q ^ ((r >> 2) & 1) : q ^ ((r >> 1) & 3);
+            const int ch = (r & ~31) + 16 * ((r >> 2) & 1) + 4 * ((r & 31) >> 3) + (r & 3);  // the channel of this row
+            off[j] = n0 + ch < a.Npad ? ch * a.Kpad * (F == W8 ? 1 : 2) + 16 * p : LIN_OOB;
+            kc[j] = -1;
+        } else {
+            const int in = at - C::WB, r = in / C::XROW, q = in % C::XROW / 16;
+            const int p = F == F32 ? q ^ (r & 7) : q ^ ((r >> 1) & 3);
+            // e4m3: a step's four bytes-of-8 are chunks c, c + 4, c + 1, c + 5 of the 64-block (c = 0 or 2)
+            kc[j] = F == W8 ? (p & 1) * 32 + (p >> 1) * 8 : p * (16 / XE);
+            off[j] = m0 + r < a.M ? (int)(r * a.ldx + kc[j]) * XE : LIN_OOB;
+        }
+    }
+    const int nk = F == W8 ? 2 * ((a.K + 63) / 64) : (a.K + 31) / 32;
+    const unsigned char* xb = (const unsigned char*)a.x + (int64_t)m0 * a.ldx * XE;
+    const unsigned char* wb = (const unsigned char*)a.w + (int64_t)n0 * a.Kpad * (F == W8 ? 1 : 2);
+    const int64_t plane = (int64_t)a.Npad * a.Kpad * 2;
+    auto issue = [&](int t, int stage) {
+        const int k0 = F == W8 ? (t >> 1) * 64 + (t & 1) * 16 : t * 32;  // x's first k
+        unsigned char* to = sm + stage * C::STAGE;
+#pragma unroll
+        for (int j = 0; j < ND; ++j) {
+            const int d = (wid * ND + j) * 1024;  // uniform
+            const bool isw = d < C::WB;
+            const unsigned char* base = isw ? wb + (T > 1 ? d / C::WPL * plane : 0) : xb;
+            const int v = kc[j] >= 0 && k0 + kc[j] >= a.K ? LIN_OOB : off[j];
+            dma16(base, to + d, v, isw ? t * C::WROW : k0 * XE);
+        }
+    };
+    f32x16 acc[WN][WM];
+#pragma unroll
+    for (int i = 0; i < WN; ++i)
+#pragma unroll
+        for (int j = 0; j < WM; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+
+    struct Frag {
+        bf16x8 w[WN][T], x[WM][T];
+    };
+    auto read = [&](Frag& f, int stage, int ks) {
+        const unsigned char* ws = sm + stage * C::STAGE;
+        const unsigned char* xs = ws + C::WB;
+        const int p = 2 * ks + lh;  // this lane's piece of 8 values
+#pragma unroll
+        for (int i = 0; i < WN; ++i) {
+            const int r = 32 * (wn * WN + i) + lc;
+            if constexpr (F == W8) {
+                f.w[i][0] = e4m3x8(*(const uint2*)(ws + r * 32 + 16 * (ks ^ ((r >> 2) & 1)) + 8 * lh));
+            } else {
+#pragma unroll
+                for (int t = 0; t < T; ++t)
+                    f.w[i][t] = *(const bf16x8*)(ws + t * C::WPL + r * 64 + 16 * (p ^ ((r >> 1) & 3)));
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < WM; ++j) {
+            const int r = 32 * (wm * WM + j) + lc;
+            if constexpr (F == F32) {
+                const f32x4 u = *(const f32x4*)(xs + r * 128 + 16 * ((2 * p) ^ (r & 7)));
+                const f32x4 v = *(const f32x4*)(xs + r * 128 + 16 * ((2 * p + 1) ^ (r & 7)));
+                const float e[8] = {u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
+                split3(e, f.x[j]);
+            } else {
+                f.x[j][0] = *(const bf16x8*)(xs + r * 64 + 16 * (p ^ ((r >> 1) & 3)));
+            }
+        }
+    };
+    auto mma = [&](const Frag& f) {
+#pragma unroll
+        for (int t = 0; t < (T > 1 ? NTERM : 1); ++t)
+#pragma unroll
+            for (int i = 0; i < WN; ++i)
+#pragma unroll
+                for (int j = 0; j < WM; ++j)
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.w[i][T > 1 ? TERM_W[t] : 0], f.x[j][T > 1 ? TERM_X[t] : 0],
+                                                                        acc[i][j], 0, 0, 0);
+    };
+#pragma unroll
+    for (int t = 0; t < NS; ++t)
+        if (t < nk) issue(t, t);
+    if (nk >= NS)
+        wait_vm<(NS - 1) * ND>();
+    else
+        wait_vm<0>();
+    asm volatile("s_barrier" ::: "memory");
+    Frag f0, f1;
+    read(f0, 0, 0);
+    int stage = 0;
+    for (int t = 0; t < nk; ++t) {
+        const int next = stage + 1 == NS ? 0 : stage + 1;
+        read(f1, stage, 1);
+        __builtin_amdgcn_sched_barrier(0);
+        mma(f0);
+        __builtin_amdgcn_sched_barrier(0);
+        // this step's fragments are in registers, the next step's DMAs are done (those of the steps behind it may fly on)
+        if (t + NS - 1 < nk)
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NS - 2) * ND) : "memory");
+        else
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (t + NS < nk) issue(t + NS, stage);
+        if (t + 1 < nk) read(f0, next, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        mma(f1);
+        stage = next;
+    }
+    // 32 tokens at a time through the wave's part of LDS, so that its stores are whole runs of a token's channels: 4 WN
+    // lanes hold a token's 32 WN channels, eight each (their bias and scale are loaded once)
+    __syncthreads();
+    unsigned char* es = sm + wid * 32 * C::EROW;
+    constexpr int LR = 4 * WN, RI = 64 / LR;  // lanes of a token, tokens an iteration
+    const int er = lane / LR, ec = lane % LR * 8, n = n0 + 32 * WN * wn + ec;
+    float scale[8], bias[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const int c = min(n + e, a.N - 1);
+        scale[e] = o.wscale ? o.wscale[c] : 1.0f;
+        bias[e] = o.bias ? o.bias[c] : 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < WM; ++j) {
+#pragma unroll
+        for (int i = 0; i < WN; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4)
+                *(f32x4*)(es + lc * C::EROW + (32 * i + 16 * lh + e) * 4) =
+                    (f32x4){acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]};
+#pragma unroll 1
+        for (int it = 0; it < 32 / RI; ++it) {
+            const int row = it * RI + er, m = m0 + 32 * (wm * WM + j) + row;
+            const f32x4 u = *(const f32x4*)(es + row * C::EROW + ec * 4), v = *(const f32x4*)(es + row * C::EROW + ec * 4 + 16);
+            float r[8] = {u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
+            if (m < o.M && n < o.N) finish8(o, m, n, r, scale, bias);
+        }
+    }
+}
+
+// ------------------------------------------------------------------ few tiles: K over the waves of a workgroup
+// 16 channels x 16 MB tokens per workgroup; its eight waves take every eighth block of 64 of K, straight from memory into
+// the fragments (weights are read once, the tokens' values come from the L2), and their sums are joined in LDS in the
+// waves' order.  v_mfma_f32_16x16x32_bf16.
+template <Form F, int MB>
+__global__ __launch_bounds__(512) void linear_few(va_tok_linear_args a, Out o, int ntn) {
+    constexpr int T = F == F32 ? 3 : 1, NW = 8;
+    __shared__ f32x4 part[NW][MB][64];
+    const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fr = lane & 15, fq = lane >> 4;
+    const int n0 = blockIdx.x % ntn * 16, m0 = blockIdx.x / ntn * 16 * MB;
+    const int nk = (a.K + 63) / 64;
+    int64_t xrow[MB];
+#pragma unroll
+    for (int j = 0; j < MB; ++j) xrow[j] = (int64_t)min(m0 + 16 * j + fr, a.M - 1) * a.ldx;
+    f32x4 acc[MB];
+#pragma unroll
+    for (int j = 0; j < MB; ++j) acc[j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+    struct Raw {
+        u32x4 w[F == W8 ? 1 : 2 * T], x[2][MB][F == F32 ? 2 : 1];
+    };
+    auto load = [&](Raw& r, int kb) {
+        const int k = kb * 64 + 8 * fq;
+        if constexpr (F == W8) {  // one 16-byte piece: chunks fq and fq + 4
+            r.w[0] = *(const u32x4*)((const uint8_t*)a.w + (int64_t)(n0 + fr) * a.Kpad + kb * 64 + 16 * fq);
+        } else {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int t = 0; t < T; ++t)
+                    r.w[h * T + t] = *(const u32x4*)((const __bf16*)a.w + ((int64_t)t * a.Npad + n0 + fr) * a.Kpad + k + 32 * h);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < MB; ++j) {
+                const int kk = k + 32 * h;
+                if constexpr (F == F32) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        r.x[h][j][e] = kk + 4 * e < a.K ? *(const u32x4*)((const float*)a.x + xrow[j] + kk + 4 * e) : (u32x4){0, 0, 0, 0};
+                } else {
+                    r.x[h][j][0] = kk < a.K ? *(const u32x4*)((const __bf16*)a.x + xrow[j] + kk) : (u32x4){0, 0, 0, 0};
+                }
+            }
+    };
+    auto mma = [&](const Raw& r) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            bf16x8 w[T];
+#pragma unroll
+            for (int t = 0; t < T; ++t)
+                w[t] = F == W8 ? e4m3x8(make_uint2(r.w[0][2 * h], r.w[0][2 * h + 1])) : (bf16x8)r.w[h * T + t];
+#pragma unroll
+            for (int j = 0; j < MB; ++j) {
+                bf16x8 x[T];
+                if constexpr (F == F32) {
+                    float e[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) e[i] = __uint_as_float(r.x[h][j][i / 4][i % 4]);
+                    split3(e, x);
+                } else {
+                    x[0] = (bf16x8)r.x[h][j][0];
+                }
+#pragma unroll
+                for (int t = 0; t < (T > 1 ? NTERM : 1); ++t)
+                    acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[T > 1 ? TERM_W[t] : 0], x[T > 1 ? TERM_X[t] : 0], acc[j], 0, 0, 0);
+            }
+        }
+    };
+    // blocks in pairs: the next pair's loads are in flight while this pair is worked on
+    constexpr int U = MB >= 4 || F == F32 ? 1 : 2;
+    Raw cur[U], nxt[U];
+    int kb = wid;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (kb + u * NW < nk) load(cur[u], kb + u * NW);
+    for (; kb < nk; kb += U * NW) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (kb + (U + u) * NW < nk) load(nxt[u], kb + (U + u) * NW);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (kb + u * NW < nk) mma(cur[u]);
+#pragma unroll
+        for (int u = 0; u < U; ++u) cur[u] = nxt[u];
+    }
+#pragma unroll
+    for (int j = 0; j < MB; ++j) part[wid][j][lane] = acc[j];
+    __syncthreads();
+    for (int i = threadIdx.x; i < MB * 64; i += 64 * NW) {
+        const int j = i / 64;
+        f32x4 v = part[0][j][lane];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) v += part[w][j][lane];
+        finish4(o, m0 + 16 * j + fr, n0 + 4 * fq, v);
+    }
+}
+
 bool linear_ok(const va_tok_linear_args& a) {
     if (a.M < 0 || a.N <= 0 || a.K <= 0 || !a.w || !a.y || (a.M > 0 && !a.x)) return false;
     if (a.dtype != VA_DTYPE_BF16 && a.dtype != VA_DTYPE_F32) return false;
@@ -149,24 +483,70 @@ bool linear_ok(const va_tok_linear_args& a) {
 
 }  // namespace
 
+namespace {
+template <Form F, int WN, int WM>
+hipError_t go_tile(const va_tok_linear_args& a, const Out& o, hipStream_t st) {
+    using C = TileCfg<F, WN, WM>;
+    constexpr int lds = C::LDS;
+    static DevFlag attr;
+    if (lds > 65536 && !attr()) {
+        const hipError_t e = hipFuncSetAttribute((const void*)linear_tile<F, WN, WM>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        if (e != hipSuccess) return e;
+        attr() = true;
+    }
+    const int ntn = (a.N + C::BN - 1) / C::BN, ntm = (a.M + C::BM - 1) / C::BM;
+    hipLaunchKernelGGL((linear_tile<F, WN, WM>), dim3((unsigned)(ntn * ntm)), dim3(256), lds, st, a, o, ntn);
+    return hipGetLastError();
+}
+
+template <Form F, int MB>
+hipError_t go_few(const va_tok_linear_args& a, const Out& o, hipStream_t st) {
+    const int ntn = (a.N + 15) / 16, ntm = (a.M + 16 * MB - 1) / (16 * MB);
+    hipLaunchKernelGGL((linear_few<F, MB>), dim3((unsigned)(ntn * ntm)), dim3(512), 0, st, a, o, ntn);
+    return hipGetLastError();
+}
+
+template <Form F>
+hipError_t go_any(const va_tok_linear_args& a, const Out& o, hipStream_t st, int xvec) {
+    const int ntn = (a.N + GB - 1) / GB, ntm = (a.M + GB - 1) / GB;
+    hipLaunchKernelGGL(linear_any<F>, dim3((unsigned)(ntn * ntm)), dim3(256), 0, st, a, o, ntn, xvec);
+    return hipGetLastError();
+}
+
+template <Form F>
+hipError_t go(const va_tok_linear_args& a, const Out& o, hipStream_t st) {
+    constexpr int E = F == F32 ? 4 : 8;
+    const int xvec = a.ldx % 8 == 0 && !((uintptr_t)a.x & 15);
+    if (a.K % E || a.ldx % E || ((uintptr_t)a.x & 15) || a.ldx > LIN_ROW || a.Kpad > LIN_ROW) return go_any<F>(a, o, st, xvec);
+    const int64_t t64 = (int64_t)((a.N + 63) / 64) * ((a.M + 63) / 64);
+    if (a.M <= 16) return go_few<F, 1>(a, o, st);
+    if (a.M <= 32) return go_few<F, 2>(a, o, st);
+    if (a.M <= 64 || t64 < 128) return go_few<F, 4>(a, o, st);
+    if constexpr (F == F32) {
+        return t64 < 1024 ? go_tile<F32, 1, 1>(a, o, st) : go_tile<F32, 2, 1>(a, o, st);
+    } else {
+        const int64_t big = (int64_t)((a.N + 255) / 256) * ((a.M + 127) / 128);
+        if (big >= 384) return go_tile<F, 4, 2>(a, o, st);
+        return go_tile<F, 2, 1>(a, o, st);
+    }
+}
+}  // namespace
+
 extern "C" int va_tok_linear(void* stream, const va_tok_linear_args* ap) {
     if (!ap || !linear_ok(*ap)) return VA_ERR_ARG;
     const va_tok_linear_args& a = *ap;
     if (a.M == 0) return VA_OK;
+    if ((int64_t)((a.N + 15) / 16) * ((a.M + 15) / 16) > INT32_MAX) return VA_ERR_RANGE;
     const bool f32 = a.dtype == VA_DTYPE_F32;
     Out o = {a.wscale, a.bias, a.res, a.y, a.ldr, a.ldy, a.M, a.N, a.act, f32, f32 || a.out_f32, 0};
-    o.vec = a.ldy % 4 == 0 && !((uintptr_t)a.y & (o.f32out ? 15 : 7)) &&
-            (!a.res || (a.ldr % 4 == 0 && !((uintptr_t)a.res & (f32 ? 15 : 7))));
-    const int64_t ntn = (a.N + GB - 1) / GB, tiles = ntn * ((a.M + GB - 1) / GB);
-    if (tiles > INT32_MAX) return VA_ERR_RANGE;
-    const int xvec = a.ldx % 8 == 0 && !((uintptr_t)a.x & 15);
-    const dim3 grid((unsigned)tiles), block(256);
+    // stores of 4 channels (1), of 8 (2)
+    const auto rows = [&](int n) {
+        const int eo = o.f32out ? 4 : 2, ei = f32 ? 4 : 2, bo = n * eo < 16 ? n * eo : 16, bi = n * ei < 16 ? n * ei : 16;
+        return a.ldy * eo % bo == 0 && !((uintptr_t)a.y & (uintptr_t)(bo - 1)) &&
+               (!a.res || (a.ldr * ei % bi == 0 && !((uintptr_t)a.res & (uintptr_t)(bi - 1))));
+    };
+    o.vec = rows(8) ? 2 : rows(4) ? 1 : 0;
     hipStream_t st = (hipStream_t)stream;
-    if (f32)
-        hipLaunchKernelGGL(linear_any<F32>, grid, block, 0, st, a, o, (int)ntn, xvec);
-    else if (a.w8)
-        hipLaunchKernelGGL(linear_any<W8>, grid, block, 0, st, a, o, (int)ntn, xvec);
-    else
-        hipLaunchKernelGGL(linear_any<BF16>, grid, block, 0, st, a, o, (int)ntn, xvec);
-    return hipGetLastError() == hipSuccess ? VA_OK : VA_ERR_HIP;
+    const hipError_t e = f32 ? go<F32>(a, o, st) : a.w8 ? go<W8>(a, o, st) : go<BF16>(a, o, st);
+    return e == hipSuccess ? VA_OK : VA_ERR_HIP;
 }

@@ -198,7 +198,7 @@ class Linear:
             self.wscale[:N] = scale.detach().to(self.device, torch.float32)
             self.w = w8_order(padded(w.view(torch.uint8)))
         elif dtype == "f32":
-            self.w = split3_bf16(padded(w.float()))
+            self.w = split3_bf16(padded(w.float())).permute(2, 0, 1, 3).reshape(3, Np, Kp).contiguous()
         else:
             self.w = padded(w.to(torch.bfloat16))
         self.bias = None if bias is None else bias.detach().to(self.device, torch.float32).contiguous()
