@@ -94,4 +94,28 @@ __device__ __forceinline__ float activate_bf16(float x, int act) {
     }
 }
 
+// n results at once: one (uniform) branch for all of them
+template <bool EXACT, int N>
+__device__ __forceinline__ void activate_n(float (&r)[N], int act) {
+    switch (act) {
+        case VA_ACT_SILU:
+#pragma unroll
+            for (int i = 0; i < N; ++i) r[i] = EXACT ? activate(r[i], VA_ACT_SILU) : activate_bf16(r[i], VA_ACT_SILU);
+            break;
+        case VA_ACT_GELU:
+#pragma unroll
+            for (int i = 0; i < N; ++i) r[i] = EXACT ? activate(r[i], VA_ACT_GELU) : activate_bf16(r[i], VA_ACT_GELU);
+            break;
+        case VA_ACT_GELU_TANH:
+#pragma unroll
+            for (int i = 0; i < N; ++i) r[i] = EXACT ? activate(r[i], VA_ACT_GELU_TANH) : activate_bf16(r[i], VA_ACT_GELU_TANH);
+            break;
+        case VA_ACT_RELU:
+#pragma unroll
+            for (int i = 0; i < N; ++i) r[i] = activate(r[i], VA_ACT_RELU);
+            break;
+        default: break;
+    }
+}
+
 }  // namespace tok

@@ -2,6 +2,8 @@
 //
 // The weights are the MFMA's A operand (its rows are output channels) and the tokens its B operand, so a lane's
 // accumulator registers are consecutive channels of one token: the epilogue stores them as vectors.
+#include <type_traits>
+
 #include "va_dev.h"
 #include "va_tok.h"
 
@@ -15,9 +17,10 @@ struct Out {
     const void* res;
     void* y;
     int64_t ldr, ldy;
-    int32_t M, N, act, f32in, f32out, vec;
+    int32_t M, N, act, vec;
 };
 
+template <bool FIN, bool FOUT>
 __device__ __forceinline__ void finish4(const Out& o, int m, int n, f32x4 v) {
     if (m >= o.M || n >= o.N) return;
     float r[4];
@@ -27,11 +30,12 @@ __device__ __forceinline__ void finish4(const Out& o, int m, int n, f32x4 v) {
         float t = v[i];
         if (o.wscale) t *= o.wscale[c];
         if (o.bias) t += o.bias[c];
-        r[i] = o.f32out ? activate(t, o.act) : activate_bf16(t, o.act);
+        r[i] = t;
     }
+    activate_n<FOUT>(r, o.act);
     if (o.vec && n + 3 < o.N) {
         if (o.res) {
-            if (o.f32in) {
+            if (FIN) {
                 const f32x4 q = *(const f32x4*)((const float*)o.res + (int64_t)m * o.ldr + n);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) r[i] += q[i];
@@ -40,7 +44,7 @@ __device__ __forceinline__ void finish4(const Out& o, int m, int n, f32x4 v) {
                 r[0] += bf_lo(q[0]), r[1] += bf_hi(q[0]), r[2] += bf_lo(q[1]), r[3] += bf_hi(q[1]);
             }
         }
-        if (o.f32out)
+        if (FOUT)
             *(f32x4*)((float*)o.y + (int64_t)m * o.ldy + n) = (f32x4){r[0], r[1], r[2], r[3]};
         else
             *(u32x2*)((__bf16*)o.y + (int64_t)m * o.ldy + n) = (u32x2){pk_bf16(r[0], r[1]), pk_bf16(r[2], r[3])};
@@ -50,25 +54,29 @@ __device__ __forceinline__ void finish4(const Out& o, int m, int n, f32x4 v) {
     for (int i = 0; i < 4; ++i) {
         if (n + i >= o.N) return;
         if (o.res)
-            r[i] += o.f32in ? ((const float*)o.res)[(int64_t)m * o.ldr + n + i]
+            r[i] += FIN ? ((const float*)o.res)[(int64_t)m * o.ldr + n + i]
                             : (float)((const __bf16*)o.res)[(int64_t)m * o.ldr + n + i];
-        if (o.f32out)
+        if (FOUT)
             ((float*)o.y)[(int64_t)m * o.ldy + n + i] = r[i];
         else
             ((__bf16*)o.y)[(int64_t)m * o.ldy + n + i] = (__bf16)r[i];
     }
 }
 
-enum Form { BF16, W8, F32 };
+// types: bf16 or e4m3 weights with bf16 tensors, the same with a float result, all float
+enum Form { BF16, W8, BF16F, W8F, F32 };
+constexpr bool is8(Form f) { return f == W8 || f == W8F; }
+constexpr bool fin(Form f) { return f == F32; }
+constexpr bool fout(Form f) { return f >= BF16F; }
 
 // ------------------------------------------------------------------ any shape, stride and alignment
 // 64 channels x 64 tokens per workgroup, four waves of 32 x 32, K in steps of 32 through LDS; rows of 40 bf16 keep the
 // fragment reads off each other's banks.  F32: three planes, six term products per fragment pair.
 constexpr int GB = 64, GK = 32, GLD = GK + 8;
 
-template <Form FORM>
+template <Form FF>
 __global__ __launch_bounds__(256) void linear_any(va_tok_linear_args a, Out o, int ntn, int xvec) {
-    constexpr int T = FORM == F32 ? 3 : 1;
+    constexpr int T = FF == F32 ? 3 : 1;
     __shared__ __align__(16) __bf16 ws[T][GB][GLD], xs[T][GB][GLD];
     const int tile = xcd_tile(blockIdx.x, gridDim.x);
     const int n0 = tile % ntn * GB, m0 = tile / ntn * GB;
@@ -80,17 +88,17 @@ __global__ __launch_bounds__(256) void linear_any(va_tok_linear_args a, Out o, i
     for (int k0 = 0; k0 < a.Kpad; k0 += GK) {
         const int k = k0 + 8 * ch;
         bf16x8 wt[T], xt[T];
-        if constexpr (FORM == F32) {
+        if constexpr (FF == F32) {
 #pragma unroll
             for (int t = 0; t < 3; ++t)
                 wt[t] = *(const bf16x8*)((const __bf16*)a.w + ((int64_t)t * a.Npad + n0 + row) * a.Kpad + k);
-        } else if constexpr (FORM == W8) {
+        } else if constexpr (is8(FF)) {
             const int c = k / 8, pos = (c & ~7) | ((c & 3) << 1) | ((c >> 2) & 1);
             wt[0] = e4m3x8(*(const uint2*)((const uint8_t*)a.w + (int64_t)(n0 + row) * a.Kpad + 8 * pos));
         } else {
             wt[0] = *(const bf16x8*)((const __bf16*)a.w + (int64_t)(n0 + row) * a.Kpad + k);
         }
-        if constexpr (FORM == F32) {
+        if constexpr (FF == F32) {
             float x[8];
             const float* p = (const float*)a.x + (int64_t)m * a.ldx + k;
 #pragma unroll
@@ -122,7 +130,7 @@ __global__ __launch_bounds__(256) void linear_any(va_tok_linear_args a, Out o, i
             }
         constexpr int TA[6] = {0, 0, 1, 0, 1, 2}, TB[6] = {0, 1, 0, 2, 1, 0};
 #pragma unroll
-        for (int t = 0; t < (FORM == F32 ? 6 : 1); ++t)
+        for (int t = 0; t < (FF == F32 ? 6 : 1); ++t)
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -133,7 +141,7 @@ __global__ __launch_bounds__(256) void linear_any(va_tok_linear_args a, Out o, i
     for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-            finish4(o, m0 + 32 * wm + 16 * j + fr, n0 + 32 * wn + 16 * i + 4 * fq, acc[i][j]);
+            finish4<fin(FF), fout(FF)>(o, m0 + 32 * wm + 16 * j + fr, n0 + 32 * wn + 16 * i + 4 * fq, acc[i][j]);
 }
 
 // the six term products that are kept of (h + m + l)(h + m + l)
@@ -162,19 +170,14 @@ __device__ __forceinline__ void wait_vm() {
 }
 
 // eight consecutive channels of a token, through every type and alignment
+template <bool FIN, bool FOUT>
 __device__ __forceinline__ void finish8(const Out& o, int m, int n, float (&r)[8], const float (&scale)[8], const float (&bias)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) r[i] = __builtin_fmaf(r[i], scale[i], bias[i]);
-    if (o.f32out) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) r[i] = activate(r[i], o.act);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) r[i] = activate_bf16(r[i], o.act);
-    }
+    activate_n<FOUT>(r, o.act);
     if (o.vec == 2 && n + 7 < o.N) {
         if (o.res) {
-            if (o.f32in) {
+            if (FIN) {
                 const f32x4* q = (const f32x4*)((const float*)o.res + (int64_t)m * o.ldr + n);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) r[i] += q[i / 4][i % 4];
@@ -184,7 +187,7 @@ __device__ __forceinline__ void finish8(const Out& o, int m, int n, float (&r)[8
                 for (int e = 0; e < 4; ++e) r[2 * e] += bf_lo(q[e]), r[2 * e + 1] += bf_hi(q[e]);
             }
         }
-        if (o.f32out) {
+        if (FOUT) {
             f32x4* y = (f32x4*)((float*)o.y + (int64_t)m * o.ldy + n);
             y[0] = (f32x4){r[0], r[1], r[2], r[3]}, y[1] = (f32x4){r[4], r[5], r[6], r[7]};
         } else {
@@ -197,19 +200,58 @@ __device__ __forceinline__ void finish8(const Out& o, int m, int n, float (&r)[8
     for (int i = 0; i < 8; ++i) {
         if (n + i >= o.N) return;
         const int64_t at = (int64_t)m * o.ldy + n + i;
-        if (o.res) r[i] += o.f32in ? ((const float*)o.res)[(int64_t)m * o.ldr + n + i]
+        if (o.res) r[i] += FIN ? ((const float*)o.res)[(int64_t)m * o.ldr + n + i]
                                    : (float)((const __bf16*)o.res)[(int64_t)m * o.ldr + n + i];
-        if (o.f32out)
+        if (FOUT)
             ((float*)o.y)[at] = r[i];
         else
             ((__bf16*)o.y)[at] = (__bf16)r[i];
     }
 }
 
+// A wave's 32 WN channels x 32 WM tokens from n, m on: 32 tokens at a time through the wave's part of LDS, so that its
+// stores are whole runs of a token's channels -- 4 WN lanes hold a token's channels, eight each, whose bias and scale are
+// loaded once.  Register e of a block: channel 16 lh + e (the staged order of the weight rows).
+template <Form FF, int WN, int WM>
+__device__ __forceinline__ void store_tile(const Out& o, const f32x16 (&acc)[WN][WM], unsigned char* es, int m, int n, int lane) {
+    constexpr int EROW = (32 * WN + 4) * 4, LR = 4 * WN, RI = 64 / LR;  // lanes of a token, tokens an iteration
+    const int lc = lane & 31, lh = lane >> 5, er = lane / LR, ec = lane % LR * 8;
+    float scale[8], bias[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) scale[e] = 1.0f, bias[e] = 0.0f;
+    if (is8(FF)) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) scale[e] = o.wscale[min(n + ec + e, o.N - 1)];
+    }
+    if (o.bias) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) bias[e] = o.bias[min(n + ec + e, o.N - 1)];
+    }
+    // (waited for here: in the loops below the wait would be for the stores before it as well)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) asm volatile("" ::"v"(scale[e]), "v"(bias[e]));
+#pragma unroll
+    for (int j = 0; j < WM; ++j) {
+#pragma unroll
+        for (int i = 0; i < WN; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4)
+                *(f32x4*)(es + lc * EROW + (32 * i + 16 * lh + e) * 4) =
+                    (f32x4){acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]};
+#pragma unroll 2
+        for (int it = 0; it < 32 / RI; ++it) {
+            const int row = it * RI + er, mr = m + 32 * j + row;
+            const f32x4 u = *(const f32x4*)(es + row * EROW + ec * 4), v = *(const f32x4*)(es + row * EROW + ec * 4 + 16);
+            float r[8] = {u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
+            if (mr < o.M && n + ec < o.N) finish8<fin(FF), fout(FF)>(o, mr, n + ec, r, scale, bias);
+        }
+    }
+}
+
 template <Form F, int WN, int WM>
 struct TileCfg {
     static constexpr int BN = 64 * WN, BM = 64 * WM, T = F == F32 ? 3 : 1;
-    static constexpr int WROW = F == W8 ? 32 : 64, XROW = F == F32 ? 128 : 64;   // bytes of a staged row
+    static constexpr int WROW = is8(F) ? 32 : 64, XROW = F == F32 ? 128 : 64;   // bytes of a staged row
     static constexpr int WPL = BN * WROW, WB = T * WPL, XB = BM * XROW, STAGE = WB + XB;
     static constexpr int ND = STAGE / 4096;                                       // DMAs of a wave and step
     static constexpr int NS = 3 * STAGE <= 80 * 1024 ? 3 : 2;
@@ -235,24 +277,24 @@ __global__ __launch_bounds__(256, 2) void linear_tile(va_tok_linear_args a, Out 
         const int at = (wid * ND + j) * 1024 + lane * 16;
         if (at < C::WB) {
             const int in = at % C::WPL, r = in / C::WROW, q = in % C::WROW / 16;
-            const int p = F == W8 ? q ^ ((r >> 2) & 1) : q ^ ((r >> 1) & 3);
+            const int p = is8(F) ? q ^ ((r >> 2) & 1) : q ^ ((r >> 1) & 3);
             const int ch = (r & ~31) + 16 * ((r >> 2) & 1) + 4 * ((r & 31) >> 3) + (r & 3);  // the channel of this row
-            off[j] = n0 + ch < a.Npad ? ch * a.Kpad * (F == W8 ? 1 : 2) + 16 * p : LIN_OOB;
+            off[j] = n0 + ch < a.Npad ? ch * a.Kpad * (is8(F) ? 1 : 2) + 16 * p : LIN_OOB;
             kc[j] = -1;
         } else {
             const int in = at - C::WB, r = in / C::XROW, q = in % C::XROW / 16;
             const int p = F == F32 ? q ^ (r & 7) : q ^ ((r >> 1) & 3);
             // e4m3: a step's four bytes-of-8 are chunks c, c + 4, c + 1, c + 5 of the 64-block (c = 0 or 2)
-            kc[j] = F == W8 ? (p & 1) * 32 + (p >> 1) * 8 : p * (16 / XE);
+            kc[j] = is8(F) ? (p & 1) * 32 + (p >> 1) * 8 : p * (16 / XE);
             off[j] = m0 + r < a.M ? (int)(r * a.ldx + kc[j]) * XE : LIN_OOB;
         }
     }
-    const int nk = F == W8 ? 2 * ((a.K + 63) / 64) : (a.K + 31) / 32;
+    const int nk = is8(F) ? 2 * ((a.K + 63) / 64) : (a.K + 31) / 32;
     const unsigned char* xb = (const unsigned char*)a.x + (int64_t)m0 * a.ldx * XE;
-    const unsigned char* wb = (const unsigned char*)a.w + (int64_t)n0 * a.Kpad * (F == W8 ? 1 : 2);
+    const unsigned char* wb = (const unsigned char*)a.w + (int64_t)n0 * a.Kpad * (is8(F) ? 1 : 2);
     const int64_t plane = (int64_t)a.Npad * a.Kpad * 2;
     auto issue = [&](int t, int stage) {
-        const int k0 = F == W8 ? (t >> 1) * 64 + (t & 1) * 16 : t * 32;  // x's first k
+        const int k0 = is8(F) ? (t >> 1) * 64 + (t & 1) * 16 : t * 32;  // x's first k
         unsigned char* to = sm + stage * C::STAGE;
 #pragma unroll
         for (int j = 0; j < ND; ++j) {
@@ -281,7 +323,7 @@ __global__ __launch_bounds__(256, 2) void linear_tile(va_tok_linear_args a, Out 
 #pragma unroll
         for (int i = 0; i < WN; ++i) {
             const int r = 32 * (wn * WN + i) + lc;
-            if constexpr (F == W8) {
+            if constexpr (is8(F)) {
                 f.w[i][0] = e4m3x8(*(const uint2*)(ws + r * 32 + 16 * (ks ^ ((r >> 2) & 1)) + 8 * lh));
             } else {
 #pragma unroll
@@ -340,35 +382,115 @@ __global__ __launch_bounds__(256, 2) void linear_tile(va_tok_linear_args a, Out 
         mma(f1);
         stage = next;
     }
-    // 32 tokens at a time through the wave's part of LDS, so that its stores are whole runs of a token's channels: 4 WN
-    // lanes hold a token's 32 WN channels, eight each (their bias and scale are loaded once)
-    __syncthreads();
-    unsigned char* es = sm + wid * 32 * C::EROW;
-    constexpr int LR = 4 * WN, RI = 64 / LR;  // lanes of a token, tokens an iteration
-    const int er = lane / LR, ec = lane % LR * 8, n = n0 + 32 * WN * wn + ec;
-    float scale[8], bias[8];
+    store_tile<F, WN, WM>(o, acc, sm + wid * 32 * C::EROW, m0 + 32 * wm * WM, n0 + 32 * wn * WN, lane);
+}
+
+// ------------------------------------------------------------------ many large tiles
+// 256 channels x 256 tokens per workgroup, one a CU: four waves of 128 x 128 (256 accumulator registers) need the fewest
+// fragment reads per MFMA -- 128 KB of LDS reads and 64 KB of DMA writes per 2048 MFMA cycles, against 128 bytes a cycle;
+// two waves a SIMD of 128 x 64 would need all of it.  K in steps of 64, so that a DMA's rows are whole cache lines (rows of
+// 64 bytes fetched each line twice: 682 against ... TFLOP/s at 8192^3), two stages.  A step is four slices of 16; the
+// fragments of a slice are read beside the MFMAs of the slice before.  One barrier a step, before its last slice, whose
+// fragments are in registers by then: it frees this stage for step t + 2 and publishes step t + 1.
+constexpr int WK = 64, WSTAGE = 2 * 256 * 128, WLDS = 2 * WSTAGE;
+
+template <Form F>
+__global__ __launch_bounds__(256, 1) void linear_wide(va_tok_linear_args a, Out o, int ntn, int ntm) {
+    static_assert(F == BF16 || F == BF16F, "");
+    extern __shared__ __align__(16) unsigned char sm[];  // [2][weights | tokens], rows of 128 bytes
+    // tiles in blocks of 4 (tokens) x all channels, tokens fastest: the 32 tiles that an XCD works on at a time share
+    // their operands' rows 4 to 8 times
+    const int tile = xcd_tile(blockIdx.x, gridDim.x);
+    const int grp = tile / (4 * ntn), gm = min(4, ntm - 4 * grp), in = tile - 4 * grp * ntn;
+    const int m0 = (4 * grp + in % gm) * 256, n0 = in / gm * 256;
+    const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lc = lane & 31, lh = lane >> 5;
+    const int wn = wid & 1, wm = wid >> 1;
+    const int nk = (a.K + WK - 1) / WK;
+    // DMA j of this wave: rows 64 wid + 8 j .. + 7 of an operand's image, lane l row l / 8, place l % 8 (piece place ^ row).
+    // The weight rows hold channels in the order that leaves a lane 16 consecutive ones in its registers.
+    const int l8 = lane >> 3, piece = (lane & 7) ^ l8;
+    const int wch = 64 * wid + 16 * (l8 >> 2) + (l8 & 3);  // + 32 (j / 4) + 4 (j % 4)
+    const int woff = wch * a.Kpad * 2 + 16 * piece, xoff = (int)((64 * wid + l8) * a.ldx) * 2 + 16 * piece;
+    const unsigned char* wb = (const unsigned char*)a.w + (int64_t)n0 * a.Kpad * 2;
+    const unsigned char* xb = (const unsigned char*)a.x + (int64_t)m0 * a.ldx * 2;
+    const int wmore = a.Npad - n0 - wch, xmore = a.M - m0 - 64 * wid - l8;  // rows from this lane's first on
+    auto issue_w = [&](int t, int j) {
+        const int up = 32 * (j / 4) + 4 * (j % 4);
+        dma16(wb, sm + (t & 1) * WSTAGE + (8 * wid + j) * 1024, up < wmore && t < nk ? woff : LIN_OOB, up * a.Kpad * 2 + t * 128);
+    };
+    auto issue_x = [&](int t, int j) {
+        const bool in = 8 * j < xmore && t * WK + 8 * piece < a.K;  // (t < nk with it)
+        dma16(xb, sm + (t & 1) * WSTAGE + 32768 + (8 * wid + j) * 1024, in ? xoff : LIN_OOB, (int)(8 * j * a.ldx) * 2 + t * 128);
+    };
+    f32x16 acc[4][4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const int c = min(n + e, a.N - 1);
-        scale[e] = o.wscale ? o.wscale[c] : 1.0f;
-        bias[e] = o.bias ? o.bias[c] : 0.0f;
-    }
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int j = 0; j < WM; ++j) {
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int i = 0; i < WN; ++i)
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+    struct Frag {
+        bf16x8 w[4], x[4];
+    };
+    const int fw = (128 * wn + lc) * 128, fx = 32768 + (128 * wm + lc) * 128;  // this lane's rows (32 i more)
+    auto read = [&](Frag& f, int t, int ks) {
+        const unsigned char* st = sm + (t & 1) * WSTAGE + 16 * ((2 * ks + lh) ^ (lc & 7));
 #pragma unroll
-            for (int e = 0; e < 16; e += 4)
-                *(f32x4*)(es + lc * C::EROW + (32 * i + 16 * lh + e) * 4) =
-                    (f32x4){acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]};
-#pragma unroll 1
-        for (int it = 0; it < 32 / RI; ++it) {
-            const int row = it * RI + er, m = m0 + 32 * (wm * WM + j) + row;
-            const f32x4 u = *(const f32x4*)(es + row * C::EROW + ec * 4), v = *(const f32x4*)(es + row * C::EROW + ec * 4 + 16);
-            float r[8] = {u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
-            if (m < o.M && n < o.N) finish8(o, m, n, r, scale, bias);
+        for (int i = 0; i < 4; ++i) {
+            f.w[i] = *(const bf16x8*)(st + fw + i * 4096);
+            f.x[i] = *(const bf16x8*)(st + fx + i * 4096);
         }
+    };
+    auto mma = [&](const Frag& f) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.w[i], f.x[j], acc[i][j], 0, 0, 0);
+    };
+    // sixteen MFMAs with eight fragment reads and DMAS DMAs between them
+    auto spread = [&](auto dmas) {
+        constexpr int DMAS = decltype(dmas)::value;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            if (DMAS == 8 || (DMAS == 4 && i % 2)) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // The DMAs of a stage that becomes free at a step's barrier go out over three slices: the tokens' (from far) first.
+    // Past the last step they and the reads run on, on offsets out of range and stale stages, so that the loop is one block.
+    for (int j = 0; j < 8; ++j) issue_x(0, j), issue_w(0, j);
+    for (int j = 0; j < 8; ++j) issue_x(1, j);
+    wait_vm<8>();
+    asm volatile("s_barrier" ::: "memory");
+    Frag f0, f1;
+    read(f0, 0, 0);
+    for (int t = 0; t < nk; ++t) {
+        read(f1, t, 1);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) issue_w(t + 1, j);
+        mma(f0);
+        spread(std::integral_constant<int, 4>());
+        read(f0, t, 2);
+#pragma unroll
+        for (int j = 4; j < 8; ++j) issue_w(t + 1, j);
+        mma(f1);
+        spread(std::integral_constant<int, 4>());
+        read(f1, t, 3);
+        mma(f0);
+        spread(std::integral_constant<int, 0>());
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        read(f0, t + 1, 0);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) issue_x(t + 2, j);
+        mma(f1);
+        spread(std::integral_constant<int, 8>());
     }
+    wait_vm<0>();
+    __syncthreads();
+    store_tile<F, 4, 4>(o, acc, sm + wid * 32 * 528, m0 + 128 * wm, n0 + 128 * wn, lane);
 }
 
 // ------------------------------------------------------------------ few tiles: K over the waves of a workgroup
@@ -389,11 +511,11 @@ __global__ __launch_bounds__(512) void linear_few(va_tok_linear_args a, Out o, i
 #pragma unroll
     for (int j = 0; j < MB; ++j) acc[j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
     struct Raw {
-        u32x4 w[F == W8 ? 1 : 2 * T], x[2][MB][F == F32 ? 2 : 1];
+        u32x4 w[is8(F) ? 1 : 2 * T], x[2][MB][F == F32 ? 2 : 1];
     };
     auto load = [&](Raw& r, int kb) {
         const int k = kb * 64 + 8 * fq;
-        if constexpr (F == W8) {  // one 16-byte piece: chunks fq and fq + 4
+        if constexpr (is8(F)) {  // one 16-byte piece: chunks fq and fq + 4
             r.w[0] = *(const u32x4*)((const uint8_t*)a.w + (int64_t)(n0 + fr) * a.Kpad + kb * 64 + 16 * fq);
         } else {
 #pragma unroll
@@ -422,7 +544,7 @@ __global__ __launch_bounds__(512) void linear_few(va_tok_linear_args a, Out o, i
             bf16x8 w[T];
 #pragma unroll
             for (int t = 0; t < T; ++t)
-                w[t] = F == W8 ? e4m3x8(make_uint2(r.w[0][2 * h], r.w[0][2 * h + 1])) : (bf16x8)r.w[h * T + t];
+                w[t] = is8(F) ? e4m3x8(make_uint2(r.w[0][2 * h], r.w[0][2 * h + 1])) : (bf16x8)r.w[h * T + t];
 #pragma unroll
             for (int j = 0; j < MB; ++j) {
                 bf16x8 x[T];
@@ -465,7 +587,7 @@ __global__ __launch_bounds__(512) void linear_few(va_tok_linear_args a, Out o, i
         f32x4 v = part[0][j][lane];
 #pragma unroll
         for (int w = 1; w < NW; ++w) v += part[w][j][lane];
-        finish4(o, m0 + 16 * j + fr, n0 + 4 * fq, v);
+        finish4<fin(F), fout(F)>(o, m0 + 16 * j + fr, n0 + 4 * fq, v);
     }
 }
 
@@ -499,6 +621,19 @@ hipError_t go_tile(const va_tok_linear_args& a, const Out& o, hipStream_t st) {
     return hipGetLastError();
 }
 
+template <Form F>
+hipError_t go_wide(const va_tok_linear_args& a, const Out& o, hipStream_t st) {
+    static DevFlag attr;
+    if (!attr()) {
+        const hipError_t e = hipFuncSetAttribute((const void*)linear_wide<F>, hipFuncAttributeMaxDynamicSharedMemorySize, WLDS);
+        if (e != hipSuccess) return e;
+        attr() = true;
+    }
+    const int ntn = (a.N + 255) / 256, ntm = (a.M + 255) / 256;
+    hipLaunchKernelGGL(linear_wide<F>, dim3((unsigned)(ntn * ntm)), dim3(256), WLDS, st, a, o, ntn, ntm);
+    return hipGetLastError();
+}
+
 template <Form F, int MB>
 hipError_t go_few(const va_tok_linear_args& a, const Out& o, hipStream_t st) {
     const int ntn = (a.N + 15) / 16, ntm = (a.M + 16 * MB - 1) / (16 * MB);
@@ -525,8 +660,10 @@ hipError_t go(const va_tok_linear_args& a, const Out& o, hipStream_t st) {
     if constexpr (F == F32) {
         return t64 < 1024 ? go_tile<F32, 1, 1>(a, o, st) : go_tile<F32, 2, 1>(a, o, st);
     } else {
-        const int64_t big = (int64_t)((a.N + 255) / 256) * ((a.M + 127) / 128);
-        if (big >= 384) return go_tile<F, 4, 2>(a, o, st);
+        if constexpr (!is8(F)) {
+            if ((int64_t)((a.N + 255) / 256) * ((a.M + 255) / 256) >= 192) return go_wide<F>(a, o, st);
+        }
+        if ((int64_t)((a.N + 255) / 256) * ((a.M + 127) / 128) >= 384) return go_tile<F, 4, 2>(a, o, st);
         return go_tile<F, 2, 1>(a, o, st);
     }
 }
@@ -538,15 +675,18 @@ extern "C" int va_tok_linear(void* stream, const va_tok_linear_args* ap) {
     if (a.M == 0) return VA_OK;
     if ((int64_t)((a.N + 15) / 16) * ((a.M + 15) / 16) > INT32_MAX) return VA_ERR_RANGE;
     const bool f32 = a.dtype == VA_DTYPE_F32;
-    Out o = {a.wscale, a.bias, a.res, a.y, a.ldr, a.ldy, a.M, a.N, a.act, f32, f32 || a.out_f32, 0};
+    const bool f32out = f32 || a.out_f32;
+    Out o = {a.wscale, a.bias, a.res, a.y, a.ldr, a.ldy, a.M, a.N, a.act, 0};
     // stores of 4 channels (1), of 8 (2)
     const auto rows = [&](int n) {
-        const int eo = o.f32out ? 4 : 2, ei = f32 ? 4 : 2, bo = n * eo < 16 ? n * eo : 16, bi = n * ei < 16 ? n * ei : 16;
+        const int eo = f32out ? 4 : 2, ei = f32 ? 4 : 2, bo = n * eo < 16 ? n * eo : 16, bi = n * ei < 16 ? n * ei : 16;
         return a.ldy * eo % bo == 0 && !((uintptr_t)a.y & (uintptr_t)(bo - 1)) &&
                (!a.res || (a.ldr * ei % bi == 0 && !((uintptr_t)a.res & (uintptr_t)(bi - 1))));
     };
     o.vec = rows(8) ? 2 : rows(4) ? 1 : 0;
     hipStream_t st = (hipStream_t)stream;
-    const hipError_t e = f32 ? go<F32>(a, o, st) : a.w8 ? go<W8>(a, o, st) : go<BF16>(a, o, st);
+    const hipError_t e = f32         ? go<F32>(a, o, st)
+                         : a.out_f32 ? (a.w8 ? go<W8F>(a, o, st) : go<BF16F>(a, o, st))
+                                     : (a.w8 ? go<W8>(a, o, st) : go<BF16>(a, o, st));
     return e == hipSuccess ? VA_OK : VA_ERR_HIP;
 }
