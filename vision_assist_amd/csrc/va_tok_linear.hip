@@ -64,6 +64,12 @@ __device__ __forceinline__ void finish4(const Out& o, int m, int n, f32x4 v) {
 }
 
 // types: bf16 or e4m3 weights with bf16 tensors, the same with a float result, all float
+// Packed weights (va355.h): blocks of 32 channels x 32 of K, [Kpad / 32][Npad / 32][32 rows], a row 64 bytes of bf16 (32 of
+// e4m3) -- the image that the kernels stage, so that staging is a linear copy.  Row r of a block is channel 16 (r / 4 % 2) +
+// 4 (r / 8) + r % 4 of it: an MFMA then leaves a lane 16 consecutive channels in its registers.  Its 16-byte pieces lie in
+// place p ^ (r / 2 % 4) (e4m3: p ^ (r / 4 % 2)): eight rows' reads of one piece spread over the LDS banks.
+__host__ __device__ constexpr int row_of(int ch) { return 8 * ((ch & 15) >> 2) + 4 * (ch >> 4) + (ch & 3); }
+
 enum Form { BF16, W8, BF16F, W8F, F32 };
 constexpr bool is8(Form f) { return f == W8 || f == W8F; }
 constexpr bool fin(Form f) { return f == F32; }
@@ -82,21 +88,20 @@ __global__ __launch_bounds__(256) void linear_any(va_tok_linear_args a, Out o, i
     const int n0 = tile % ntn * GB, m0 = tile / ntn * GB;
     const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, fr = lane & 15, fq = lane >> 4;
     const int wn = wid & 1, wm = wid >> 1;
-    const int row = tid >> 2, ch = tid & 3;  // this thread's staged row and 8-value chunk
+    const int row = tid >> 2, kq = tid & 3;  // this thread's staged row and 8-value chunk
     const int m = m0 + row;
     f32x4 acc[2][2] = {};
     for (int k0 = 0; k0 < a.Kpad; k0 += GK) {
-        const int k = k0 + 8 * ch;
+        const int k = k0 + 8 * kq;
         bf16x8 wt[T], xt[T];
-        if constexpr (FF == F32) {
-#pragma unroll
-            for (int t = 0; t < 3; ++t)
-                wt[t] = *(const bf16x8*)((const __bf16*)a.w + ((int64_t)t * a.Npad + n0 + row) * a.Kpad + k);
-        } else if constexpr (is8(FF)) {
-            const int c = k / 8, pos = (c & ~7) | ((c & 3) << 1) | ((c >> 2) & 1);
-            wt[0] = e4m3x8(*(const uint2*)((const uint8_t*)a.w + (int64_t)(n0 + row) * a.Kpad + 8 * pos));
+        const int ch = n0 + row, r = row_of(ch & 31);
+        const int64_t block = (int64_t)(k / 32) * (a.Npad / 32) + ch / 32;
+        if constexpr (is8(FF)) {
+            wt[0] = e4m3x8(*(const uint2*)((const uint8_t*)a.w + block * 1024 + r * 32 + 16 * ((k % 32 / 16) ^ ((r >> 2) & 1)) + k % 16));
         } else {
-            wt[0] = *(const bf16x8*)((const __bf16*)a.w + (int64_t)(n0 + row) * a.Kpad + k);
+#pragma unroll
+            for (int t = 0; t < T; ++t)
+                wt[t] = *(const bf16x8*)((const __bf16*)a.w + (int64_t)t * a.Npad * a.Kpad + block * 1024 + r * 32 + 8 * ((k % 32 / 8) ^ ((r >> 1) & 3)));
         }
         if constexpr (FF == F32) {
             float x[8];
@@ -116,8 +121,8 @@ __global__ __launch_bounds__(256) void linear_any(va_tok_linear_args a, Out o, i
         __syncthreads();
 #pragma unroll
         for (int t = 0; t < T; ++t) {
-            *(bf16x8*)&ws[t][row][8 * ch] = wt[t];
-            *(bf16x8*)&xs[t][row][8 * ch] = xt[t];
+            *(bf16x8*)&ws[t][row][8 * kq] = wt[t];
+            *(bf16x8*)&xs[t][row][8 * kq] = xt[t];
         }
         __syncthreads();
         bf16x8 fw[T][2], fx[T][2];
@@ -147,16 +152,16 @@ __global__ __launch_bounds__(256) void linear_any(va_tok_linear_args a, Out o, i
 // the six term products that are kept of (h + m + l)(h + m + l)
 constexpr int NTERM = 6, TERM_W[6] = {0, 0, 1, 0, 1, 2}, TERM_X[6] = {0, 1, 0, 2, 1, 0};
 
-// ------------------------------------------------------------------ many tiles: LDS-DMA ring, counted waits
-// 64 WN channels x 64 WM tokens per workgroup, four waves of 32 WN x 32 WM on v_mfma_f32_32x32x16_bf16, K in steps of 32
-// through a ring of NS stages.  A step is two slices of 16; the fragments of a slice are read while the MFMAs of the slice
-// before run.  One barrier a step, after its first slice: by then every wave has read the whole step (its second slice's
-// fragments have arrived), so its stage is free and step t + NS is sent into it; and the wait before the barrier has
-// retired step t + 1's DMAs, whose fragments are read next, while those of t + 2 .. t + NS - 1 stay in flight.
-// Two workgroups share a CU: the epilogue of one (activations: VALU) runs beside the MFMAs of the other.
-//   rows of a stage: 64 bytes (bf16: 32 values), piece p of row r in place p ^ ((r >> 1) & 3); F32's x 128 bytes, place
-//   p ^ (r & 7); e4m3 weights 32 bytes, piece p in place p ^ ((r >> 2) & 1): eight lanes' 16 bytes cover the banks
-//   weight rows are staged in an order that leaves a lane 16 consecutive channels of its token in its registers
+// ------------------------------------------------------------------ many tiles: LDS-DMA rings, counted waits
+// 64 WN channels x 64 WM tokens per workgroup, four waves of 32 WN x 32 WM on v_mfma_f32_32x32x16_bf16, K in steps of 32.
+// Weights go through a ring of NSW stages of a step; tokens in stages of whole 128-byte lines, two steps of bf16 or one of
+// float (rows of 64 bytes would fetch each line twice).  A step is two slices of 16; the fragments of a slice are read
+// while the MFMAs of the slice before run.  One barrier a step, after its first slice: by then every wave has read the
+// whole step, so its stage is free and the weights of step t + NSW (after a token stage's last step: the tokens two stages
+// on) are sent into it; and the wait before the barrier has retired what step t + 1 needs -- all but what the barrier
+// before sent -- whose fragments are read next.
+// Two workgroups of 256 x 128 share a CU: the epilogue of one (activations: VALU, stores) runs beside the MFMAs of the
+// other.
 constexpr int LIN_OOB = 0x7ffffff0;      // an offset that a descriptor of that many bytes answers with zeros
 constexpr int LIN_ROW = 1 << 21;         // longest rows in values: the offsets of 256 of them stay within 31 bits
 
@@ -251,59 +256,48 @@ __device__ __forceinline__ void store_tile(const Out& o, const f32x16 (&acc)[WN]
 template <Form F, int WN, int WM>
 struct TileCfg {
     static constexpr int BN = 64 * WN, BM = 64 * WM, T = F == F32 ? 3 : 1;
-    static constexpr int WROW = is8(F) ? 32 : 64, XROW = F == F32 ? 128 : 64;   // bytes of a staged row
-    static constexpr int WPL = BN * WROW, WB = T * WPL, XB = BM * XROW, STAGE = WB + XB;
-    static constexpr int ND = STAGE / 4096;                                       // DMAs of a wave and step
-    static constexpr int NS = 3 * STAGE <= 80 * 1024 ? 3 : 2;
-    // the epilogue's blocks: a wave's 32 tokens x 32 WN channels of float, rows padded by 16 bytes
-    static constexpr int EROW = (32 * WN + 4) * 4, EPI = 4 * 32 * EROW, LDS = NS * STAGE > EPI ? NS * STAGE : EPI;
-    static_assert(STAGE % 4096 == 0 && LDS <= 80 * 1024, "two workgroups a CU");
+    static constexpr int WROW = is8(F) ? 32 : 64, XP = F == F32 ? 1 : 2;        // bytes of a weight row; steps of a token stage
+    static constexpr int WPL = BN * WROW, WB = T * WPL, XB = BM * 128;          // bytes of a plane, of the stages
+    static constexpr int NSW = 3 * WB + (F == F32 ? 3 : 2) * XB <= 80 * 1024 ? 3 : 2, NSX = F == F32 ? NSW : 2;
+    static constexpr int DW = WB / 4096, DX = XB / 4096;                        // DMAs of a wave
+    static constexpr int EROW = (32 * WN + 4) * 4, EPI = 4 * 32 * EROW;         // the epilogue's blocks (store_tile)
+    static constexpr int RING = NSW * WB + NSX * XB, LDS = RING > EPI ? RING : EPI;
+    static_assert(WB % 4096 == 0 && XB % 4096 == 0 && WPL % 1024 == 0 && LDS <= 80 * 1024, "two workgroups a CU");
 };
 
 template <Form F, int WN, int WM>
 __global__ __launch_bounds__(256, 2) void linear_tile(va_tok_linear_args a, Out o, int ntn) {
     using C = TileCfg<F, WN, WM>;
-    constexpr int NS = C::NS, ND = C::ND, T = C::T;
-    extern __shared__ __align__(16) unsigned char sm[];
+    constexpr int T = C::T, XE = F == F32 ? 4 : 2;
+    extern __shared__ __align__(16) unsigned char sm[];  // [NSW] weights, [NSX] tokens
     const int tile = xcd_tile(blockIdx.x, gridDim.x);
     const int n0 = tile % ntn * C::BN, m0 = tile / ntn * C::BM;
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lc = lane & 31, lh = lane >> 5;
     const int wn = wid & 1, wm = wid >> 1;
-    constexpr int XE = F == F32 ? 4 : 2;
-    // this lane's DMAs: instruction d = wid * ND + j fills bytes [1024 d, 1024 d + 1024) of a stage
-    int off[ND], kc[ND];  // byte offset of the piece from its operand's tile; for x its first k of a step
+    const int nk = 2 * ((a.K + 63) / 64);
+    // weights: DMA d of a stage's plane copies its bytes [1024 d, 1024 d + 1024); blocks from channel Npad on are not there
+    const unsigned char* wb = (const unsigned char*)a.w + (int64_t)(n0 / 32) * 32 * C::WROW;
+    const int64_t wstep = (int64_t)a.Npad * C::WROW, plane = wstep * (a.Kpad / 32);
+    const int wend = (a.Npad - n0) * C::WROW;
+    auto issue_w = [&](int t) {
+        unsigned char* to = sm + t % C::NSW * C::WB;
+        const unsigned char* from = wb + min(t, nk - 1) * wstep;
 #pragma unroll
-    for (int j = 0; j < ND; ++j) {
-        const int at = (wid * ND + j) * 1024 + lane * 16;
-        if (at < C::WB) {
-            const int in = at % C::WPL, r = in / C::WROW, q = in % C::WROW / 16;
-            const int p = is8(F) ? q ^ ((r >> 2) & 1) : q ^ ((r >> 1) & 3);
-            const int ch = (r & ~31) + 16 * ((r >> 2) & 1) + 4 * ((r & 31) >> 3) + (r & 3);  // the channel of this row
-            off[j] = n0 + ch < a.Npad ? ch * a.Kpad * (is8(F) ? 1 : 2) + 16 * p : LIN_OOB;
-            kc[j] = -1;
-        } else {
-            const int in = at - C::WB, r = in / C::XROW, q = in % C::XROW / 16;
-            const int p = F == F32 ? q ^ (r & 7) : q ^ ((r >> 1) & 3);
-            // e4m3: a step's four bytes-of-8 are chunks c, c + 4, c + 1, c + 5 of the 64-block (c = 0 or 2)
-            kc[j] = is8(F) ? (p & 1) * 32 + (p >> 1) * 8 : p * (16 / XE);
-            off[j] = m0 + r < a.M ? (int)(r * a.ldx + kc[j]) * XE : LIN_OOB;
+        for (int j = 0; j < C::DW; ++j) {
+            const int d = (wid * C::DW + j) * 1024, in = d % C::WPL;  // uniform
+            dma16(from + (T > 1 ? d / C::WPL * plane : 0), to + d, t < nk && in < wend ? lane * 16 : LIN_OOB, in);
         }
-    }
-    const int nk = is8(F) ? 2 * ((a.K + 63) / 64) : (a.K + 31) / 32;
+    };
+    // tokens: DMA j takes rows 8 (wid DX + j) .. + 7, lane l row l / 8, place l % 8 (piece place ^ row)
+    const int l8 = lane >> 3, piece = (lane & 7) ^ l8;
     const unsigned char* xb = (const unsigned char*)a.x + (int64_t)m0 * a.ldx * XE;
-    const unsigned char* wb = (const unsigned char*)a.w + (int64_t)n0 * a.Kpad * (is8(F) ? 1 : 2);
-    const int64_t plane = (int64_t)a.Npad * a.Kpad * 2;
-    auto issue = [&](int t, int stage) {
-        const int k0 = is8(F) ? (t >> 1) * 64 + (t & 1) * 16 : t * 32;  // x's first k
-        unsigned char* to = sm + stage * C::STAGE;
+    const int xrow = 8 * wid * C::DX + l8, xoff = (int)(xrow * a.ldx) * XE + 16 * piece, xmore = a.M - m0 - xrow;
+    auto issue_x = [&](int st) {
+        unsigned char* to = sm + C::NSW * C::WB + st % C::NSX * C::XB + wid * C::DX * 1024;
+        const bool in = st * (128 / XE) + piece * (16 / XE) < a.K;
 #pragma unroll
-        for (int j = 0; j < ND; ++j) {
-            const int d = (wid * ND + j) * 1024;  // uniform
-            const bool isw = d < C::WB;
-            const unsigned char* base = isw ? wb + (T > 1 ? d / C::WPL * plane : 0) : xb;
-            const int v = kc[j] >= 0 && k0 + kc[j] >= a.K ? LIN_OOB : off[j];
-            dma16(base, to + d, v, isw ? t * C::WROW : k0 * XE);
-        }
+        for (int j = 0; j < C::DX; ++j)
+            dma16(xb, to + j * 1024, in && 8 * j < xmore ? xoff : LIN_OOB, (int)(8 * j * a.ldx) * XE + st * 128);
     };
     f32x16 acc[WN][WM];
 #pragma unroll
@@ -316,31 +310,29 @@ __global__ __launch_bounds__(256, 2) void linear_tile(va_tok_linear_args a, Out 
     struct Frag {
         bf16x8 w[WN][T], x[WM][T];
     };
-    auto read = [&](Frag& f, int stage, int ks) {
-        const unsigned char* ws = sm + stage * C::STAGE;
-        const unsigned char* xs = ws + C::WB;
-        const int p = 2 * ks + lh;  // this lane's piece of 8 values
+    auto read = [&](Frag& f, int t, int ks) {
+        const unsigned char* ws = sm + t % C::NSW * C::WB;
+        const unsigned char* xs = sm + C::NSW * C::WB + t / C::XP % C::NSX * C::XB;
 #pragma unroll
         for (int i = 0; i < WN; ++i) {
-            const int r = 32 * (wn * WN + i) + lc;
+            const unsigned char* wr = ws + (32 * (wn * WN + i) + lc) * C::WROW;
             if constexpr (is8(F)) {
-                f.w[i][0] = e4m3x8(*(const uint2*)(ws + r * 32 + 16 * (ks ^ ((r >> 2) & 1)) + 8 * lh));
+                f.w[i][0] = e4m3x8(*(const uint2*)(wr + 16 * (ks ^ ((lc >> 2) & 1)) + 8 * lh));
             } else {
 #pragma unroll
-                for (int t = 0; t < T; ++t)
-                    f.w[i][t] = *(const bf16x8*)(ws + t * C::WPL + r * 64 + 16 * (p ^ ((r >> 1) & 3)));
+                for (int p = 0; p < T; ++p) f.w[i][p] = *(const bf16x8*)(wr + p * C::WPL + 16 * ((2 * ks + lh) ^ ((lc >> 1) & 3)));
             }
         }
 #pragma unroll
         for (int j = 0; j < WM; ++j) {
-            const int r = 32 * (wm * WM + j) + lc;
+            const unsigned char* xr = xs + (32 * (wm * WM + j) + lc) * 128;
             if constexpr (F == F32) {
-                const f32x4 u = *(const f32x4*)(xs + r * 128 + 16 * ((2 * p) ^ (r & 7)));
-                const f32x4 v = *(const f32x4*)(xs + r * 128 + 16 * ((2 * p + 1) ^ (r & 7)));
+                const int p = 2 * (2 * ks + lh);
+                const f32x4 u = *(const f32x4*)(xr + 16 * (p ^ (lc & 7))), v = *(const f32x4*)(xr + 16 * ((p + 1) ^ (lc & 7)));
                 const float e[8] = {u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
                 split3(e, f.x[j]);
             } else {
-                f.x[j][0] = *(const bf16x8*)(xs + r * 64 + 16 * (p ^ ((r >> 1) & 3)));
+                f.x[j][0] = *(const bf16x8*)(xr + 16 * ((4 * (t & 1) + 2 * ks + lh) ^ (lc & 7)));
             }
         }
     };
@@ -354,34 +346,41 @@ __global__ __launch_bounds__(256, 2) void linear_tile(va_tok_linear_args a, Out 
                     acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.w[i][T > 1 ? TERM_W[t] : 0], f.x[j][T > 1 ? TERM_X[t] : 0],
                                                                         acc[i][j], 0, 0, 0);
     };
-#pragma unroll
-    for (int t = 0; t < NS; ++t)
-        if (t < nk) issue(t, t);
-    if (nk >= NS)
-        wait_vm<(NS - 1) * ND>();
-    else
-        wait_vm<0>();
+    // in the order in which the steps need them; past the last step they run on, on offsets out of range
+    issue_x(0);
+    issue_w(0);
+    issue_w(1);
+    issue_x(1);
+    if constexpr (C::NSW == 3) {
+        issue_w(2);
+        if constexpr (C::XP == 1) issue_x(2);
+    }
+    wait_vm<C::NSW == 3 ? 2 * C::DW + C::DX * (C::XP == 1 ? 2 : 1) : C::DW + C::DX>();
     asm volatile("s_barrier" ::: "memory");
     Frag f0, f1;
     read(f0, 0, 0);
-    int stage = 0;
-    for (int t = 0; t < nk; ++t) {
-        const int next = stage + 1 == NS ? 0 : stage + 1;
-        read(f1, stage, 1);
-        __builtin_amdgcn_sched_barrier(0);
-        mma(f0);
-        __builtin_amdgcn_sched_barrier(0);
-        // this step's fragments are in registers, the next step's DMAs are done (those of the steps behind it may fly on)
-        if (t + NS - 1 < nk)
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NS - 2) * ND) : "memory");
-        else
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (t + NS < nk) issue(t + NS, stage);
-        if (t + 1 < nk) read(f0, next, 0);
-        __builtin_amdgcn_sched_barrier(0);
-        mma(f1);
-        stage = next;
+    for (int t2 = 0; t2 < nk; t2 += 2) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int t = t2 + u;
+            read(f1, t, 1);
+            __builtin_amdgcn_sched_barrier(0);
+            mma(f0);
+            __builtin_amdgcn_sched_barrier(0);
+            constexpr int XS = C::XP == 1 ? C::DX : 0;
+            if (u == 0)
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(C::NSW == 3 ? C::DW + C::DX : 0) : "memory");
+            else
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(C::NSW == 3 ? C::DW + XS : 0) : "memory");
+            issue_w(t + C::NSW);
+            if (C::XP == 1 || u == 1) issue_x(t / C::XP + C::NSX);
+            read(f0, t + 1, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            mma(f1);
+        }
     }
+    wait_vm<0>();
+    __syncthreads();
     store_tile<F, WN, WM>(o, acc, sm + wid * 32 * C::EROW, m0 + 32 * wm * WM, n0 + 32 * wn * WN, lane);
 }
 
@@ -397,7 +396,7 @@ constexpr int WK = 64, WSTAGE = 2 * 256 * 128, WLDS = 2 * WSTAGE;
 template <Form F>
 __global__ __launch_bounds__(256, 1) void linear_wide(va_tok_linear_args a, Out o, int ntn, int ntm) {
     static_assert(F == BF16 || F == BF16F, "");
-    extern __shared__ __align__(16) unsigned char sm[];  // [2][weights | tokens], rows of 128 bytes
+    extern __shared__ __align__(16) unsigned char sm[];  // [2][weights, 2 x 256 rows of 64 bytes | tokens, 256 rows of 128]
     // tiles in blocks of 4 (tokens) x all channels, tokens fastest: the 32 tiles that an XCD works on at a time share
     // their operands' rows 4 to 8 times
     const int tile = xcd_tile(blockIdx.x, gridDim.x);
@@ -407,16 +406,17 @@ __global__ __launch_bounds__(256, 1) void linear_wide(va_tok_linear_args a, Out 
     const int wn = wid & 1, wm = wid >> 1;
     const int nk = (a.K + WK - 1) / WK;
     // DMA j of this wave: rows 64 wid + 8 j .. + 7 of an operand's image, lane l row l / 8, place l % 8 (piece place ^ row).
-    // The weight rows hold channels in the order that leaves a lane 16 consecutive ones in its registers.
+    // DMA j of the weights: bytes [1024 (8 wid + j) ..) of their image, two steps of 32 one after the other.
     const int l8 = lane >> 3, piece = (lane & 7) ^ l8;
-    const int wch = 64 * wid + 16 * (l8 >> 2) + (l8 & 3);  // + 32 (j / 4) + 4 (j % 4)
-    const int woff = wch * a.Kpad * 2 + 16 * piece, xoff = (int)((64 * wid + l8) * a.ldx) * 2 + 16 * piece;
-    const unsigned char* wb = (const unsigned char*)a.w + (int64_t)n0 * a.Kpad * 2;
+    const int xoff = (int)((64 * wid + l8) * a.ldx) * 2 + 16 * piece;
+    const unsigned char* wb = (const unsigned char*)a.w + (int64_t)(n0 / 32) * 2048;
+    const int64_t wstep = (int64_t)a.Npad * 64;
     const unsigned char* xb = (const unsigned char*)a.x + (int64_t)m0 * a.ldx * 2;
-    const int wmore = a.Npad - n0 - wch, xmore = a.M - m0 - 64 * wid - l8;  // rows from this lane's first on
+    const int wend = (a.Npad - n0) * 64, xmore = a.M - m0 - 64 * wid - l8;  // bytes of a step; rows from this lane's first on
     auto issue_w = [&](int t, int j) {
-        const int up = 32 * (j / 4) + 4 * (j % 4);
-        dma16(wb, sm + (t & 1) * WSTAGE + (8 * wid + j) * 1024, up < wmore && t < nk ? woff : LIN_OOB, up * a.Kpad * 2 + t * 128);
+        const int d = 8 * wid + j, in = d % 16 * 1024;
+        dma16(wb + min(2 * t + d / 16, a.Kpad / 32 - 1) * wstep, sm + (t & 1) * WSTAGE + d * 1024,
+              in < wend && t < nk ? lane * 16 : LIN_OOB, in);
     };
     auto issue_x = [&](int t, int j) {
         const bool in = 8 * j < xmore && t * WK + 8 * piece < a.K;  // (t < nk with it)
@@ -432,13 +432,15 @@ __global__ __launch_bounds__(256, 1) void linear_wide(va_tok_linear_args a, Out 
     struct Frag {
         bf16x8 w[4], x[4];
     };
-    const int fw = (128 * wn + lc) * 128, fx = 32768 + (128 * wm + lc) * 128;  // this lane's rows (32 i more)
+    const int fw = (128 * wn + lc) * 64, fx = 32768 + (128 * wm + lc) * 128;  // this lane's rows (32 i more)
     auto read = [&](Frag& f, int t, int ks) {
-        const unsigned char* st = sm + (t & 1) * WSTAGE + 16 * ((2 * ks + lh) ^ (lc & 7));
+        const unsigned char* st = sm + (t & 1) * WSTAGE;
+        const unsigned char* sw = st + fw + ks / 2 * 16384 + 16 * ((2 * (ks & 1) + lh) ^ ((lc >> 1) & 3));
+        const unsigned char* sx = st + fx + 16 * ((2 * ks + lh) ^ (lc & 7));
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            f.w[i] = *(const bf16x8*)(st + fw + i * 4096);
-            f.x[i] = *(const bf16x8*)(st + fx + i * 4096);
+            f.w[i] = *(const bf16x8*)(sw + i * 2048);
+            f.x[i] = *(const bf16x8*)(sx + i * 4096);
         }
     };
     auto mma = [&](const Frag& f) {
@@ -504,6 +506,7 @@ __global__ __launch_bounds__(512) void linear_few(va_tok_linear_args a, Out o, i
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fr = lane & 15, fq = lane >> 4;
     const int n0 = blockIdx.x % ntn * 16, m0 = blockIdx.x / ntn * 16 * MB;
     const int nk = (a.K + 63) / 64;
+    const int wrow = (n0 / 32) * 32 + row_of((n0 & 16) + fr);  // this lane's weight row among a step's
     int64_t xrow[MB];
 #pragma unroll
     for (int j = 0; j < MB; ++j) xrow[j] = (int64_t)min(m0 + 16 * j + fr, a.M - 1) * a.ldx;
@@ -515,20 +518,23 @@ __global__ __launch_bounds__(512) void linear_few(va_tok_linear_args a, Out o, i
     };
     auto load = [&](Raw& r, int kb) {
         const int k = kb * 64 + 8 * fq;
-        if constexpr (is8(F)) {  // one 16-byte piece: chunks fq and fq + 4
-            r.w[0] = *(const u32x4*)((const uint8_t*)a.w + (int64_t)(n0 + fr) * a.Kpad + kb * 64 + 16 * fq);
+        if constexpr (is8(F)) {  // one 16-byte piece: 16 of K
+            r.w[0] = *(const u32x4*)((const uint8_t*)a.w + ((int64_t)(2 * kb + fq / 2) * (a.Npad / 32)) * 1024 + wrow * 32 +
+                                     16 * ((fq & 1) ^ ((wrow >> 2) & 1)));
         } else {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int t = 0; t < T; ++t)
-                    r.w[h * T + t] = *(const u32x4*)((const __bf16*)a.w + ((int64_t)t * a.Npad + n0 + fr) * a.Kpad + k + 32 * h);
+                    r.w[h * T + t] = *(const u32x4*)((const __bf16*)a.w + (int64_t)t * a.Npad * a.Kpad +
+                                                     ((int64_t)(2 * kb + h) * (a.Npad / 32)) * 1024 + wrow * 32 +
+                                                     8 * (fq ^ ((wrow >> 1) & 3)));
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int j = 0; j < MB; ++j) {
-                const int kk = k + 32 * h;
+                const int kk = is8(F) ? kb * 64 + 16 * fq + 8 * h : k + 32 * h;
                 if constexpr (F == F32) {
 #pragma unroll
                     for (int e = 0; e < 2; ++e)

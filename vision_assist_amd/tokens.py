@@ -22,7 +22,7 @@ import struct
 import torch
 
 from . import _lib
-from .seg import VA_DTYPE_BF16, VA_DTYPE_F32, split3_bf16, w8_order
+from .seg import VA_DTYPE_BF16, VA_DTYPE_F32, split3_bf16
 
 VOIDP, I32, I64, F32 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float
 ACTS = {None: 0, "none": 0, "silu": 1, "gelu": 2, "gelu_tanh": 3, "relu": 4}
@@ -151,6 +151,18 @@ def _here(dev: torch.device, stream) -> bool:
 
 
 # ------------------------------------------------------------------ matrix product
+def _blocks(w: torch.Tensor) -> torch.Tensor:
+    """[N, K] (multiples of 32; bf16 or bytes) in the packed order of va_tok_linear_args.w: [K / 32, N / 32, 32, 32]."""
+    N, K = w.shape
+    r = torch.arange(32, device=w.device)
+    n = 16 // w.element_size()  # values of a piece
+    ch = 16 * (r // 4 % 2) + 4 * (r // 8) + r % 4
+    turn = r // 2 % 4 if n == 8 else r // 4 % 2
+    col = ((torch.arange(32 // n, device=w.device)[None] ^ turn[:, None]) * n)[:, :, None] + torch.arange(n, device=w.device)
+    b = w.view(N // 32, 32, K // 32, 32).permute(2, 0, 1, 3)
+    return b[:, :, ch].gather(3, col.reshape(32, 32).expand(b.shape)).contiguous()
+
+
 class Linear:
     """y = act(x w^T + bias) + residual, the weights packed once.
 
@@ -196,11 +208,11 @@ class Linear:
                 w = (w / scale[:, None]).clamp(-F8_MAX, F8_MAX).to(torch.float8_e4m3fn)
             self.wscale = torch.ones(Np, dtype=torch.float32, device=self.device)
             self.wscale[:N] = scale.detach().to(self.device, torch.float32)
-            self.w = w8_order(padded(w.view(torch.uint8)))
+            self.w = _blocks(padded(w.view(torch.uint8)))
         elif dtype == "f32":
-            self.w = split3_bf16(padded(w.float())).permute(2, 0, 1, 3).reshape(3, Np, Kp).contiguous()
+            self.w = torch.stack([_blocks(t) for t in split3_bf16(padded(w.float())).permute(2, 0, 1, 3).reshape(3, Np, Kp)])
         else:
-            self.w = padded(w.to(torch.bfloat16))
+            self.w = _blocks(padded(w.to(torch.bfloat16)))
         self.bias = None if bias is None else bias.detach().to(self.device, torch.float32).contiguous()
         self._ptrs = (self.w.data_ptr(), self.wscale.data_ptr() if self.wscale is not None else 0,
                       self.bias.data_ptr() if bias is not None else 0)
