@@ -561,8 +561,7 @@ typedef struct va_tok_linear_args {
     const void* w;          /* packed weights, 16-byte aligned, zeros from row N and column K on; Kpad, Npad % 64 == 0:
                                blocks of 32 rows (of w) x 32 columns, [Kpad / 32][Npad / 32][32][32].  Place r of a block
                                holds its row 16 (r / 4 % 2) + 4 (r / 8) + r % 4, whose columns 8 p .. 8 p + 7 stand in
-                               the 16 bytes p ^ (r / 2 % 4) (w8: columns 16 p .. 16 p + 15 in the 16 bytes
-                               p ^ (r / 4 % 2)).  BF16: bf16;  w8 = 1 (BF16): e4m3 bytes;  F32: bf16 [3] such arrays,
+                               place p ^ (r / 4 % 4) of its four (w8: p ^ (r / 8 % 4)).  BF16: bf16;  w8 = 1 (BF16): e4m3 bytes;  F32: bf16 [3] such arrays,
                                the weights' exact terms h, m, l (w = h + m + l, each the round-to-nearest bf16 of what
                                remains): six exact term products each, float sums, for values below bf16's largest in
                                size */

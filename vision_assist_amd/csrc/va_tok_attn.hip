@@ -67,16 +67,17 @@ struct Dims {
     static_assert(SLDS <= 128 * 1024 && SW / 2 * NV * 16 * 64 * 4 <= SLDS, "");
 };
 
-// LDS image of a tile: rows of CS 16-byte pieces, piece c of row r in place c ^ swz(r).  K is read by 8 lanes of
-// consecutive rows at one piece, V by 4 rows at 4 pieces: both spread over the banks.
-template <int CS>
+// LDS image of a tile: rows of CS 16-byte pieces, piece c of row r in place c ^ swz(r), so that the lanes that a read
+// serves at a time (256 bytes) touch every bank once: K is read at one piece of 16 consecutive rows; V by the transposing
+// read at 4 pieces of 4 rows (bf16), or at 8 pieces of two rows 4 apart (float).
+template <typename T, int CS>
 __device__ __forceinline__ int swz(int r) {
     if constexpr (CS >= 16)
-        return ((r & 3) << 2) | ((r >> 2) & 3);
+        return sizeof(T) == 2 ? ((r & 3) << 2) | ((r >> 2) & 3) : ((r & 4) << 1) | ((r & 3) << 1) | ((r >> 3) & 1);
     else if constexpr (CS == 8)
-        return ((r & 1) << 2) | ((r >> 1) & 3);
+        return ((r & 2) << 1) | ((r >> 2) & 3);
     else
-        return (r >> 1) & 3;
+        return (r >> 2) & 3;
 }
 
 __device__ __forceinline__ int slot_of(const va_tok_attn_args& a, int p) {
@@ -151,7 +152,7 @@ __device__ __forceinline__ void softmax(Row<NV>& r, f32x16 (&sc)[KB], float c) {
 }
 
 // lane group (lh, column half): 4 keys of column 32 v + (lane & 31) from rows row0 + 4 lh .., for the two 8-key groups
-template <int CS>
+template <typename T, int CS>
 __device__ __forceinline__ u32x4 values_bf16(const unsigned char* vs, int row0, int v, int lane) {
     const int lh = lane >> 5, q = lane & 15, ch = (lane >> 4) & 1;
     u32x4 vf;
@@ -159,7 +160,7 @@ __device__ __forceinline__ u32x4 values_bf16(const unsigned char* vs, int row0, 
     for (int u = 0; u < 2; ++u) {
         // 16 lanes read 4 rows of 16 columns: lane q gets column q's 4 keys
         const int row = row0 + 8 * u + 4 * lh + (q >> 2), pc = 4 * v + 2 * ch + ((q & 3) >> 1);
-        const unsigned char* at = vs + (row * CS + (pc ^ swz<CS>(row))) * 16 + 8 * (q & 1);
+        const unsigned char* at = vs + (row * CS + (pc ^ swz<T, CS>(row))) * 16 + 8 * (q & 1);
         const u32x2 t = __builtin_bit_cast(
             u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at));
         vf[2 * u] = t[0], vf[2 * u + 1] = t[1];
@@ -183,7 +184,7 @@ __device__ __forceinline__ bool add_values(Row<DP / 32>& r, const f32x16& p, con
             if constexpr (DP > 64) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
-                u32x4 vf = values_bf16<CS>(vs, r0 + 2 * c, v, lane);
+                u32x4 vf = values_bf16<T, CS>(vs, r0 + 2 * c, v, lane);
                 if constexpr (FIN) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
@@ -203,7 +204,7 @@ __device__ __forceinline__ bool add_values(Row<DP / 32>& r, const f32x16& p, con
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
                 const int d = 32 * v + lc;
-                float x = *(const float*)(vs + (row * CS + ((d / 4) ^ swz<CS>(row))) * 16 + 4 * (d % 4));
+                float x = *(const float*)(vs + (row * CS + ((d / 4) ^ swz<T, CS>(row))) * 16 + 4 * (d % 4));
                 if constexpr (FIN) {
                     const bool nf = !(fabsf(x) < INFINITY);
                     x = nf ? 0.0f : x;
@@ -230,7 +231,7 @@ __device__ void add_nonfinite(Row<DP / 32>& r, const unsigned char* vs, int from
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int d = 32 * v + key_of(i, lh);
-                const float x = (float)*(const T*)(vs + (k * CS + ((d / VE) ^ swz<CS>(k))) * 16 + (d % VE) * sizeof(T));
+                const float x = (float)*(const T*)(vs + (k * CS + ((d / VE) ^ swz<T, CS>(k))) * 16 + (d % VE) * sizeof(T));
                 if (see && !(fabsf(x) < INFINITY)) r.acc[v][i] += x;
                 if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // few registers, not speed
             }
@@ -332,7 +333,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_kernel(va_to
     int rr[NP], ko[NP], vo[NP];
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
-        const int i = (wid * NP + j) * 64 + lane, c = (i % CS) ^ swz<CS>(i / CS);
+        const int i = (wid * NP + j) * 64 + lane, c = (i % CS) ^ swz<T, CS>(i / CS);
         rr[j] = i / CS;
         ko[j] = c * VE < a.D ? (int)(rr[j] * a.k_ss + c * VE) * (int)sizeof(T) : TILE_OOB;
         vo[j] = c * VE < a.Dv ? (int)(rr[j] * a.v_ss + c * VE) * (int)sizeof(T) : TILE_OOB;
@@ -365,7 +366,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_kernel(va_to
             for (int k = 0; k < KB; ++k) {
                 scores<T, DP>(sc[k], qf, [&](int c) {
                     const int kr = 32 * k + lc;
-                    return *(const u32x4*)(ks + (kr * CS + ((2 * c + lh) ^ swz<CS>(kr))) * 16);
+                    return *(const u32x4*)(ks + (kr * CS + ((2 * c + lh) ^ swz<T, CS>(kr))) * 16);
                 });
                 __builtin_amdgcn_sched_barrier(0);  // (one block's fragments in registers at a time)
             }
@@ -441,7 +442,7 @@ __global__ __launch_bounds__((64 * Dims<T, DP>::SW), 1) void attn_split(va_tok_a
     int ko[NP], vo[NP];  // this lane's DMAs: piece j * 64 + lane of the tile's image
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
-        const int rr = (j * 64 + lane) / CS, c = (lane % CS) ^ swz<CS>(rr);
+        const int rr = (j * 64 + lane) / CS, c = (lane % CS) ^ swz<T, CS>(rr);
         ko[j] = c * VE < a.D ? (int)(rr * a.k_ss + c * VE) * (int)sizeof(T) : TILE_OOB;
         vo[j] = c * VE < a.Dv ? (int)(rr * a.v_ss + c * VE) * (int)sizeof(T) : TILE_OOB;
     }
@@ -469,7 +470,7 @@ __global__ __launch_bounds__((64 * Dims<T, DP>::SW), 1) void attn_split(va_tok_a
         w.tile(t, &t0, &end);
         const bool sink = t < w.n0;
         f32x16 sc[1];
-        scores<T, DP>(sc[0], qf, [&](int c) { return *(const u32x4*)(ks + (lc * CS + ((2 * c + lh) ^ swz<CS>(lc))) * 16); });
+        scores<T, DP>(sc[0], qf, [&](int c) { return *(const u32x4*)(ks + (lc * CS + ((2 * c + lh) ^ swz<T, CS>(lc))) * 16); });
         if (t0 + 32 <= min(f0.top, end) && (sink || t0 >= f1.low)) {  // every row sees every key
             softmax<1, NV>(r, sc, cexp);
             add_values<T, DP>(r, sc[0], vs, 0, lane);

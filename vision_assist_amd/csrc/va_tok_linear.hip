@@ -66,8 +66,9 @@ __device__ __forceinline__ void finish4(const Out& o, int m, int n, f32x4 v) {
 // types: bf16 or e4m3 weights with bf16 tensors, the same with a float result, all float
 // Packed weights (va355.h): blocks of 32 channels x 32 of K, [Kpad / 32][Npad / 32][32 rows], a row 64 bytes of bf16 (32 of
 // e4m3) -- the image that the kernels stage, so that staging is a linear copy.  Row r of a block is channel 16 (r / 4 % 2) +
-// 4 (r / 8) + r % 4 of it: an MFMA then leaves a lane 16 consecutive channels in its registers.  Its 16-byte pieces lie in
-// place p ^ (r / 2 % 4) (e4m3: p ^ (r / 4 % 2)): eight rows' reads of one piece spread over the LDS banks.
+// 4 (r / 8) + r % 4 of it: an MFMA then leaves a lane 16 consecutive channels in its registers.  Its pieces of 8 values lie in
+// place p ^ (r / 4 % 4) (e4m3: p ^ (r / 8 % 4)): the lanes that an LDS read serves at a time (256 bytes: 16 rows' 16 bytes,
+// 32 rows' 8) touch every bank once.  With an order that is so for 8 rows alone half of the LDS' cycles were conflicts.
 __host__ __device__ constexpr int row_of(int ch) { return 8 * ((ch & 15) >> 2) + 4 * (ch >> 4) + (ch & 3); }
 
 enum Form { BF16, W8, BF16F, W8F, F32 };
@@ -97,11 +98,11 @@ __global__ __launch_bounds__(256) void linear_any(va_tok_linear_args a, Out o, i
         const int ch = n0 + row, r = row_of(ch & 31);
         const int64_t block = (int64_t)(k / 32) * (a.Npad / 32) + ch / 32;
         if constexpr (is8(FF)) {
-            wt[0] = e4m3x8(*(const uint2*)((const uint8_t*)a.w + block * 1024 + r * 32 + 16 * ((k % 32 / 16) ^ ((r >> 2) & 1)) + k % 16));
+            wt[0] = e4m3x8(*(const uint2*)((const uint8_t*)a.w + block * 1024 + r * 32 + 8 * ((k % 32 / 8) ^ ((r >> 3) & 3))));
         } else {
 #pragma unroll
             for (int t = 0; t < T; ++t)
-                wt[t] = *(const bf16x8*)((const __bf16*)a.w + (int64_t)t * a.Npad * a.Kpad + block * 1024 + r * 32 + 8 * ((k % 32 / 8) ^ ((r >> 1) & 3)));
+                wt[t] = *(const bf16x8*)((const __bf16*)a.w + (int64_t)t * a.Npad * a.Kpad + block * 1024 + r * 32 + 8 * ((k % 32 / 8) ^ ((r >> 2) & 3)));
         }
         if constexpr (FF == F32) {
             float x[8];
@@ -288,16 +289,19 @@ __global__ __launch_bounds__(256, 2) void linear_tile(va_tok_linear_args a, Out 
             dma16(from + (T > 1 ? d / C::WPL * plane : 0), to + d, t < nk && in < wend ? lane * 16 : LIN_OOB, in);
         }
     };
-    // tokens: DMA j takes rows 8 (wid DX + j) .. + 7, lane l row l / 8, place l % 8 (piece place ^ row)
-    const int l8 = lane >> 3, piece = (lane & 7) ^ l8;
+    // tokens: DMA j takes rows 8 (wid DX + j) .. + 7, lane l row l / 8, place l % 8: piece place ^ (row / 2 % 8), so rows of
+    // odd DMAs (4 more) have the other half of the pieces
+    static_assert(C::DX % 2 == 0, "");
+    const int l8 = lane >> 3, piece = (lane & 7) ^ (l8 >> 1);
     const unsigned char* xb = (const unsigned char*)a.x + (int64_t)m0 * a.ldx * XE;
-    const int xrow = 8 * wid * C::DX + l8, xoff = (int)(xrow * a.ldx) * XE + 16 * piece, xmore = a.M - m0 - xrow;
+    const int xrow = 8 * wid * C::DX + l8, xmore = a.M - m0 - xrow;
+    const int xoff[2] = {(int)(xrow * a.ldx) * XE + 16 * piece, (int)(xrow * a.ldx) * XE + 16 * (piece ^ 4)};
     auto issue_x = [&](int st) {
         unsigned char* to = sm + C::NSW * C::WB + st % C::NSX * C::XB + wid * C::DX * 1024;
-        const bool in = st * (128 / XE) + piece * (16 / XE) < a.K;
+        const bool in[2] = {st * (128 / XE) + piece * (16 / XE) < a.K, st * (128 / XE) + (piece ^ 4) * (16 / XE) < a.K};
 #pragma unroll
         for (int j = 0; j < C::DX; ++j)
-            dma16(xb, to + j * 1024, in && 8 * j < xmore ? xoff : LIN_OOB, (int)(8 * j * a.ldx) * XE + st * 128);
+            dma16(xb, to + j * 1024, in[j & 1] && 8 * j < xmore ? xoff[j & 1] : LIN_OOB, (int)(8 * j * a.ldx) * XE + st * 128);
     };
     f32x16 acc[WN][WM];
 #pragma unroll
@@ -317,10 +321,10 @@ __global__ __launch_bounds__(256, 2) void linear_tile(va_tok_linear_args a, Out 
         for (int i = 0; i < WN; ++i) {
             const unsigned char* wr = ws + (32 * (wn * WN + i) + lc) * C::WROW;
             if constexpr (is8(F)) {
-                f.w[i][0] = e4m3x8(*(const uint2*)(wr + 16 * (ks ^ ((lc >> 2) & 1)) + 8 * lh));
+                f.w[i][0] = e4m3x8(*(const uint2*)(wr + 8 * ((2 * ks + lh) ^ (lc >> 3))));
             } else {
 #pragma unroll
-                for (int p = 0; p < T; ++p) f.w[i][p] = *(const bf16x8*)(wr + p * C::WPL + 16 * ((2 * ks + lh) ^ ((lc >> 1) & 3)));
+                for (int p = 0; p < T; ++p) f.w[i][p] = *(const bf16x8*)(wr + p * C::WPL + 16 * ((2 * ks + lh) ^ ((lc >> 2) & 3)));
             }
         }
 #pragma unroll
@@ -328,11 +332,12 @@ __global__ __launch_bounds__(256, 2) void linear_tile(va_tok_linear_args a, Out 
             const unsigned char* xr = xs + (32 * (wm * WM + j) + lc) * 128;
             if constexpr (F == F32) {
                 const int p = 2 * (2 * ks + lh);
-                const f32x4 u = *(const f32x4*)(xr + 16 * (p ^ (lc & 7))), v = *(const f32x4*)(xr + 16 * ((p + 1) ^ (lc & 7)));
+                const int q = (lc >> 1) & 7;
+                const f32x4 u = *(const f32x4*)(xr + 16 * (p ^ q)), v = *(const f32x4*)(xr + 16 * ((p + 1) ^ q));
                 const float e[8] = {u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
                 split3(e, f.x[j]);
             } else {
-                f.x[j][0] = *(const bf16x8*)(xr + 16 * ((4 * (t & 1) + 2 * ks + lh) ^ (lc & 7)));
+                f.x[j][0] = *(const bf16x8*)(xr + 16 * ((4 * (t & 1) + 2 * ks + lh) ^ ((lc >> 1) & 7)));
             }
         }
     };
@@ -405,10 +410,10 @@ __global__ __launch_bounds__(256, 1) void linear_wide(va_tok_linear_args a, Out 
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lc = lane & 31, lh = lane >> 5;
     const int wn = wid & 1, wm = wid >> 1;
     const int nk = (a.K + WK - 1) / WK;
-    // DMA j of this wave: rows 64 wid + 8 j .. + 7 of an operand's image, lane l row l / 8, place l % 8 (piece place ^ row).
+    // DMA j of this wave: rows 64 wid + 8 j .. + 7 of an operand's image, lane l row l / 8, place l % 8 (piece place ^ (row / 2 % 8)).
     // DMA j of the weights: bytes [1024 (8 wid + j) ..) of their image, two steps of 32 one after the other.
-    const int l8 = lane >> 3, piece = (lane & 7) ^ l8;
-    const int xoff = (int)((64 * wid + l8) * a.ldx) * 2 + 16 * piece;
+    const int l8 = lane >> 3, piece = (lane & 7) ^ (l8 >> 1);
+    const int xoff[2] = {(int)((64 * wid + l8) * a.ldx) * 2 + 16 * piece, (int)((64 * wid + l8) * a.ldx) * 2 + 16 * (piece ^ 4)};
     const unsigned char* wb = (const unsigned char*)a.w + (int64_t)(n0 / 32) * 2048;
     const int64_t wstep = (int64_t)a.Npad * 64;
     const unsigned char* xb = (const unsigned char*)a.x + (int64_t)m0 * a.ldx * 2;
@@ -419,8 +424,8 @@ __global__ __launch_bounds__(256, 1) void linear_wide(va_tok_linear_args a, Out 
               in < wend && t < nk ? lane * 16 : LIN_OOB, in);
     };
     auto issue_x = [&](int t, int j) {
-        const bool in = 8 * j < xmore && t * WK + 8 * piece < a.K;  // (t < nk with it)
-        dma16(xb, sm + (t & 1) * WSTAGE + 32768 + (8 * wid + j) * 1024, in ? xoff : LIN_OOB, (int)(8 * j * a.ldx) * 2 + t * 128);
+        const bool in = 8 * j < xmore && t * WK + 8 * (piece ^ (j & 1 ? 4 : 0)) < a.K;  // (t < nk with it)
+        dma16(xb, sm + (t & 1) * WSTAGE + 32768 + (8 * wid + j) * 1024, in ? xoff[j & 1] : LIN_OOB, (int)(8 * j * a.ldx) * 2 + t * 128);
     };
     f32x16 acc[4][4];
 #pragma unroll
@@ -435,8 +440,8 @@ __global__ __launch_bounds__(256, 1) void linear_wide(va_tok_linear_args a, Out 
     const int fw = (128 * wn + lc) * 64, fx = 32768 + (128 * wm + lc) * 128;  // this lane's rows (32 i more)
     auto read = [&](Frag& f, int t, int ks) {
         const unsigned char* st = sm + (t & 1) * WSTAGE;
-        const unsigned char* sw = st + fw + ks / 2 * 16384 + 16 * ((2 * (ks & 1) + lh) ^ ((lc >> 1) & 3));
-        const unsigned char* sx = st + fx + 16 * ((2 * ks + lh) ^ (lc & 7));
+        const unsigned char* sw = st + fw + ks / 2 * 16384 + 16 * ((2 * (ks & 1) + lh) ^ ((lc >> 2) & 3));
+        const unsigned char* sx = st + fx + 16 * ((2 * ks + lh) ^ ((lc >> 1) & 7));
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             f.w[i] = *(const bf16x8*)(sw + i * 2048);
@@ -520,7 +525,8 @@ __global__ __launch_bounds__(512) void linear_few(va_tok_linear_args a, Out o, i
         const int k = kb * 64 + 8 * fq;
         if constexpr (is8(F)) {  // one 16-byte piece: 16 of K
             r.w[0] = *(const u32x4*)((const uint8_t*)a.w + ((int64_t)(2 * kb + fq / 2) * (a.Npad / 32)) * 1024 + wrow * 32 +
-                                     16 * ((fq & 1) ^ ((wrow >> 2) & 1)));
+                                     16 * ((fq & 1) ^ ((wrow >> 4) & 1)));
+            if (wrow & 8) r.w[0] = (u32x4){r.w[0][2], r.w[0][3], r.w[0][0], r.w[0][1]};
         } else {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
@@ -528,7 +534,7 @@ __global__ __launch_bounds__(512) void linear_few(va_tok_linear_args a, Out o, i
                 for (int t = 0; t < T; ++t)
                     r.w[h * T + t] = *(const u32x4*)((const __bf16*)a.w + (int64_t)t * a.Npad * a.Kpad +
                                                      ((int64_t)(2 * kb + h) * (a.Npad / 32)) * 1024 + wrow * 32 +
-                                                     8 * (fq ^ ((wrow >> 1) & 3)));
+                                                     8 * (fq ^ ((wrow >> 2) & 3)));
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h)

@@ -155,10 +155,9 @@ def _blocks(w: torch.Tensor) -> torch.Tensor:
     """[N, K] (multiples of 32; bf16 or bytes) in the packed order of va_tok_linear_args.w: [K / 32, N / 32, 32, 32]."""
     N, K = w.shape
     r = torch.arange(32, device=w.device)
-    n = 16 // w.element_size()  # values of a piece
     ch = 16 * (r // 4 % 2) + 4 * (r // 8) + r % 4
-    turn = r // 2 % 4 if n == 8 else r // 4 % 2
-    col = ((torch.arange(32 // n, device=w.device)[None] ^ turn[:, None]) * n)[:, :, None] + torch.arange(n, device=w.device)
+    turn = r // (4 if w.element_size() == 2 else 8) % 4
+    col = 8 * (torch.arange(4, device=w.device) ^ turn[:, None])[:, :, None] + torch.arange(8, device=w.device)
     b = w.view(N // 32, 32, K // 32, 32).permute(2, 0, 1, 3)
     return b[:, :, ch].gather(3, col.reshape(32, 32).expand(b.shape)).contiguous()
 
