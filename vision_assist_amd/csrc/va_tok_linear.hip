@@ -2,8 +2,6 @@
 //
 // The weights are the MFMA's A operand (its rows are output channels) and the tokens its B operand, so a lane's
 // accumulator registers are consecutive channels of one token: the epilogue stores them as vectors.
-#include <type_traits>
-
 #include "va_dev.h"
 #include "va_tok.h"
 
@@ -153,6 +151,16 @@ __global__ __launch_bounds__(256) void linear_any(va_tok_linear_args a, Out o, i
 // the six term products that are kept of (h + m + l)(h + m + l)
 constexpr int NTERM = 6, TERM_W[6] = {0, 0, 1, 0, 1, 2}, TERM_X[6] = {0, 1, 0, 2, 1, 0};
 
+// Tile i of ntn x ntm in groups of G rows of token tiles, tokens fastest: the consecutive tiles that an XCD works on at a
+// time form a block G high, so that each operand's rows come from beyond its L2 few times (G = 1 at 8192^3: 64 tiles of
+// 256 x 128 in two rows fetched 528 KB a step, 937 TFLOP/s).
+template <int G>
+__device__ __forceinline__ void grouped_tile(int i, int ntn, int ntm, int* tn, int* tm) {
+    const int grp = i / (G * ntn), gm = min(G, ntm - G * grp), in = i - G * grp * ntn;
+    *tm = G * grp + in % gm;
+    *tn = in / gm;
+}
+
 // ------------------------------------------------------------------ many tiles: LDS-DMA rings, counted waits
 // 64 WN channels x 64 WM tokens per workgroup, four waves of 32 WN x 32 WM on v_mfma_f32_32x32x16_bf16, K in steps of 32.
 // Weights go through a ring of NSW stages of a step; tokens in stages of whole 128-byte lines, two steps of bf16 or one of
@@ -267,12 +275,13 @@ struct TileCfg {
 };
 
 template <Form F, int WN, int WM>
-__global__ __launch_bounds__(256, 2) void linear_tile(va_tok_linear_args a, Out o, int ntn) {
+__global__ __launch_bounds__(256, 2) void linear_tile(va_tok_linear_args a, Out o, int ntn, int ntm) {
     using C = TileCfg<F, WN, WM>;
     constexpr int T = C::T, XE = F == F32 ? 4 : 2;
     extern __shared__ __align__(16) unsigned char sm[];  // [NSW] weights, [NSX] tokens
-    const int tile = xcd_tile(blockIdx.x, gridDim.x);
-    const int n0 = tile % ntn * C::BN, m0 = tile / ntn * C::BM;
+    int tn, tm;
+    grouped_tile<8>(xcd_tile(blockIdx.x, gridDim.x), ntn, ntm, &tn, &tm);
+    const int n0 = tn * C::BN, m0 = tm * C::BM;
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lc = lane & 31, lh = lane >> 5;
     const int wn = wid & 1, wm = wid >> 1;
     const int nk = 2 * ((a.K + 63) / 64);
@@ -313,6 +322,7 @@ __global__ __launch_bounds__(256, 2) void linear_tile(va_tok_linear_args a, Out 
 
     struct Frag {
         bf16x8 w[WN][T], x[WM][T];
+        f32x4 raw[F == F32 ? WM : 1][2];
     };
     auto read = [&](Frag& f, int t, int ks) {
         const unsigned char* ws = sm + t % C::NSW * C::WB;
@@ -333,9 +343,7 @@ __global__ __launch_bounds__(256, 2) void linear_tile(va_tok_linear_args a, Out 
             if constexpr (F == F32) {
                 const int p = 2 * (2 * ks + lh);
                 const int q = (lc >> 1) & 7;
-                const f32x4 u = *(const f32x4*)(xr + 16 * (p ^ q)), v = *(const f32x4*)(xr + 16 * ((p + 1) ^ q));
-                const float e[8] = {u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
-                split3(e, f.x[j]);
+                f.raw[j][0] = *(const f32x4*)(xr + 16 * (p ^ q)), f.raw[j][1] = *(const f32x4*)(xr + 16 * ((p + 1) ^ q));
             } else {
                 f.x[j][0] = *(const bf16x8*)(xr + 16 * ((4 * (t & 1) + 2 * ks + lh) ^ ((lc >> 1) & 7)));
             }
@@ -351,6 +359,34 @@ __global__ __launch_bounds__(256, 2) void linear_tile(va_tok_linear_args a, Out 
                     acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.w[i][T > 1 ? TERM_W[t] : 0], f.x[j][T > 1 ? TERM_X[t] : 0],
                                                                         acc[i][j], 0, 0, 0);
     };
+    auto split = [&](Frag& f) {  // F32: the tokens' terms
+        if constexpr (F == F32) {
+#pragma unroll
+            for (int j = 0; j < WM; ++j) {
+                const f32x4 u = f.raw[j][0], v = f.raw[j][1];
+                const float e[8] = {u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
+                split3(e, f.x[j]);
+            }
+        }
+    };
+    // the next slice's fragments are read before this slice's MFMAs; F32: and split beside the second half of them
+    auto slice = [&](Frag& next, const Frag& f) {
+        if constexpr (F == F32) {
+            mma(f);
+            split(next);
+            constexpr int NM = NTERM * WN * WM, NV = 52 * WM;
+            __builtin_amdgcn_sched_group_barrier(0x100, WN * T + 2 * WM, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, NM / 2, 0);
+#pragma unroll
+            for (int i = 0; i < NM - NM / 2; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x002, NV / (NM - NM / 2), 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            }
+        } else {
+            __builtin_amdgcn_sched_barrier(0);
+            mma(f);
+        }
+    };
     // in the order in which the steps need them; past the last step they run on, on offsets out of range
     issue_x(0);
     issue_w(0);
@@ -364,13 +400,13 @@ __global__ __launch_bounds__(256, 2) void linear_tile(va_tok_linear_args a, Out 
     asm volatile("s_barrier" ::: "memory");
     Frag f0, f1;
     read(f0, 0, 0);
+    split(f0);
     for (int t2 = 0; t2 < nk; t2 += 2) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const int t = t2 + u;
             read(f1, t, 1);
-            __builtin_amdgcn_sched_barrier(0);
-            mma(f0);
+            slice(f1, f0);
             __builtin_amdgcn_sched_barrier(0);
             constexpr int XS = C::XP == 1 ? C::DX : 0;
             if (u == 0)
@@ -380,124 +416,13 @@ __global__ __launch_bounds__(256, 2) void linear_tile(va_tok_linear_args a, Out 
             issue_w(t + C::NSW);
             if (C::XP == 1 || u == 1) issue_x(t / C::XP + C::NSX);
             read(f0, t + 1, 0);
-            __builtin_amdgcn_sched_barrier(0);
-            mma(f1);
+            slice(f0, f1);
+            if constexpr (F == F32) __builtin_amdgcn_sched_barrier(0);
         }
     }
     wait_vm<0>();
     __syncthreads();
     store_tile<F, WN, WM>(o, acc, sm + wid * 32 * C::EROW, m0 + 32 * wm * WM, n0 + 32 * wn * WN, lane);
-}
-
-// ------------------------------------------------------------------ many large tiles
-// 256 channels x 256 tokens per workgroup, one a CU: four waves of 128 x 128 (256 accumulator registers) need the fewest
-// fragment reads per MFMA -- 128 KB of LDS reads and 64 KB of DMA writes per 2048 MFMA cycles, against 128 bytes a cycle;
-// two waves a SIMD of 128 x 64 would need all of it.  K in steps of 64, so that a DMA's rows are whole cache lines (rows of
-// 64 bytes fetched each line twice: 682 against ... TFLOP/s at 8192^3), two stages.  A step is four slices of 16; the
-// fragments of a slice are read beside the MFMAs of the slice before.  One barrier a step, before its last slice, whose
-// fragments are in registers by then: it frees this stage for step t + 2 and publishes step t + 1.
-constexpr int WK = 64, WSTAGE = 2 * 256 * 128, WLDS = 2 * WSTAGE;
-
-template <Form F>
-__global__ __launch_bounds__(256, 1) void linear_wide(va_tok_linear_args a, Out o, int ntn, int ntm) {
-    static_assert(F == BF16 || F == BF16F, "");
-    extern __shared__ __align__(16) unsigned char sm[];  // [2][weights, 2 x 256 rows of 64 bytes | tokens, 256 rows of 128]
-    // tiles in blocks of 4 (tokens) x all channels, tokens fastest: the 32 tiles that an XCD works on at a time share
-    // their operands' rows 4 to 8 times
-    const int tile = xcd_tile(blockIdx.x, gridDim.x);
-    const int grp = tile / (4 * ntn), gm = min(4, ntm - 4 * grp), in = tile - 4 * grp * ntn;
-    const int m0 = (4 * grp + in % gm) * 256, n0 = in / gm * 256;
-    const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lc = lane & 31, lh = lane >> 5;
-    const int wn = wid & 1, wm = wid >> 1;
-    const int nk = (a.K + WK - 1) / WK;
-    // DMA j of this wave: rows 64 wid + 8 j .. + 7 of an operand's image, lane l row l / 8, place l % 8 (piece place ^ (row / 2 % 8)).
-    // DMA j of the weights: bytes [1024 (8 wid + j) ..) of their image, two steps of 32 one after the other.
-    const int l8 = lane >> 3, piece = (lane & 7) ^ (l8 >> 1);
-    const int xoff[2] = {(int)((64 * wid + l8) * a.ldx) * 2 + 16 * piece, (int)((64 * wid + l8) * a.ldx) * 2 + 16 * (piece ^ 4)};
-    const unsigned char* wb = (const unsigned char*)a.w + (int64_t)(n0 / 32) * 2048;
-    const int64_t wstep = (int64_t)a.Npad * 64;
-    const unsigned char* xb = (const unsigned char*)a.x + (int64_t)m0 * a.ldx * 2;
-    const int wend = (a.Npad - n0) * 64, xmore = a.M - m0 - 64 * wid - l8;  // bytes of a step; rows from this lane's first on
-    auto issue_w = [&](int t, int j) {
-        const int d = 8 * wid + j, in = d % 16 * 1024;
-        dma16(wb + min(2 * t + d / 16, a.Kpad / 32 - 1) * wstep, sm + (t & 1) * WSTAGE + d * 1024,
-              in < wend && t < nk ? lane * 16 : LIN_OOB, in);
-    };
-    auto issue_x = [&](int t, int j) {
-        const bool in = 8 * j < xmore && t * WK + 8 * (piece ^ (j & 1 ? 4 : 0)) < a.K;  // (t < nk with it)
-        dma16(xb, sm + (t & 1) * WSTAGE + 32768 + (8 * wid + j) * 1024, in ? xoff[j & 1] : LIN_OOB, (int)(8 * j * a.ldx) * 2 + t * 128);
-    };
-    f32x16 acc[4][4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
-    struct Frag {
-        bf16x8 w[4], x[4];
-    };
-    const int fw = (128 * wn + lc) * 64, fx = 32768 + (128 * wm + lc) * 128;  // this lane's rows (32 i more)
-    auto read = [&](Frag& f, int t, int ks) {
-        const unsigned char* st = sm + (t & 1) * WSTAGE;
-        const unsigned char* sw = st + fw + ks / 2 * 16384 + 16 * ((2 * (ks & 1) + lh) ^ ((lc >> 2) & 3));
-        const unsigned char* sx = st + fx + 16 * ((2 * ks + lh) ^ ((lc >> 1) & 7));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            f.w[i] = *(const bf16x8*)(sw + i * 2048);
-            f.x[i] = *(const bf16x8*)(sx + i * 4096);
-        }
-    };
-    auto mma = [&](const Frag& f) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.w[i], f.x[j], acc[i][j], 0, 0, 0);
-    };
-    // sixteen MFMAs with eight fragment reads and DMAS DMAs between them
-    auto spread = [&](auto dmas) {
-        constexpr int DMAS = decltype(dmas)::value;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-            if (DMAS == 8 || (DMAS == 4 && i % 2)) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-    };
-    // The DMAs of a stage that becomes free at a step's barrier go out over three slices: the tokens' (from far) first.
-    // Past the last step they and the reads run on, on offsets out of range and stale stages, so that the loop is one block.
-    for (int j = 0; j < 8; ++j) issue_x(0, j), issue_w(0, j);
-    for (int j = 0; j < 8; ++j) issue_x(1, j);
-    wait_vm<8>();
-    asm volatile("s_barrier" ::: "memory");
-    Frag f0, f1;
-    read(f0, 0, 0);
-    for (int t = 0; t < nk; ++t) {
-        read(f1, t, 1);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) issue_w(t + 1, j);
-        mma(f0);
-        spread(std::integral_constant<int, 4>());
-        read(f0, t, 2);
-#pragma unroll
-        for (int j = 4; j < 8; ++j) issue_w(t + 1, j);
-        mma(f1);
-        spread(std::integral_constant<int, 4>());
-        read(f1, t, 3);
-        mma(f0);
-        spread(std::integral_constant<int, 0>());
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        read(f0, t + 1, 0);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) issue_x(t + 2, j);
-        mma(f1);
-        spread(std::integral_constant<int, 8>());
-    }
-    wait_vm<0>();
-    __syncthreads();
-    store_tile<F, 4, 4>(o, acc, sm + wid * 32 * 528, m0 + 128 * wm, n0 + 128 * wn, lane);
 }
 
 // ------------------------------------------------------------------ few tiles: K over the waves of a workgroup
@@ -629,20 +554,7 @@ hipError_t go_tile(const va_tok_linear_args& a, const Out& o, hipStream_t st) {
         attr() = true;
     }
     const int ntn = (a.N + C::BN - 1) / C::BN, ntm = (a.M + C::BM - 1) / C::BM;
-    hipLaunchKernelGGL((linear_tile<F, WN, WM>), dim3((unsigned)(ntn * ntm)), dim3(256), lds, st, a, o, ntn);
-    return hipGetLastError();
-}
-
-template <Form F>
-hipError_t go_wide(const va_tok_linear_args& a, const Out& o, hipStream_t st) {
-    static DevFlag attr;
-    if (!attr()) {
-        const hipError_t e = hipFuncSetAttribute((const void*)linear_wide<F>, hipFuncAttributeMaxDynamicSharedMemorySize, WLDS);
-        if (e != hipSuccess) return e;
-        attr() = true;
-    }
-    const int ntn = (a.N + 255) / 256, ntm = (a.M + 255) / 256;
-    hipLaunchKernelGGL(linear_wide<F>, dim3((unsigned)(ntn * ntm)), dim3(256), WLDS, st, a, o, ntn, ntm);
+    hipLaunchKernelGGL((linear_tile<F, WN, WM>), dim3((unsigned)(ntn * ntm)), dim3(256), lds, st, a, o, ntn, ntm);
     return hipGetLastError();
 }
 
@@ -668,15 +580,16 @@ hipError_t go(const va_tok_linear_args& a, const Out& o, hipStream_t st) {
     const int64_t t64 = (int64_t)((a.N + 63) / 64) * ((a.M + 63) / 64);
     if (a.M <= 16) return go_few<F, 1>(a, o, st);
     if (a.M <= 32) return go_few<F, 2>(a, o, st);
-    if (a.M <= 64 || t64 < 128) return go_few<F, 4>(a, o, st);
+    // Measured (us, graph replays, K 512-4096; few | 128 x 64 tiles | 256 x 128): bf16 64 tiles of 64 x 64 20.4 | 30.8,
+    // 56: 4.8 | 7.2, 112: 11.1 | 10.3, 256: 17.9 | 10.5; large tiles 100: 16.0 | 23.9, 208: 25.2 | 25.5, 400: 42.0 | 37.4
+    // (e4m3 208: 28.9 | 33.4, 400: 50.1 | 44.5).  Float, few | 64 x 64 | 128 x 64: 56: 8.3 | 13.3, 112: 25.8 | 23.7,
+    // 208: 25.3 | 30.5, 400: 35.3 | 33.5, 832: 74 | 53
+    if (a.M <= 64 || t64 < 100) return go_few<F, 4>(a, o, st);
     if constexpr (F == F32) {
-        return t64 < 1024 ? go_tile<F32, 1, 1>(a, o, st) : go_tile<F32, 2, 1>(a, o, st);
+        return t64 < 320 ? go_tile<F32, 1, 1>(a, o, st) : go_tile<F32, 2, 1>(a, o, st);
     } else {
-        if constexpr (!is8(F)) {
-            if ((int64_t)((a.N + 255) / 256) * ((a.M + 255) / 256) >= 192) return go_wide<F>(a, o, st);
-        }
-        if ((int64_t)((a.N + 255) / 256) * ((a.M + 127) / 128) >= 384) return go_tile<F, 4, 2>(a, o, st);
-        return go_tile<F, 2, 1>(a, o, st);
+        const int64_t big = (int64_t)((a.N + 255) / 256) * ((a.M + 127) / 128);
+        return big >= (is8(F) ? 320 : 224) ? go_tile<F, 4, 2>(a, o, st) : go_tile<F, 2, 1>(a, o, st);
     }
 }
 }  // namespace
