@@ -151,16 +151,35 @@ __device__ __forceinline__ void softmax(Row<NV>& r, f32x16 (&sc)[KB], float c) {
     r.sum += (part[0] + part[1]) + (part[2] + part[3]);
 }
 
-// lane group (lh, column half): 4 keys of column 32 v + (lane & 31) from rows row0 + 4 lh .., for the two 8-key groups
-template <typename T, int CS>
-__device__ __forceinline__ u32x4 values_bf16(const unsigned char* vs, int row0, int v, int lane) {
-    const int lh = lane >> 5, q = lane & 15, ch = (lane >> 4) & 1;
+// This lane's LDS addresses in a tile's image, formed once: K of row lane & 31, piece 2 c + lh; V for the reads of block v.
+// bf16: 16 lanes read 4 keys of 16 columns (rows 4 lh + 0 .. 3 of the 8-key group u, columns 32 v + 16 (lane / 16 % 2) ..)
+// and lane q of them gets column q's 4 keys.  Later keys of a tile are a constant away (32 rows' swizzles are 0 .. 31's).
+template <typename T, int DP>
+struct Addr {
+    static constexpr int CS = Dims<T, DP>::CS, NV = DP / 32, NF = DP / (2 * Tr<T>::VE), U = sizeof(T) == 2 ? 2 : 1;
+    int k[NF], v[U][NV];
+    __device__ __forceinline__ Addr(int lane) {
+        const int lc = lane & 31, lh = lane >> 5, q = lane & 15, ch = (lane >> 4) & 1;
+#pragma unroll
+        for (int c = 0; c < NF; ++c) k[c] = (lc * CS + ((2 * c + lh) ^ swz<T, CS>(lc))) * 16;
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    const int row = 8 * u + 4 * lh + (q >> 2), pc = 4 * i + 2 * ch + ((q & 3) >> 1);
+                    v[u][i] = (row * CS + (pc ^ swz<T, CS>(row))) * 16 + 8 * (q & 1);
+                }
+        }
+    }
+};
+
+template <typename T, int DP>
+__device__ __forceinline__ u32x4 values_bf16(const Addr<T, DP>& ad, const unsigned char* vs, int row0, int v) {
     u32x4 vf;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-        // 16 lanes read 4 rows of 16 columns: lane q gets column q's 4 keys
-        const int row = row0 + 8 * u + 4 * lh + (q >> 2), pc = 4 * v + 2 * ch + ((q & 3) >> 1);
-        const unsigned char* at = vs + (row * CS + (pc ^ swz<T, CS>(row))) * 16 + 8 * (q & 1);
+        const unsigned char* at = vs + ad.v[u][v] + row0 * (Dims<T, DP>::CS * 16);
         const u32x2 t = __builtin_bit_cast(
             u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at));
         vf[2 * u] = t[0], vf[2 * u + 1] = t[1];
@@ -168,33 +187,21 @@ __device__ __forceinline__ u32x4 values_bf16(const unsigned char* vs, int row0, 
     return vf;
 }
 
-// O^T += V^T P^T over 32 keys whose values lie in LDS rows r0 .. r0 + 31 of vs.  FIN: values that are not finite count as
-// zeros (add_nonfinite adds them)
-// -> whether this lane met any
-template <typename T, int DP, bool FIN = false>
-__device__ __forceinline__ bool add_values(Row<DP / 32>& r, const f32x16& p, const unsigned char* vs, int r0, int lane) {
+// O^T += V^T P^T over 32 keys whose values lie in LDS rows r0 .. r0 + 31 of vs
+template <typename T, int DP>
+__device__ __forceinline__ void add_values(Row<DP / 32>& r, const f32x16& p, const Addr<T, DP>& ad, const unsigned char* vs, int r0,
+                                           int lane) {
     constexpr int CS = Dims<T, DP>::CS, NV = DP / 32;
-    bool bad = false;
     if constexpr (sizeof(T) == 2) {
 #pragma unroll
         for (int c = 0; c < 16; c += 8) {
             u32x4 pf;
 #pragma unroll
             for (int e = 0; e < 4; ++e) pf[e] = pk_bf16(p[c + 2 * e], p[c + 2 * e + 1]);
-            if constexpr (DP > 64) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int v = 0; v < NV; ++v) {
-                u32x4 vf = values_bf16<T, CS>(vs, r0 + 2 * c, v, lane);
-                if constexpr (FIN) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const bool lo = (vf[e] & 0x7f80u) == 0x7f80u, hi = (vf[e] & 0x7f800000u) == 0x7f800000u;
-                        vf[e] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
-                        bad |= lo || hi;
-                    }
-                }
-                r.acc[v] = __builtin_amdgcn_mfma_f32_32x32x16_bf16((bf16x8)vf, (bf16x8)pf, r.acc[v], 0, 0, 0);
-            }
+            for (int v = 0; v < NV; ++v)
+                r.acc[v] = __builtin_amdgcn_mfma_f32_32x32x16_bf16((bf16x8)values_bf16<T, DP>(ad, vs, r0 + 2 * c, v), (bf16x8)pf,
+                                                                  r.acc[v], 0, 0, 0);
         }
     } else {
         const int lc = lane & 31, lh = lane >> 5;
@@ -204,36 +211,60 @@ __device__ __forceinline__ bool add_values(Row<DP / 32>& r, const f32x16& p, con
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
                 const int d = 32 * v + lc;
-                float x = *(const float*)(vs + (row * CS + ((d / 4) ^ swz<T, CS>(row))) * 16 + 4 * (d % 4));
-                if constexpr (FIN) {
-                    const bool nf = !(fabsf(x) < INFINITY);
-                    x = nf ? 0.0f : x;
-                    bad |= nf;
-                }
+                const float x = *(const float*)(vs + (row * CS + ((d / 4) ^ swz<T, CS>(row))) * 16 + 4 * (d % 4));
                 r.acc[v] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, p[i], r.acc[v], 0, 0, 0);
             }
         }
     }
-    return bad;
 }
 
-// A tile that some row does not see whole and that holds values which are not finite: the product would carry them, as
-// 0 x inf, into rows that do not see their key.  They are left out of it, and each row adds those of the keys it sees
-// (positions from .. to - 1 of the tile's n keys).
+// Values that are not finite, in tiles that some row does not see whole: the product would carry them, as 0 x inf, into
+// rows that do not see their key.  A wave takes them out of the pieces that it has staged -- zeros in their places, two
+// bits a value of what stood there (1 +inf, 2 -inf, 3 NaN) in kinds, one word a piece -- and after the product each row
+// adds those of the keys it sees.
+template <typename T>
+__device__ __forceinline__ bool take_out(unsigned char* piece, unsigned short* kind) {
+    u32x4 x = *(const u32x4*)piece;
+    unsigned k = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const unsigned y = x[e] >> (16 * h) & 0xffffu;
+                if ((y & 0x7f80u) == 0x7f80u) {
+                    k |= (y & 0x7fu ? 3u : y >> 15 ? 2u : 1u) << (4 * e + 2 * h);
+                    x[e] &= h ? 0xffffu : 0xffff0000u;
+                }
+            }
+        } else if ((x[e] & 0x7f800000u) == 0x7f800000u) {
+            k |= (x[e] & 0x7fffffu ? 3u : x[e] >> 31 ? 2u : 1u) << (2 * e);
+            x[e] = 0;
+        }
+    }
+    *kind = (unsigned short)k;
+    if (k) *(u32x4*)piece = x;
+    return k != 0;
+}
+
+// ... positions from .. to - 1 of the tile's n keys are seen
 template <typename T, int DP>
-__device__ void add_nonfinite(Row<DP / 32>& r, const unsigned char* vs, int from, int to, int n, int lh) {
+__device__ __forceinline__ void add_nonfinite(Row<DP / 32>& r, const unsigned short* kinds, int from, int to, int n, int lh) {
     constexpr int CS = Dims<T, DP>::CS, NV = DP / 32, VE = Tr<T>::VE;
 #pragma unroll 1
-    for (int k = 0; k < n; ++k) {
-        const bool see = k >= from && k < to;
+    for (int k = max(from, 0); k < min(to, n); ++k) {
 #pragma unroll
         for (int v = 0; v < NV; ++v)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
+            for (int i = 0; i < 16; i += 4) {  // four values of one piece
                 const int d = 32 * v + key_of(i, lh);
-                const float x = (float)*(const T*)(vs + (k * CS + ((d / VE) ^ swz<T, CS>(k))) * 16 + (d % VE) * sizeof(T));
-                if (see && !(fabsf(x) < INFINITY)) r.acc[v][i] += x;
-                if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // few registers, not speed
+                const unsigned w = kinds[k * CS + ((d / VE) ^ swz<T, CS>(k))] >> (2 * (d % VE));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const unsigned q = w >> (2 * e) & 3u;
+                    if (q) r.acc[v][i + e] += q == 1 ? INFINITY : q == 2 ? -INFINITY : NAN;
+                }
+                __builtin_amdgcn_sched_barrier(0);  // few registers, not speed
             }
     }
 }
@@ -293,9 +324,9 @@ struct Walk {
 constexpr int TILE_OOB = 0x7ffffff0;
 
 // (a plain function: the host pass drops the stub of a kernel template that names the builtin)
-__device__ __forceinline__ void dma16(const void* base, void* lds, int off) {
+__device__ __forceinline__ void dma16(const void* base, void* lds, int off, int uniform) {
     const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, TILE_OOB, 0x00020000);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lvoid_t*)lds, 16, off, 0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lvoid_t*)lds, 16, off, uniform, 0, 0);
 }
 
 template <typename T, int DP>
@@ -303,6 +334,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_kernel(va_to
     constexpr int VE = Tr<T>::VE, KT = Tr<T>::KT, CS = Dims<T, DP>::CS, KB = KT / 32, NV = DP / 32;
     constexpr int NP = KT * CS / 256, BUF = KT * CS * 16;  // DMAs of a wave for K; bytes of a tile of K
     extern __shared__ __align__(16) unsigned char sm[];    // [2][K | V]
+    __shared__ unsigned short kinds[2][KT * CS];
+    __shared__ int bad_tile[2];  // the tile of a buffer, if values were taken out of it
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), lc = lane & 31, lh = lane >> 5;
     const int G = a.Hq / a.Hk;
     int bid = xcd_tile(blockIdx.x, gridDim.x);
@@ -316,7 +349,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_kernel(va_to
     const bool there = row < rows;
     const Span sp = there ? attn_span(a, sq, sq.first + s) : Span{a.sinks, 0};
     // spans grow with the position: the workgroup's keys, and this wave's
-    const Walk<KT> w(a, attn_span(a, sq, max(sq.first + r0 / G, 0)), attn_span(a, sq, sq.first + (min(r0 + 128, rows) - 1) / G));
+    const Span g0 = attn_span(a, sq, sq.first + r0 / G), g1 = attn_span(a, sq, sq.first + (min(r0 + 128, rows) - 1) / G);
+    const Walk<KT> w(a, attn_span(a, sq, max(sq.first + r0 / G, 0)), g1);
     const Span f0 = attn_span(a, sq, sq.first + min(r0 + 32 * wid, rows - 1) / G);
     const Span f1 = attn_span(a, sq, sq.first + min(r0 + 32 * wid + 31, rows - 1) / G);
     const bool idle = r0 + 32 * wid >= rows;
@@ -326,31 +360,53 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_kernel(va_to
     const float cexp = a.scale * 1.4426950408889634f;
     Row<NV> r;
     r.clear();
+    const Addr<T, DP> ad(lane);
 
     const T* kb = (const T*)a.k + b * a.k_sb + hk * a.k_sh;
     const T* vb = (const T*)a.v + b * a.v_sb + hk * a.v_sh;
-    // this lane's DMAs: piece i = (wid * NP + j) * 64 + lane of the tile's image
-    int rr[NP], ko[NP], vo[NP];
-#pragma unroll
-    for (int j = 0; j < NP; ++j) {
-        const int i = (wid * NP + j) * 64 + lane, c = (i % CS) ^ swz<T, CS>(i / CS);
-        rr[j] = i / CS;
-        ko[j] = c * VE < a.D ? (int)(rr[j] * a.k_ss + c * VE) * (int)sizeof(T) : TILE_OOB;
-        vo[j] = c * VE < a.Dv ? (int)(rr[j] * a.v_ss + c * VE) * (int)sizeof(T) : TILE_OOB;
-    }
+    // this lane's DMAs: place i = (wid * NP + j) * 64 + lane of the tile's image, row i / CS = r_0 + j RS, piece i % CS ^ swz
+    constexpr int RS = 64 / CS > 0 ? 64 / CS : 1;
+    const int rr = wid * NP * RS + lane / CS;
+    const int krow = (int)(rr * a.k_ss) * (int)sizeof(T), vrow = (int)(rr * a.v_ss) * (int)sizeof(T);
+    const bool whole_d = a.D == DP && a.Dv == DP;
     auto fetch = [&](int t, int buf) {
         int t0, end;
         w.tile(t, &t0, &end);
         const int64_t slot = slot_of(a, t0);
         const T *kt = kb + slot * a.k_ss, *vt = vb + slot * a.v_ss;
         unsigned char* ks = sm + buf * 2 * BUF + wid * NP * 1024;
+        const bool whole = whole_d && t0 + KT <= end;  // (uniform) no row and no piece is missing
 #pragma unroll
-        for (int j = 0; j < NP; ++j) dma16(kt, ks + j * 1024, t0 + rr[j] < end ? ko[j] : TILE_OOB);
-#pragma unroll
-        for (int j = 0; j < NP; ++j) dma16(vt, ks + BUF + j * 1024, t0 + rr[j] < end ? vo[j] : TILE_OOB);
+        for (int j = 0; j < NP; ++j) {
+            const int c = lane % CS ^ swz<T, CS>(rr + j * RS);
+            const bool in = whole || t0 + rr + j * RS < end;
+            dma16(kt, ks + j * 1024, in && (whole || c * VE < a.D) ? krow + 16 * c : TILE_OOB, j * RS * (int)a.k_ss * (int)sizeof(T));
+            dma16(vt, ks + BUF + j * 1024, in && (whole || c * VE < a.Dv) ? vrow + 16 * c : TILE_OOB,
+                  j * RS * (int)a.v_ss * (int)sizeof(T));
+        }
     };
-    if (w.nt > 0) fetch(0, 0);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    // whether some row of the workgroup does not see a tile whole
+    auto partial = [&](int t) {
+        int t0, end;
+        w.tile(t, &t0, &end);
+        return t0 + KT > min(g0.top, end) || (t >= w.n0 && t0 < g1.low);
+    };
+    // this wave's pieces of tile t are there: what is not finite leaves them before the barrier shows them to the others
+    auto clean = [&](int t) {
+        const int buf = t & 1, first = wid * NP * 64 + lane;
+        bool bad = false;
+#pragma unroll
+        for (int j = 0; j < NP; ++j)
+            bad |= take_out<T>(sm + buf * 2 * BUF + BUF + (first + j * 64) * 16, &kinds[buf][first + j * 64]);
+        if (bad) bad_tile[buf] = t;
+    };
+    if (tid < 2) bad_tile[tid] = -1;
+    __syncthreads();
+    if (w.nt > 0) {
+        fetch(0, 0);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (partial(0)) clean(0);
+    }
     __syncthreads();
     for (int t = 0; t < w.nt; ++t) {
         const int buf = t & 1;
@@ -364,18 +420,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_kernel(va_to
             f32x16 sc[KB];
 #pragma unroll
             for (int k = 0; k < KB; ++k) {
-                scores<T, DP>(sc[k], qf, [&](int c) {
-                    const int kr = 32 * k + lc;
-                    return *(const u32x4*)(ks + (kr * CS + ((2 * c + lh) ^ swz<T, CS>(kr))) * 16);
-                });
+                scores<T, DP>(sc[k], qf, [&](int c) { return *(const u32x4*)(ks + ad.k[c] + k * 32 * CS * 16); });
                 __builtin_amdgcn_sched_barrier(0);  // (one block's fragments in registers at a time)
             }
-            if (t0 + KT <= min(f0.top, end) && (sink || t0 >= f1.low)) {  // every row of the wave sees every key
-                softmax<KB, NV>(r, sc, cexp);
-#pragma unroll
-                for (int k = 0; k < KB; ++k) add_values<T, DP>(r, sc[k], vs, 32 * k, lane);
-            } else {
-                const int from = (sink ? 0 : sp.low) - t0, upto = min(sp.top, end) - t0;
+            const int from = (sink ? 0 : sp.low) - t0, upto = min(sp.top, end) - t0;
+            if (t0 + KT > min(f0.top, end) || (!sink && t0 < f1.low)) {  // some row of the wave does not see some key
 #pragma unroll
                 for (int k = 0; k < KB; ++k)
 #pragma unroll
@@ -383,14 +432,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_kernel(va_to
                         const int p = 32 * k + key_of(i, lh);
                         sc[k][i] = p >= from && p < upto ? sc[k][i] : -INFINITY;
                     }
-                softmax<KB, NV>(r, sc, cexp);
-                bool bad = false;
-#pragma unroll
-                for (int k = 0; k < KB; ++k) bad |= add_values<T, DP, true>(r, sc[k], vs, 32 * k, lane);
-                if (__any(bad)) add_nonfinite<T, DP>(r, vs, from, upto, KT, lh);
             }
+            softmax<KB, NV>(r, sc, cexp);
+#pragma unroll
+            for (int k = 0; k < KB; ++k) add_values<T, DP>(r, sc[k], ad, vs, 32 * k, lane);
+            if (bad_tile[buf] == t) add_nonfinite<T, DP>(r, kinds[buf], from, upto, KT, lh);
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (t + 1 < w.nt && partial(t + 1)) clean(t + 1);
         __syncthreads();
     }
     const float total = r.sum + __shfl_xor(r.sum, 32);
@@ -414,6 +463,7 @@ __global__ __launch_bounds__((64 * Dims<T, DP>::SW), 1) void attn_split(va_tok_a
     constexpr int VE = Tr<T>::VE, CS = Dims<T, DP>::CS, NV = DP / 32;
     constexpr int NP = 32 * CS / 64, BUF = 32 * CS * 16, ACC = NV * 16 * 64 * 4, SW = Dims<T, DP>::SW;
     extern __shared__ __align__(16) unsigned char sm[];  // a wave: [2][K | V]; then the waves' registers
+    __shared__ unsigned short kinds[SW][32 * CS];
     __shared__ float sms[2][2][64];
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), lc = lane & 31, lh = lane >> 5;
     const int G = a.Hq / a.Hk;
@@ -437,27 +487,34 @@ __global__ __launch_bounds__((64 * Dims<T, DP>::SW), 1) void attn_split(va_tok_a
     const float cexp = a.scale * 1.4426950408889634f;
     Row<NV> r;
     r.clear();
+    const Addr<T, DP> ad(lane);
     const T* kb = (const T*)a.k + b * a.k_sb + hk * a.k_sh;
     const T* vb = (const T*)a.v + b * a.v_sb + hk * a.v_sh;
-    int ko[NP], vo[NP];  // this lane's DMAs: piece j * 64 + lane of the tile's image
-#pragma unroll
-    for (int j = 0; j < NP; ++j) {
-        const int rr = (j * 64 + lane) / CS, c = (lane % CS) ^ swz<T, CS>(rr);
-        ko[j] = c * VE < a.D ? (int)(rr * a.k_ss + c * VE) * (int)sizeof(T) : TILE_OOB;
-        vo[j] = c * VE < a.Dv ? (int)(rr * a.v_ss + c * VE) * (int)sizeof(T) : TILE_OOB;
-    }
+    constexpr int RS = 64 / CS;
+    const int rr = lane / CS;  // this lane's DMAs: place j * 64 + lane of the tile's image, row rr + j RS
+    const int krow = (int)(rr * a.k_ss) * (int)sizeof(T), vrow = (int)(rr * a.v_ss) * (int)sizeof(T);
     unsigned char* mine = sm + wid * 4 * BUF;
+    const bool whole_d = a.D == DP && a.Dv == DP;
     auto fetch = [&](int t, int buf) {
         int t0, end;
         w.tile(t, &t0, &end);
         const int64_t slot = slot_of(a, t0);
         const T *k = kb + slot * a.k_ss, *v = vb + slot * a.v_ss;
         unsigned char* to = mine + buf * 2 * BUF;
-        const int n = end - t0 - lane / CS;  // rows of the tile from this lane's first on
+        const bool whole = whole_d && t0 + 32 <= end;
 #pragma unroll
-        for (int j = 0; j < NP; ++j) dma16(k, to + j * 1024, j * (64 / CS) < n ? ko[j] : TILE_OOB);
+        for (int j = 0; j < NP; ++j) {
+            const int c = lane % CS ^ swz<T, CS>(rr + j * RS);
+            const bool in = whole || t0 + rr + j * RS < end;
+            dma16(k, to + j * 1024, in && (whole || c * VE < a.D) ? krow + 16 * c : TILE_OOB, j * RS * (int)a.k_ss * (int)sizeof(T));
+        }
 #pragma unroll
-        for (int j = 0; j < NP; ++j) dma16(v, to + BUF + j * 1024, j * (64 / CS) < n ? vo[j] : TILE_OOB);
+        for (int j = 0; j < NP; ++j) {
+            const int c = lane % CS ^ swz<T, CS>(rr + j * RS);
+            const bool in = whole || t0 + rr + j * RS < end;
+            dma16(v, to + BUF + j * 1024, in && (whole || c * VE < a.Dv) ? vrow + 16 * c : TILE_OOB,
+                  j * RS * (int)a.v_ss * (int)sizeof(T));
+        }
     };
     int t = split * per + wid, buf = 0;
     if (t < t1) fetch(t, 0);
@@ -465,22 +522,25 @@ __global__ __launch_bounds__((64 * Dims<T, DP>::SW), 1) void attn_split(va_tok_a
         // this tile is there (the wave's own loads, and its reads of the other buffer are done: their values were used)
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         if (t + SW < t1) fetch(t + SW, buf ^ 1);
-        const unsigned char *ks = mine + buf * 2 * BUF, *vs = ks + BUF;
+        unsigned char *ks = mine + buf * 2 * BUF, *vs = ks + BUF;
         int t0, end;
         w.tile(t, &t0, &end);
-        const bool sink = t < w.n0;
+        const bool sink = t < w.n0, partial = t0 + 32 > min(f0.top, end) || (!sink && t0 < f1.low);  // for some row
+        bool bad = false;
+        if (partial) {
+#pragma unroll
+            for (int j = 0; j < NP; ++j) bad |= take_out<T>(vs + (j * 64 + lane) * 16, &kinds[wid][j * 64 + lane]);
+            bad = __any(bad);
+        }
         f32x16 sc[1];
-        scores<T, DP>(sc[0], qf, [&](int c) { return *(const u32x4*)(ks + (lc * CS + ((2 * c + lh) ^ swz<T, CS>(lc))) * 16); });
-        if (t0 + 32 <= min(f0.top, end) && (sink || t0 >= f1.low)) {  // every row sees every key
-            softmax<1, NV>(r, sc, cexp);
-            add_values<T, DP>(r, sc[0], vs, 0, lane);
-        } else {
-            const int from = (sink ? 0 : sp.low) - t0, upto = min(sp.top, end) - t0;
+        scores<T, DP>(sc[0], qf, [&](int c) { return *(const u32x4*)(ks + ad.k[c]); });
+        const int from = (sink ? 0 : sp.low) - t0, upto = min(sp.top, end) - t0;
+        if (partial)
 #pragma unroll
             for (int i = 0; i < 16; ++i) sc[0][i] = key_of(i, lh) >= from && key_of(i, lh) < upto ? sc[0][i] : -INFINITY;
-            softmax<1, NV>(r, sc, cexp);
-            if (__any(add_values<T, DP, true>(r, sc[0], vs, 0, lane))) add_nonfinite<T, DP>(r, vs, from, upto, 32, lh);
-        }
+        softmax<1, NV>(r, sc, cexp);
+        add_values<T, DP>(r, sc[0], ad, vs, 0, lane);
+        if (bad) add_nonfinite<T, DP>(r, kinds[wid], from, upto, 32, lh);
     }
     // the upper half of the waves into the lower, until one is left
     r.sum += __shfl_xor(r.sum, 32);
