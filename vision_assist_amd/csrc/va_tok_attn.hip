@@ -85,26 +85,53 @@ __device__ __forceinline__ int slot_of(const va_tok_attn_args& a, int p) {
     return a.sinks + (p - a.sinks) % (a.slots - a.sinks);
 }
 
-// sc += K Q^T of 32 keys x 32 rows; kf(c): piece 2 c + lh of this lane's key
-template <typename T, int DP, typename F>
-__device__ __forceinline__ void scores(f32x16& sc, const u32x4 (&qf)[DP / (2 * Tr<T>::VE)], F kf) {
+// sc = K Q^T of KB blocks of 32 keys x 32 rows; kf(k, c): piece 2 c + lh of this lane's key in block k.  bf16: a block's
+// fragments are read beside the MFMAs of the block before.
+template <typename T, int DP, int KB, typename F>
+__device__ __forceinline__ void scores(f32x16 (&sc)[KB], const u32x4 (&qf)[DP / (2 * Tr<T>::VE)], F kf) {
+    constexpr int NF = DP / (2 * Tr<T>::VE);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) sc[i] = 0.0f;
+    for (int k = 0; k < KB; ++k)
 #pragma unroll
-    for (int c = 0; c < DP / (2 * Tr<T>::VE); ++c) {
-        const u32x4 k = kf(c);
-        if constexpr (sizeof(T) == 2) {
-            sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16((bf16x8)k, (bf16x8)qf[c], sc, 0, 0, 0);
-        } else {
+        for (int i = 0; i < 16; ++i) sc[k][i] = 0.0f;
+    if constexpr (sizeof(T) == 2) {
+        u32x4 f[KB][NF];
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                sc = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k[e]), __uint_as_float(qf[c][e]), sc, 0, 0, 0);
+        for (int c = 0; c < NF; ++c) f[0][c] = kf(0, c);
+#pragma unroll
+        for (int k = 0; k < KB; ++k)
+#pragma unroll
+            for (int c = 0; c < NF; ++c) {
+                if (k + 1 < KB) f[k + 1][c] = kf(k + 1, c);
+                sc[k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16((bf16x8)f[k][c], (bf16x8)qf[c], sc[k], 0, 0, 0);
+            }
+        __builtin_amdgcn_sched_group_barrier(0x100, NF, 0);
+#pragma unroll
+        for (int i = 0; i < KB * NF; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            if (i < (KB - 1) * NF) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
+    } else {
+#pragma unroll
+        for (int k = 0; k < KB; ++k)
+#pragma unroll
+            for (int c = 0; c < NF; ++c) {
+                const u32x4 f = kf(k, c);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    sc[k] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(f[e]), __uint_as_float(qf[c][e]), sc[k], 0, 0, 0);
+            }
     }
 }
 
 // the key of register i of a block of 32 scores
 __device__ __forceinline__ int key_of(int i, int lh) { return 8 * (i / 4) + 4 * lh + i % 4; }
+
+// the larger of this lane's value and its partner's (lane ^ 32): the swap of x with itself leaves both lanes' values in both
+__device__ __forceinline__ float pair_max(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
 
 // The running softmax of one row (a lane and its partner lane ^ 32): mx is the reference of the exponents in units of
 // the raw scores, kept while the maximum grows by less than 2^8 in the result (the sums are float, and a probability
@@ -121,6 +148,19 @@ struct Row {
     }
 };
 
+// keys from .. to - 1 of a tile are this row's (the bounds moved by the lane's 4 lh, so that they meet constants)
+template <int KB>
+__device__ __forceinline__ void mask(f32x16 (&sc)[KB], int from, int to, int lh) {
+    from -= 4 * lh, to -= 4 * lh;
+#pragma unroll
+    for (int k = 0; k < KB; ++k)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int p = 32 * k + key_of(i, 0);
+            sc[k][i] = ((from <= p) & (p < to)) ? sc[k][i] : -INFINITY;
+        }
+}
+
 template <int KB, int NV>
 __device__ __forceinline__ void softmax(Row<NV>& r, f32x16 (&sc)[KB], float c) {
     float nm = -INFINITY;
@@ -128,7 +168,7 @@ __device__ __forceinline__ void softmax(Row<NV>& r, f32x16 (&sc)[KB], float c) {
     for (int k = 0; k < KB; ++k)
 #pragma unroll
         for (int i = 0; i < 16; ++i) nm = fmaxf(nm, sc[k][i]);
-    nm = fmaxf(nm, __shfl_xor(nm, 32));
+    nm = pair_max(nm);
     const bool up = nm > r.mx && !((nm - r.mx) * c <= 8.0f);
     if (__any(up)) {  // (each row by its own maximum alone: a row's result does not depend on the others')
         const float alpha = up ? __builtin_amdgcn_exp2f((r.mx - nm) * c) : 1.0f;
@@ -187,34 +227,49 @@ __device__ __forceinline__ u32x4 values_bf16(const Addr<T, DP>& ad, const unsign
     return vf;
 }
 
-// O^T += V^T P^T over 32 keys whose values lie in LDS rows r0 .. r0 + 31 of vs
+// V^T of step st (16 keys) of a tile, block v of columns
 template <typename T, int DP>
-__device__ __forceinline__ void add_values(Row<DP / 32>& r, const f32x16& p, const Addr<T, DP>& ad, const unsigned char* vs, int r0,
-                                           int lane) {
+struct Values {
+    u32x4 f[DP / 32];
+    __device__ __forceinline__ void read(const Addr<T, DP>& ad, const unsigned char* vs, int st) {
+#pragma unroll
+        for (int v = 0; v < DP / 32; ++v) f[v] = values_bf16<T, DP>(ad, vs, 16 * st, v);
+    }
+};
+
+// O^T += V^T P^T over the KB blocks of 32 keys of a tile; bf16: first = step 0's values, read before the softmax, and each
+// step's are read beside the MFMAs of the step before
+template <typename T, int DP, int KB>
+__device__ __forceinline__ void add_values(Row<DP / 32>& r, const f32x16 (&p)[KB], const Values<T, DP>& first, const Addr<T, DP>& ad,
+                                           const unsigned char* vs, int lane) {
     constexpr int CS = Dims<T, DP>::CS, NV = DP / 32;
     if constexpr (sizeof(T) == 2) {
+        Values<T, DP> cur = first, next;
 #pragma unroll
-        for (int c = 0; c < 16; c += 8) {
+        for (int st = 0; st < 2 * KB; ++st) {
+            if (st + 1 < 2 * KB) next.read(ad, vs, st + 1);
             u32x4 pf;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) pf[e] = pk_bf16(p[c + 2 * e], p[c + 2 * e + 1]);
+            for (int e = 0; e < 4; ++e) pf[e] = pk_bf16(p[st / 2][8 * (st & 1) + 2 * e], p[st / 2][8 * (st & 1) + 2 * e + 1]);
 #pragma unroll
             for (int v = 0; v < NV; ++v)
-                r.acc[v] = __builtin_amdgcn_mfma_f32_32x32x16_bf16((bf16x8)values_bf16<T, DP>(ad, vs, r0 + 2 * c, v), (bf16x8)pf,
-                                                                  r.acc[v], 0, 0, 0);
+                r.acc[v] = __builtin_amdgcn_mfma_f32_32x32x16_bf16((bf16x8)cur.f[v], (bf16x8)pf, r.acc[v], 0, 0, 0);
+            cur = next;
         }
     } else {
         const int lc = lane & 31, lh = lane >> 5;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int row = r0 + key_of(i, lh);
+        for (int k = 0; k < KB; ++k)
 #pragma unroll
-            for (int v = 0; v < NV; ++v) {
-                const int d = 32 * v + lc;
-                const float x = *(const float*)(vs + (row * CS + ((d / 4) ^ swz<T, CS>(row))) * 16 + 4 * (d % 4));
-                r.acc[v] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, p[i], r.acc[v], 0, 0, 0);
+            for (int i = 0; i < 16; ++i) {
+                const int row = 32 * k + key_of(i, lh);
+#pragma unroll
+                for (int v = 0; v < NV; ++v) {
+                    const int d = 32 * v + lc;
+                    const float x = *(const float*)(vs + (row * CS + ((d / 4) ^ swz<T, CS>(row))) * 16 + 4 * (d % 4));
+                    r.acc[v] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, p[k][i], r.acc[v], 0, 0, 0);
+                }
             }
-        }
     }
 }
 
@@ -329,8 +384,9 @@ __device__ __forceinline__ void dma16(const void* base, void* lds, int off, int 
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lvoid_t*)lds, 16, off, uniform, 0, 0);
 }
 
+// waves of a SIMD: three where the registers of D <= 64 allow it
 template <typename T, int DP>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_kernel(va_tok_attn_args a, int ntiles) {
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 64 ? 2 : 1)) void attn_kernel(va_tok_attn_args a, int ntiles) {
     constexpr int VE = Tr<T>::VE, KT = Tr<T>::KT, CS = Dims<T, DP>::CS, KB = KT / 32, NV = DP / 32;
     constexpr int NP = KT * CS / 256, BUF = KT * CS * 16;  // DMAs of a wave for K; bytes of a tile of K
     extern __shared__ __align__(16) unsigned char sm[];    // [2][K | V]
@@ -368,21 +424,21 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_kernel(va_to
     constexpr int RS = 64 / CS > 0 ? 64 / CS : 1;
     const int rr = wid * NP * RS + lane / CS;
     const int krow = (int)(rr * a.k_ss) * (int)sizeof(T), vrow = (int)(rr * a.v_ss) * (int)sizeof(T);
-    const bool whole_d = a.D == DP && a.Dv == DP;
     auto fetch = [&](int t, int buf) {
         int t0, end;
         w.tile(t, &t0, &end);
         const int64_t slot = slot_of(a, t0);
         const T *kt = kb + slot * a.k_ss, *vt = vb + slot * a.v_ss;
         unsigned char* ks = sm + buf * 2 * BUF + wid * NP * 1024;
-        const bool whole = whole_d && t0 + KT <= end;  // (uniform) no row and no piece is missing
+        const bool whole = t0 + KT <= end;  // (uniform) no row is missing
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
             const int c = lane % CS ^ swz<T, CS>(rr + j * RS);
-            const bool in = whole || t0 + rr + j * RS < end;
-            dma16(kt, ks + j * 1024, in && (whole || c * VE < a.D) ? krow + 16 * c : TILE_OOB, j * RS * (int)a.k_ss * (int)sizeof(T));
-            dma16(vt, ks + BUF + j * 1024, in && (whole || c * VE < a.Dv) ? vrow + 16 * c : TILE_OOB,
-                  j * RS * (int)a.v_ss * (int)sizeof(T));
+            const int out = whole ? 0 : (int)(t0 + rr + j * RS >= end);  // (no short cuts: a branch would split the DMA)
+            const int ko = (out | (int)(c * VE >= a.D)) ? TILE_OOB : krow + 16 * c;
+            const int vo = (out | (int)(c * VE >= a.Dv)) ? TILE_OOB : vrow + 16 * c;
+            dma16(kt, ks + j * 1024, ko, j * RS * (int)a.k_ss * (int)sizeof(T));
+            dma16(vt, ks + BUF + j * 1024, vo, j * RS * (int)a.v_ss * (int)sizeof(T));
         }
     };
     // whether some row of the workgroup does not see a tile whole
@@ -418,24 +474,13 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_kernel(va_to
         const bool sink = t < w.n0;
         if (!idle && t0 < f1.top && (sink || t0 + KT > f0.low)) {
             f32x16 sc[KB];
-#pragma unroll
-            for (int k = 0; k < KB; ++k) {
-                scores<T, DP>(sc[k], qf, [&](int c) { return *(const u32x4*)(ks + ad.k[c] + k * 32 * CS * 16); });
-                __builtin_amdgcn_sched_barrier(0);  // (one block's fragments in registers at a time)
-            }
+            scores<T, DP, KB>(sc, qf, [&](int k, int c) { return *(const u32x4*)(ks + ad.k[c] + k * 32 * CS * 16); });
+            Values<T, DP> v0;
+            if constexpr (sizeof(T) == 2) v0.read(ad, vs, 0);
             const int from = (sink ? 0 : sp.low) - t0, upto = min(sp.top, end) - t0;
-            if (t0 + KT > min(f0.top, end) || (!sink && t0 < f1.low)) {  // some row of the wave does not see some key
-#pragma unroll
-                for (int k = 0; k < KB; ++k)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int p = 32 * k + key_of(i, lh);
-                        sc[k][i] = p >= from && p < upto ? sc[k][i] : -INFINITY;
-                    }
-            }
+            if (t0 + KT > min(f0.top, end) || (!sink && t0 < f1.low)) mask<KB>(sc, from, upto, lh);  // not all see all
             softmax<KB, NV>(r, sc, cexp);
-#pragma unroll
-            for (int k = 0; k < KB; ++k) add_values<T, DP>(r, sc[k], ad, vs, 32 * k, lane);
+            add_values<T, DP, KB>(r, sc, v0, ad, vs, lane);
             if (bad_tile[buf] == t) add_nonfinite<T, DP>(r, kinds[buf], from, upto, KT, lh);
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -494,26 +539,26 @@ __global__ __launch_bounds__((64 * Dims<T, DP>::SW), 1) void attn_split(va_tok_a
     const int rr = lane / CS;  // this lane's DMAs: place j * 64 + lane of the tile's image, row rr + j RS
     const int krow = (int)(rr * a.k_ss) * (int)sizeof(T), vrow = (int)(rr * a.v_ss) * (int)sizeof(T);
     unsigned char* mine = sm + wid * 4 * BUF;
-    const bool whole_d = a.D == DP && a.Dv == DP;
     auto fetch = [&](int t, int buf) {
         int t0, end;
         w.tile(t, &t0, &end);
         const int64_t slot = slot_of(a, t0);
         const T *k = kb + slot * a.k_ss, *v = vb + slot * a.v_ss;
         unsigned char* to = mine + buf * 2 * BUF;
-        const bool whole = whole_d && t0 + 32 <= end;
+        const bool whole = t0 + 32 <= end;
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
             const int c = lane % CS ^ swz<T, CS>(rr + j * RS);
-            const bool in = whole || t0 + rr + j * RS < end;
-            dma16(k, to + j * 1024, in && (whole || c * VE < a.D) ? krow + 16 * c : TILE_OOB, j * RS * (int)a.k_ss * (int)sizeof(T));
+            const int out = whole ? 0 : (int)(t0 + rr + j * RS >= end);
+            const int off = (out | (int)(c * VE >= a.D)) ? TILE_OOB : krow + 16 * c;
+            dma16(k, to + j * 1024, off, j * RS * (int)a.k_ss * (int)sizeof(T));
         }
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
             const int c = lane % CS ^ swz<T, CS>(rr + j * RS);
-            const bool in = whole || t0 + rr + j * RS < end;
-            dma16(v, to + BUF + j * 1024, in && (whole || c * VE < a.Dv) ? vrow + 16 * c : TILE_OOB,
-                  j * RS * (int)a.v_ss * (int)sizeof(T));
+            const int out = whole ? 0 : (int)(t0 + rr + j * RS >= end);
+            const int off = (out | (int)(c * VE >= a.Dv)) ? TILE_OOB : vrow + 16 * c;
+            dma16(v, to + BUF + j * 1024, off, j * RS * (int)a.v_ss * (int)sizeof(T));
         }
     };
     int t = split * per + wid, buf = 0;
@@ -533,13 +578,13 @@ __global__ __launch_bounds__((64 * Dims<T, DP>::SW), 1) void attn_split(va_tok_a
             bad = __any(bad);
         }
         f32x16 sc[1];
-        scores<T, DP>(sc[0], qf, [&](int c) { return *(const u32x4*)(ks + ad.k[c]); });
+        scores<T, DP, 1>(sc, qf, [&](int, int c) { return *(const u32x4*)(ks + ad.k[c]); });
+        Values<T, DP> v0;
+        if constexpr (sizeof(T) == 2) v0.read(ad, vs, 0);
         const int from = (sink ? 0 : sp.low) - t0, upto = min(sp.top, end) - t0;
-        if (partial)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) sc[0][i] = key_of(i, lh) >= from && key_of(i, lh) < upto ? sc[0][i] : -INFINITY;
+        if (partial) mask<1>(sc, from, upto, lh);
         softmax<1, NV>(r, sc, cexp);
-        add_values<T, DP>(r, sc[0], ad, vs, 0, lane);
+        add_values<T, DP, 1>(r, sc, v0, ad, vs, lane);
         if (bad) add_nonfinite<T, DP>(r, kinds[wid], from, upto, 32, lh);
     }
     // the upper half of the waves into the lower, until one is left
