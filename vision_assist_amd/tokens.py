@@ -103,6 +103,14 @@ def _interleaved(x: torch.Tensor, y: torch.Tensor) -> bool:
     return False
 
 
+def _plain(t: torch.Tensor, item: int) -> tuple:
+    """A 4-d tensor as (address, its strides, the end of its bytes)."""
+    at = t.data_ptr()
+    a, b, c, d = t.stride()
+    n, m, h, w = t.shape
+    return at, a, b, c, d, at + ((n - 1) * a + (m - 1) * b + (h - 1) * c + (w - 1) * d + 1) * item
+
+
 def _meet(x: tuple[int, int], y: tuple[int, int]) -> bool:
     return x[0] < y[1] and y[0] < x[1]
 
@@ -342,7 +350,9 @@ class TokenCache:
         _apart(k, v, "the values")
         self.k, self.v, self.sinks, self.len = k, v, int(sinks), length
         self.slots = k.shape[1]
-        self._k_range, self._v_range = _range(k), _range(v)
+        item = k.element_size()
+        (ka, k0, k1, k2, _, kend), (va, v0, v1, v2, _, vend) = _plain(k, item), _plain(v, item)
+        self._plain = (ka, k0, k1, k2, kend, va, v0, v1, v2, vend)
 
     @classmethod
     def of(cls, k: torch.Tensor, v: torch.Tensor, sinks: int = 0, length: torch.Tensor | None = None) -> "TokenCache":
@@ -381,7 +391,8 @@ class QKNorm:
         self.eps = float(eps)
         self._norm = (self.wq.data_ptr() if self.wq is not None else 0, self.wk.data_ptr() if self.wk is not None else 0,
                       self.eps)
-        self._rot = (0, 0, 0) if rotary is None else (rotary.dim, rotary.turns.data_ptr(), rotary.axis.data_ptr())
+        self._turn = (0, 0, 0) if rotary is None else (rotary.dim, rotary.turns.data_ptr(), rotary.axis.data_ptr())
+        self._rot = (0, 0) if rotary is None else (rotary.axes, LAYOUTS[rotary.layout])
 
     def __call__(self, q: torch.Tensor, k: torch.Tensor, pos: torch.Tensor | None = None,
                  q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None, stream=None):
@@ -390,7 +401,7 @@ class QKNorm:
         q / k themselves."""
         if not _here(self.device, stream):
             return _elsewhere(self.device, stream, (q, k, pos, q_out, k_out), lambda: self(q, k, pos, q_out, k_out))
-        q, k, pos = self._begin(q, k, pos)
+        q, k, pos, turn, B, S, Hq, Hk, item = self._begin(q, k, pos)
         if q_out is None and k_out is None:
             q_out, k_out = q.new_empty(q.shape), k.new_empty(k.shape)
         else:
@@ -398,7 +409,15 @@ class QKNorm:
             _apart(q_out, k, "k")
             _apart(k_out, q, "q")
             _apart(q_out, k_out, "k_out")
-        self._launch(q, k, None, pos, q_out, k_out, None, 0, 0, 0, 0)
+        if B and S:
+            qa, q0, q1, q2 = q.data_ptr(), *q.stride()[:3]
+            ka, k0, k1, k2 = k.data_ptr(), *k.stride()[:3]
+            a = QK_PACK.pack(qa, ka, 0, q_out.data_ptr(), k_out.data_ptr(), 0, q0, q1, q2, k0, k1, k2, 0, 0, 0,
+                             *q_out.stride()[:3], *k_out.stride()[:3], 0, 0, 0, *self._norm, *turn, 0, 0, B, S, Hq, Hk, self.D, 0,
+                             *self._rot, 0, 0, DTYPES[q.dtype], 0)
+            rc = self.lib.va_tok_qk(_raw_stream(self.device.index), a)
+            if rc:
+                _lib.check(rc, "va_tok_qk")
         return q_out, k_out
 
     def store(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor | None, cache: TokenCache,
@@ -409,85 +428,92 @@ class QKNorm:
         if not _here(self.device, stream):
             return _elsewhere(self.device, stream, (q, k, v, pos, q_len, q_out, cache.k, cache.v, cache.len),
                               lambda: self.store(q, k, v, pos, cache, q_len, q_out))
-        q, k, pos = self._begin(q, k, pos)
-        B, S, Hk, D = k.shape
-        ck, cv = cache.k, cache.v
+        q, k, pos, turn, B, S, Hq, Hk, item = self._begin(q, k, pos)
+        Dv = cache.v.shape[3]
         _on(v, self.device, q.dtype, "v")
-        _on(ck, self.device, q.dtype, "the cache")
-        if v.shape != (B, S, Hk, cv.shape[3]):
-            raise _lib.VaError(f"v {tuple(v.shape)}: {(B, S, Hk, cv.shape[3])}")
-        if ck.shape[0] != B or ck.shape[2] != Hk or ck.shape[3] != D:
-            raise _lib.VaError(f"the cache holds {tuple(ck.shape)}")
-        v = v if v.stride(3) == 1 or v.shape[3] == 1 else v.contiguous()
+        _on(cache.k, self.device, q.dtype, "the cache")
+        if v.shape != (B, S, Hk, Dv):
+            raise _lib.VaError(f"v {tuple(v.shape)}: {(B, S, Hk, Dv)}")
+        if cache.k.shape != (B, cache.slots, Hk, self.D):
+            raise _lib.VaError(f"the cache holds {tuple(cache.k.shape)}")
         if q_len is not None:
             _lens(q_len, B, self.device, "q_len")
         if q_out is None:
             q_out = (torch.empty if q_len is None else torch.zeros)(q.shape, dtype=q.dtype, device=self.device)
         else:
             q_out = self._out(q_out, q, "q_out")
-            out = _range(q_out)
-            for t, n in ((k, "k"), (v, "v"), (ck, "the cache's keys"), (cv, "the cache's values")):
-                if _meet(out, _range(t)):
-                    _apart(q_out, t, n)
-        for t, n in ((q, "q"), (k, "k"), (v, "v")):
-            at = _range(t)
-            for c, r in ((ck, cache._k_range), (cv, cache._v_range)):
-                if _meet(r, at):
-                    _apart(c, t, n)
-        self._launch(q, k, v, pos, q_out, ck, cv, 0 if q_len is None else q_len.data_ptr(), cache.len.data_ptr(),
-                     cache.slots, cache.sinks)
+        if not (B and S):
+            return q_out
+        va, v0, v1, v2, v3, vend = _plain(v, item)
+        if v3 != 1 and Dv > 1:
+            v = v.contiguous()
+            va, v0, v1, v2, v3, vend = _plain(v, item)
+        qa, q0, q1, q2, _, qend = _plain(q, item)
+        ka, k0, k1, k2, _, kend = _plain(k, item)
+        oa, o0, o1, o2, _, oend = _plain(q_out, item)
+        c = cache._plain
+        # (cheap first: whether two ranges of bytes meet at all)
+        for n, t, at, end in (("k", k, ka, kend), ("v", v, va, vend)):
+            if oa < end and at < oend:
+                _apart(q_out, t, n)
+        for cn, ct, cat, cend in (("the cache's keys", cache.k, c[0], c[4]), ("the cache's values", cache.v, c[5], c[9])):
+            if oa < cend and cat < oend:
+                _apart(q_out, ct, cn)
+            for n, t, at, end in (("q", q, qa, qend), ("k", k, ka, kend), ("v", v, va, vend)):
+                if at < cend and cat < end:
+                    _apart(ct, t, n)
+        a = QK_PACK.pack(qa, ka, va, oa, c[0], c[5], q0, q1, q2, k0, k1, k2, v0, v1, v2, o0, o1, o2, *c[1:4], *c[6:9],
+                         *self._norm, *turn, 0 if q_len is None else q_len.data_ptr(), cache.len.data_ptr(), B, S, Hq, Hk, self.D, Dv,
+                         *self._rot, cache.slots, cache.sinks, DTYPES[q.dtype], 0)
+        rc = self.lib.va_tok_qk(_raw_stream(self.device.index), a)
+        if rc:
+            _lib.check(rc, "va_tok_qk")
         return q_out
 
     def _begin(self, q, k, pos):
-        if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != self.D or k.shape[3] != self.D:
+        """Checks -> q, k with contiguous values, pos, (rot, turns, axis, pos, its strides), the sizes."""
+        if q.dim() != 4 or k.dim() != 4:
             raise _lib.VaError(f"q {tuple(q.shape)}, k {tuple(k.shape)}: [B, S, heads, {self.D}]")
-        if q.dtype not in DTYPES:
-            raise _lib.VaError(f"q is {q.dtype}: bfloat16 or float32")
-        _on(q, self.device, q.dtype, "q")
-        _on(k, self.device, q.dtype, "k")
-        if max(q.shape) > I32_MAX or max(q.shape[2], k.shape[2]) > 1 << 20:
+        B, S, Hq, D = q.shape
+        Bk, Sk, Hk, Dk = k.shape
+        if Bk != B or Sk != S or D != self.D or Dk != D:
+            raise _lib.VaError(f"q {tuple(q.shape)}, k {tuple(k.shape)}: [B, S, heads, {self.D}]")
+        dtype = q.dtype
+        if dtype not in DTYPES:
+            raise _lib.VaError(f"q is {dtype}: bfloat16 or float32")
+        _on(q, self.device, dtype, "q")
+        _on(k, self.device, dtype, "k")
+        if B > I32_MAX or S > I32_MAX or Hq > 1 << 20 or Hk > 1 << 20:
             raise _lib.VaError("a side beyond what the kernel counts")
-        if self.D > 1:
+        if D > 1:
             q = q if q.stride(3) == 1 else q.contiguous()
             k = k if k.stride(3) == 1 else k.contiguous()
-        if self.rotary is None:
+        rotary = self.rotary
+        if rotary is None:
             _need(pos is None, "pos: there is no rotation")
-            return q, k, None
+            return q, k, None, (0, 0, 0, 0, 0, 0), B, S, Hq, Hk, q.element_size()
         if pos is None:
             raise _lib.VaError("pos: a rotation needs positions")
         _on(pos, self.device, torch.int32, "pos")
-        n = self.rotary.axes
-        pos = pos.unsqueeze(-1) if pos.dim() == 2 and n == 1 else pos
-        if pos.shape != (q.shape[0], q.shape[1], n):
-            raise _lib.VaError(f"pos {tuple(pos.shape)}: {(q.shape[0], q.shape[1], n)}")
-        return q, k, pos if n == 1 or pos.stride(2) == 1 else pos.contiguous()
+        n = rotary.axes
+        pos = pos.unsqueeze(-1) if n == 1 and pos.dim() == 2 else pos
+        if pos.shape != (B, S, n):
+            raise _lib.VaError(f"pos {tuple(pos.shape)}: {(B, S, n)}")
+        a, b, c = pos.stride()
+        if n > 1 and c != 1:
+            pos = pos.contiguous()
+            a, b, c = pos.stride()
+        return q, k, pos, (*self._turn, pos.data_ptr(), a, b), B, S, Hq, Hk, q.element_size()
 
     def _out(self, t, like, name):
         if t is None:
             return like.new_empty(like.shape)
         _on(t, self.device, like.dtype, name)
-        _need(t.shape == like.shape and (t.stride(3) == 1 or self.D == 1),
-              f"{name} {tuple(t.shape)}: {tuple(like.shape)} with contiguous values")
+        if t.shape != like.shape or (t.stride(3) != 1 and self.D > 1):
+            raise _lib.VaError(f"{name} {tuple(t.shape)}: {tuple(like.shape)} with contiguous values")
         _own_elements(t)
         _apart(t, like, "its input", same_ok=True)
         return t
-
-    def _launch(self, q, k, v, pos, q_out, k_out, v_out, q_len, kv_len, slots, sinks):
-        B, S, Hq, D = q.shape
-        if B * S == 0:
-            return
-        rot, turns, axis = self._rot
-        none = (0, 0, 0)
-        a = QK_PACK.pack(
-            q.data_ptr(), k.data_ptr(), 0 if v is None else v.data_ptr(), q_out.data_ptr(), k_out.data_ptr(),
-            0 if v is None else v_out.data_ptr(), *q.stride()[:3], *k.stride()[:3], *(none if v is None else v.stride()[:3]),
-            *q_out.stride()[:3], *k_out.stride()[:3], *(none if v is None else v_out.stride()[:3]), *self._norm, rot, turns, axis,
-            *((0, 0, 0) if pos is None else (pos.data_ptr(), pos.stride(0), pos.stride(1))), q_len, kv_len, B, S, Hq, k.shape[2],
-            D, 0 if v is None else v.shape[3], 0 if pos is None else pos.shape[2],
-            0 if self.rotary is None else LAYOUTS[self.rotary.layout], slots, sinks, DTYPES[q.dtype], 0)
-        rc = self.lib.va_tok_qk(_raw_stream(self.device.index), a)
-        if rc:
-            _lib.check(rc, "va_tok_qk")
 
 
 # ------------------------------------------------------------------ attention
@@ -500,7 +526,8 @@ def _lens(t, B, dev, name):
 def _aligned(t: torch.Tensor) -> torch.Tensor:
     """t, or a copy of it, with contiguous values and every row 16-byte aligned."""
     a, b, c, d = t.stride()
-    return t if d == 1 and not (a | b | c) % 8 and not t.data_ptr() & 15 else t.clone(memory_format=torch.contiguous_format)
+    fine = d == 1 and not (a | b | c) % 8 and not t.data_ptr() & 15 and b < 1 << 22
+    return t if fine else t.clone(memory_format=torch.contiguous_format)
 
 
 def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float | None = None, frame: int = 1,
@@ -564,12 +591,12 @@ def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float | 
                 _apart(out, t, n)
     if B == 0 or S == 0:
         return out
-    q, k, v = _aligned(q), _aligned(k), _aligned(v)
-    o = _aligned(out)
+    q, k, v, o = _aligned(q), _aligned(k), _aligned(v), _aligned(out)
     lib = _lib.load()
-    ints = (B, S, Hq, Hk, D, Dv, slots, frame, window, sinks, DTYPES[dtype])
-    most = (q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
-            *o.stride()[:3], 0 if q_len is None else q_len.data_ptr(), 0 if kv_len is None else kv_len.data_ptr(), scale, *ints)
+    (q0, q1, q2, _), (k0, k1, k2, _), (v0, v1, v2, _), (o0, o1, o2, _) = q.stride(), k.stride(), v.stride(), o.stride()
+    most = (q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), q0, q1, q2, k0, k1, k2, v0, v1, v2, o0, o1, o2,
+            0 if q_len is None else q_len.data_ptr(), 0 if kv_len is None else kv_len.data_ptr(), scale, B, S, Hq, Hk, D, Dv,
+            slots, frame, window, sinks, DTYPES[dtype])
     a = ATTN_PACK.pack(*most, 0, 0)
     n = lib.va_tok_attn_workspace_bytes(a)
     if n:
