@@ -57,14 +57,16 @@ struct Tr<float> {
     static constexpr int VE = 4;
     static constexpr int KT = 32;
 };
-template <typename T, int DP>
+// rows of D values (a multiple of 32) as they are staged: NC pieces, laid out as CS (a power of two)
+template <typename T, int D>
 struct Dims {
-    static constexpr int VE = Tr<T>::VE, NC = DP / VE;                      // pieces of a row
-    static constexpr int CS = NC <= 4 ? 4 : NC <= 8 ? 8 : NC <= 16 ? 16 : 32;  // ... as laid out in LDS
-    static constexpr int NV = DP / 32;
-    // attn_split: waves of a workgroup (two buffers of K and V tiles each within the LDS), and its bytes
-    static constexpr int SW = CS == 32 ? 2 : 4, SLDS = SW * 4 * 32 * CS * 16;
-    static_assert(SLDS <= 128 * 1024 && SW / 2 * NV * 16 * 64 * 4 <= SLDS, "");
+    static constexpr int NC = D / Tr<T>::VE, CS = NC <= 4 ? 4 : NC <= 8 ? 8 : NC <= 16 ? 16 : 32;
+};
+// attn_split: waves of a workgroup (two buffers of K and V tiles each within the LDS), and its bytes
+template <typename T, int DQ, int DV>
+struct Split {
+    static constexpr int CK = Dims<T, DQ>::CS, CV = Dims<T, DV>::CS, SW = CK + CV > 32 ? 2 : 4, LDS = SW * 2 * 32 * (CK + CV) * 16;
+    static_assert(LDS <= 128 * 1024 && SW / 2 * (DV / 32) * 16 * 64 * 4 <= LDS, "");
 };
 
 // LDS image of a tile: rows of CS 16-byte pieces, piece c of row r in place c ^ swz(r), so that the lanes that a read
@@ -87,9 +89,9 @@ __device__ __forceinline__ int slot_of(const va_tok_attn_args& a, int p) {
 
 // sc = K Q^T of KB blocks of 32 keys x 32 rows; kf(k, c): piece 2 c + lh of this lane's key in block k.  bf16: a block's
 // fragments are read beside the MFMAs of the block before.
-template <typename T, int DP, int KB, typename F>
-__device__ __forceinline__ void scores(f32x16 (&sc)[KB], const u32x4 (&qf)[DP / (2 * Tr<T>::VE)], F kf) {
-    constexpr int NF = DP / (2 * Tr<T>::VE);
+template <typename T, int DQ, int KB, typename F>
+__device__ __forceinline__ void scores(f32x16 (&sc)[KB], const u32x4 (&qf)[DQ / (2 * Tr<T>::VE)], F kf) {
+    constexpr int NF = DQ / (2 * Tr<T>::VE);
 #pragma unroll
     for (int k = 0; k < KB; ++k)
 #pragma unroll
@@ -194,32 +196,32 @@ __device__ __forceinline__ void softmax(Row<NV>& r, f32x16 (&sc)[KB], float c) {
 // This lane's LDS addresses in a tile's image, formed once: K of row lane & 31, piece 2 c + lh; V for the reads of block v.
 // bf16: 16 lanes read 4 keys of 16 columns (rows 4 lh + 0 .. 3 of the 8-key group u, columns 32 v + 16 (lane / 16 % 2) ..)
 // and lane q of them gets column q's 4 keys.  Later keys of a tile are a constant away (32 rows' swizzles are 0 .. 31's).
-template <typename T, int DP>
+template <typename T, int DQ, int DV>
 struct Addr {
-    static constexpr int CS = Dims<T, DP>::CS, NV = DP / 32, NF = DP / (2 * Tr<T>::VE), U = sizeof(T) == 2 ? 2 : 1;
+    static constexpr int CK = Dims<T, DQ>::CS, CV = Dims<T, DV>::CS, NV = DV / 32, NF = DQ / (2 * Tr<T>::VE), U = sizeof(T) == 2 ? 2 : 1;
     int k[NF], v[U][NV];
     __device__ __forceinline__ Addr(int lane) {
         const int lc = lane & 31, lh = lane >> 5, q = lane & 15, ch = (lane >> 4) & 1;
 #pragma unroll
-        for (int c = 0; c < NF; ++c) k[c] = (lc * CS + ((2 * c + lh) ^ swz<T, CS>(lc))) * 16;
+        for (int c = 0; c < NF; ++c) k[c] = (lc * CK + ((2 * c + lh) ^ swz<T, CK>(lc))) * 16;
         if constexpr (sizeof(T) == 2) {
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
                     const int row = 8 * u + 4 * lh + (q >> 2), pc = 4 * i + 2 * ch + ((q & 3) >> 1);
-                    v[u][i] = (row * CS + (pc ^ swz<T, CS>(row))) * 16 + 8 * (q & 1);
+                    v[u][i] = (row * CV + (pc ^ swz<T, CV>(row))) * 16 + 8 * (q & 1);
                 }
         }
     }
 };
 
-template <typename T, int DP>
-__device__ __forceinline__ u32x4 values_bf16(const Addr<T, DP>& ad, const unsigned char* vs, int row0, int v) {
+template <typename T, int DQ, int DV>
+__device__ __forceinline__ u32x4 values_bf16(const Addr<T, DQ, DV>& ad, const unsigned char* vs, int row0, int v) {
     u32x4 vf;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-        const unsigned char* at = vs + ad.v[u][v] + row0 * (Dims<T, DP>::CS * 16);
+        const unsigned char* at = vs + ad.v[u][v] + row0 * (Dims<T, DV>::CS * 16);
         const u32x2 t = __builtin_bit_cast(
             u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at));
         vf[2 * u] = t[0], vf[2 * u + 1] = t[1];
@@ -228,23 +230,23 @@ __device__ __forceinline__ u32x4 values_bf16(const Addr<T, DP>& ad, const unsign
 }
 
 // V^T of step st (16 keys) of a tile, block v of columns
-template <typename T, int DP>
+template <typename T, int DQ, int DV>
 struct Values {
-    u32x4 f[DP / 32];
-    __device__ __forceinline__ void read(const Addr<T, DP>& ad, const unsigned char* vs, int st) {
+    u32x4 f[DV / 32];
+    __device__ __forceinline__ void read(const Addr<T, DQ, DV>& ad, const unsigned char* vs, int st) {
 #pragma unroll
-        for (int v = 0; v < DP / 32; ++v) f[v] = values_bf16<T, DP>(ad, vs, 16 * st, v);
+        for (int v = 0; v < DV / 32; ++v) f[v] = values_bf16<T, DQ, DV>(ad, vs, 16 * st, v);
     }
 };
 
 // O^T += V^T P^T over the KB blocks of 32 keys of a tile; bf16: first = step 0's values, read before the softmax, and each
 // step's are read beside the MFMAs of the step before
-template <typename T, int DP, int KB>
-__device__ __forceinline__ void add_values(Row<DP / 32>& r, const f32x16 (&p)[KB], const Values<T, DP>& first, const Addr<T, DP>& ad,
-                                           const unsigned char* vs, int lane) {
-    constexpr int CS = Dims<T, DP>::CS, NV = DP / 32;
+template <typename T, int DQ, int DV, int KB>
+__device__ __forceinline__ void add_values(Row<DV / 32>& r, const f32x16 (&p)[KB], const Values<T, DQ, DV>& first,
+                                           const Addr<T, DQ, DV>& ad, const unsigned char* vs, int lane) {
+    constexpr int CS = Dims<T, DV>::CS, NV = DV / 32;
     if constexpr (sizeof(T) == 2) {
-        Values<T, DP> cur = first, next;
+        Values<T, DQ, DV> cur = first, next;
 #pragma unroll
         for (int st = 0; st < 2 * KB; ++st) {
             if (st + 1 < 2 * KB) next.read(ad, vs, st + 1);
@@ -303,9 +305,9 @@ __device__ __forceinline__ bool take_out(unsigned char* piece, unsigned short* k
 }
 
 // ... positions from .. to - 1 of the tile's n keys are seen
-template <typename T, int DP>
-__device__ __forceinline__ void add_nonfinite(Row<DP / 32>& r, const unsigned short* kinds, int from, int to, int n, int lh) {
-    constexpr int CS = Dims<T, DP>::CS, NV = DP / 32, VE = Tr<T>::VE;
+template <typename T, int DV>
+__device__ __forceinline__ void add_nonfinite(Row<DV / 32>& r, const unsigned short* kinds, int from, int to, int n, int lh) {
+    constexpr int CS = Dims<T, DV>::CS, NV = DV / 32, VE = Tr<T>::VE;
 #pragma unroll 1
     for (int k = max(from, 0); k < min(to, n); ++k) {
 #pragma unroll
@@ -338,12 +340,12 @@ __device__ __forceinline__ void store_block(T* op, const f32x16& x, float by, in
     }
 }
 
-template <typename T, int DP>
+template <typename T, int DQ>
 __device__ __forceinline__ void load_q(const va_tok_attn_args& a, const T* qp, bool there, int lh,
-                                       u32x4 (&qf)[DP / (2 * Tr<T>::VE)]) {
+                                       u32x4 (&qf)[DQ / (2 * Tr<T>::VE)]) {
     constexpr int VE = Tr<T>::VE;
 #pragma unroll
-    for (int c = 0; c < DP / (2 * VE); ++c) {
+    for (int c = 0; c < DQ / (2 * VE); ++c) {
         const int d = (2 * c + lh) * VE;
         qf[c] = there && d < a.D ? *(const u32x4*)(qp + d) : (u32x4){0, 0, 0, 0};
     }
@@ -385,12 +387,13 @@ __device__ __forceinline__ void dma16(const void* base, void* lds, int off, int 
 }
 
 // waves of a SIMD: three where the registers of D <= 64 allow it
-template <typename T, int DP>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 64 ? 2 : 1)) void attn_kernel(va_tok_attn_args a, int ntiles) {
-    constexpr int VE = Tr<T>::VE, KT = Tr<T>::KT, CS = Dims<T, DP>::CS, KB = KT / 32, NV = DP / 32;
-    constexpr int NP = KT * CS / 256, BUF = KT * CS * 16;  // DMAs of a wave for K; bytes of a tile of K
+template <typename T, int DQ, int DV>
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? (DV <= 64 ? 3 : 2) : (DV <= 64 ? 2 : 1)) void attn_kernel(va_tok_attn_args a, int ntiles) {
+    constexpr int VE = Tr<T>::VE, KT = Tr<T>::KT, CK = Dims<T, DQ>::CS, CV = Dims<T, DV>::CS, KB = KT / 32, NV = DV / 32;
+    constexpr int NK = KT * CK / 256, NP = KT * CV / 256;             // DMAs of a wave for K, for V
+    constexpr int KBUF = KT * CK * 16, BUF = KBUF + KT * CV * 16;      // bytes of a tile of K, of both
     extern __shared__ __align__(16) unsigned char sm[];    // [2][K | V]
-    __shared__ unsigned short kinds[2][KT * CS];
+    __shared__ unsigned short kinds[2][KT * CV];
     __shared__ int bad_tile[2];  // the tile of a buffer, if values were taken out of it
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), lc = lane & 31, lh = lane >> 5;
     const int G = a.Hq / a.Hk;
@@ -411,34 +414,38 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 6
     const Span f1 = attn_span(a, sq, sq.first + min(r0 + 32 * wid + 31, rows - 1) / G);
     const bool idle = r0 + 32 * wid >= rows;
 
-    u32x4 qf[DP / (2 * VE)];
-    load_q<T, DP>(a, (const T*)a.q + b * a.q_sb + s * a.q_ss + (int64_t)(hk * G + g) * a.q_sh, there, lh, qf);
+    u32x4 qf[DQ / (2 * VE)];
+    load_q<T, DQ>(a, (const T*)a.q + b * a.q_sb + s * a.q_ss + (int64_t)(hk * G + g) * a.q_sh, there, lh, qf);
     const float cexp = a.scale * 1.4426950408889634f;
     Row<NV> r;
     r.clear();
-    const Addr<T, DP> ad(lane);
+    const Addr<T, DQ, DV> ad(lane);
 
     const T* kb = (const T*)a.k + b * a.k_sb + hk * a.k_sh;
     const T* vb = (const T*)a.v + b * a.v_sb + hk * a.v_sh;
-    // this lane's DMAs: place i = (wid * NP + j) * 64 + lane of the tile's image, row i / CS = r_0 + j RS, piece i % CS ^ swz
-    constexpr int RS = 64 / CS > 0 ? 64 / CS : 1;
-    const int rr = wid * NP * RS + lane / CS;
-    const int krow = (int)(rr * a.k_ss) * (int)sizeof(T), vrow = (int)(rr * a.v_ss) * (int)sizeof(T);
+    // this lane's DMAs: place i = (wid * N + j) * 64 + lane of an operand's image, row i / CS = r_0 + j 64 / CS, piece i % CS ^ swz
+    const int kr = wid * NK * (64 / CK) + lane / CK, vr = wid * NP * (64 / CV) + lane / CV;
+    const int krow = (int)(kr * a.k_ss) * (int)sizeof(T), vrow = (int)(vr * a.v_ss) * (int)sizeof(T);
     auto fetch = [&](int t, int buf) {
         int t0, end;
         w.tile(t, &t0, &end);
         const int64_t slot = slot_of(a, t0);
         const T *kt = kb + slot * a.k_ss, *vt = vb + slot * a.v_ss;
-        unsigned char* ks = sm + buf * 2 * BUF + wid * NP * 1024;
+        unsigned char *ks = sm + buf * BUF + wid * NK * 1024, *vs = sm + buf * BUF + KBUF + wid * NP * 1024;
         const bool whole = t0 + KT <= end;  // (uniform) no row is missing
 #pragma unroll
+        for (int j = 0; j < NK; ++j) {
+            const int rj = kr + j * (64 / CK), c = lane % CK ^ swz<T, CK>(rj);
+            const int out = whole ? 0 : (int)(t0 + rj >= end);  // (no short cuts: a branch would split the DMA)
+            dma16(kt, ks + j * 1024, (out | (int)(c * VE >= a.D)) ? TILE_OOB : krow + 16 * c,
+                  j * (64 / CK) * (int)a.k_ss * (int)sizeof(T));
+        }
+#pragma unroll
         for (int j = 0; j < NP; ++j) {
-            const int c = lane % CS ^ swz<T, CS>(rr + j * RS);
-            const int out = whole ? 0 : (int)(t0 + rr + j * RS >= end);  // (no short cuts: a branch would split the DMA)
-            const int ko = (out | (int)(c * VE >= a.D)) ? TILE_OOB : krow + 16 * c;
-            const int vo = (out | (int)(c * VE >= a.Dv)) ? TILE_OOB : vrow + 16 * c;
-            dma16(kt, ks + j * 1024, ko, j * RS * (int)a.k_ss * (int)sizeof(T));
-            dma16(vt, ks + BUF + j * 1024, vo, j * RS * (int)a.v_ss * (int)sizeof(T));
+            const int rj = vr + j * (64 / CV), c = lane % CV ^ swz<T, CV>(rj);
+            const int out = whole ? 0 : (int)(t0 + rj >= end);
+            dma16(vt, vs + j * 1024, (out | (int)(c * VE >= a.Dv)) ? TILE_OOB : vrow + 16 * c,
+                  j * (64 / CV) * (int)a.v_ss * (int)sizeof(T));
         }
     };
     // whether some row of the workgroup does not see a tile whole
@@ -453,7 +460,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 6
         bool bad = false;
 #pragma unroll
         for (int j = 0; j < NP; ++j)
-            bad |= take_out<T>(sm + buf * 2 * BUF + BUF + (first + j * 64) * 16, &kinds[buf][first + j * 64]);
+            bad |= take_out<T>(sm + buf * BUF + KBUF + (first + j * 64) * 16, &kinds[buf][first + j * 64]);
         if (bad) bad_tile[buf] = t;
     };
     if (tid < 2) bad_tile[tid] = -1;
@@ -467,21 +474,20 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 6
     for (int t = 0; t < w.nt; ++t) {
         const int buf = t & 1;
         if (t + 1 < w.nt) fetch(t + 1, buf ^ 1);
-        const unsigned char* ks = sm + buf * 2 * BUF;
-        const unsigned char* vs = ks + BUF;
+        const unsigned char *ks = sm + buf * BUF, *vs = ks + KBUF;
         int t0, end;
         w.tile(t, &t0, &end);
         const bool sink = t < w.n0;
         if (!idle && t0 < f1.top && (sink || t0 + KT > f0.low)) {
             f32x16 sc[KB];
-            scores<T, DP, KB>(sc, qf, [&](int k, int c) { return *(const u32x4*)(ks + ad.k[c] + k * 32 * CS * 16); });
-            Values<T, DP> v0;
+            scores<T, DQ, KB>(sc, qf, [&](int k, int c) { return *(const u32x4*)(ks + ad.k[c] + k * 32 * CK * 16); });
+            Values<T, DQ, DV> v0;
             if constexpr (sizeof(T) == 2) v0.read(ad, vs, 0);
             const int from = (sink ? 0 : sp.low) - t0, upto = min(sp.top, end) - t0;
             if (t0 + KT > min(f0.top, end) || (!sink && t0 < f1.low)) mask<KB>(sc, from, upto, lh);  // not all see all
             softmax<KB, NV>(r, sc, cexp);
-            add_values<T, DP, KB>(r, sc, v0, ad, vs, lane);
-            if (bad_tile[buf] == t) add_nonfinite<T, DP>(r, kinds[buf], from, upto, KT, lh);
+            add_values<T, DQ, DV, KB>(r, sc, v0, ad, vs, lane);
+            if (bad_tile[buf] == t) add_nonfinite<T, DV>(r, kinds[buf], from, upto, KT, lh);
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         if (t + 1 < w.nt && partial(t + 1)) clean(t + 1);
@@ -503,12 +509,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 6
 // A share's result: [NV * 16][64] registers as they lie in the wave, then the 32 rows' maxima and sums.
 __device__ __forceinline__ int64_t part_floats(int NV) { return NV * 16 * 64 + 64; }
 
-template <typename T, int DP>
-__global__ __launch_bounds__((64 * Dims<T, DP>::SW), 1) void attn_split(va_tok_attn_args a, int nrb, int nsplit) {
-    constexpr int VE = Tr<T>::VE, CS = Dims<T, DP>::CS, NV = DP / 32;
-    constexpr int NP = 32 * CS / 64, BUF = 32 * CS * 16, ACC = NV * 16 * 64 * 4, SW = Dims<T, DP>::SW;
+template <typename T, int DQ, int DV>
+__global__ __launch_bounds__((64 * Split<T, DQ, DV>::SW), 1) void attn_split(va_tok_attn_args a, int nrb, int nsplit) {
+    constexpr int VE = Tr<T>::VE, CK = Dims<T, DQ>::CS, CV = Dims<T, DV>::CS, NV = DV / 32, SW = Split<T, DQ, DV>::SW;
+    constexpr int NK = 32 * CK / 64, NP = 32 * CV / 64, KBUF = 32 * CK * 16, BUF = KBUF + 32 * CV * 16, ACC = NV * 16 * 64 * 4;
     extern __shared__ __align__(16) unsigned char sm[];  // a wave: [2][K | V]; then the waves' registers
-    __shared__ unsigned short kinds[SW][32 * CS];
+    __shared__ unsigned short kinds[SW][32 * CV];
     __shared__ float sms[2][2][64];
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), lc = lane & 31, lh = lane >> 5;
     const int G = a.Hq / a.Hk;
@@ -527,38 +533,37 @@ __global__ __launch_bounds__((64 * Dims<T, DP>::SW), 1) void attn_split(va_tok_a
     const Walk<32> w(a, attn_span(a, sq, max(sq.first + r0 / G, 0)), f1);
     const int per = (w.nt + nsplit - 1) / nsplit, t1 = min((split + 1) * per, w.nt);
 
-    u32x4 qf[DP / (2 * VE)];
-    load_q<T, DP>(a, (const T*)a.q + b * a.q_sb + s * a.q_ss + (int64_t)(hk * G + g) * a.q_sh, there, lh, qf);
+    u32x4 qf[DQ / (2 * VE)];
+    load_q<T, DQ>(a, (const T*)a.q + b * a.q_sb + s * a.q_ss + (int64_t)(hk * G + g) * a.q_sh, there, lh, qf);
     const float cexp = a.scale * 1.4426950408889634f;
     Row<NV> r;
     r.clear();
-    const Addr<T, DP> ad(lane);
+    const Addr<T, DQ, DV> ad(lane);
     const T* kb = (const T*)a.k + b * a.k_sb + hk * a.k_sh;
     const T* vb = (const T*)a.v + b * a.v_sb + hk * a.v_sh;
-    constexpr int RS = 64 / CS;
-    const int rr = lane / CS;  // this lane's DMAs: place j * 64 + lane of the tile's image, row rr + j RS
-    const int krow = (int)(rr * a.k_ss) * (int)sizeof(T), vrow = (int)(rr * a.v_ss) * (int)sizeof(T);
-    unsigned char* mine = sm + wid * 4 * BUF;
+    // this lane's DMAs: place j * 64 + lane of an operand's image, row lane / CS + j 64 / CS
+    const int kr = lane / CK, vr = lane / CV;
+    const int krow = (int)(kr * a.k_ss) * (int)sizeof(T), vrow = (int)(vr * a.v_ss) * (int)sizeof(T);
+    unsigned char* mine = sm + wid * 2 * BUF;
     auto fetch = [&](int t, int buf) {
         int t0, end;
         w.tile(t, &t0, &end);
         const int64_t slot = slot_of(a, t0);
         const T *k = kb + slot * a.k_ss, *v = vb + slot * a.v_ss;
-        unsigned char* to = mine + buf * 2 * BUF;
+        unsigned char* to = mine + buf * BUF;
         const bool whole = t0 + 32 <= end;
 #pragma unroll
-        for (int j = 0; j < NP; ++j) {
-            const int c = lane % CS ^ swz<T, CS>(rr + j * RS);
-            const int out = whole ? 0 : (int)(t0 + rr + j * RS >= end);
-            const int off = (out | (int)(c * VE >= a.D)) ? TILE_OOB : krow + 16 * c;
-            dma16(k, to + j * 1024, off, j * RS * (int)a.k_ss * (int)sizeof(T));
+        for (int j = 0; j < NK; ++j) {
+            const int rj = kr + j * (64 / CK), c = lane % CK ^ swz<T, CK>(rj);
+            const int out = whole ? 0 : (int)(t0 + rj >= end);
+            dma16(k, to + j * 1024, (out | (int)(c * VE >= a.D)) ? TILE_OOB : krow + 16 * c, j * (64 / CK) * (int)a.k_ss * (int)sizeof(T));
         }
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
-            const int c = lane % CS ^ swz<T, CS>(rr + j * RS);
-            const int out = whole ? 0 : (int)(t0 + rr + j * RS >= end);
-            const int off = (out | (int)(c * VE >= a.Dv)) ? TILE_OOB : vrow + 16 * c;
-            dma16(v, to + BUF + j * 1024, off, j * RS * (int)a.v_ss * (int)sizeof(T));
+            const int rj = vr + j * (64 / CV), c = lane % CV ^ swz<T, CV>(rj);
+            const int out = whole ? 0 : (int)(t0 + rj >= end);
+            dma16(v, to + KBUF + j * 1024, (out | (int)(c * VE >= a.Dv)) ? TILE_OOB : vrow + 16 * c,
+                  j * (64 / CV) * (int)a.v_ss * (int)sizeof(T));
         }
     };
     int t = split * per + wid, buf = 0;
@@ -567,7 +572,7 @@ __global__ __launch_bounds__((64 * Dims<T, DP>::SW), 1) void attn_split(va_tok_a
         // this tile is there (the wave's own loads, and its reads of the other buffer are done: their values were used)
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         if (t + SW < t1) fetch(t + SW, buf ^ 1);
-        unsigned char *ks = mine + buf * 2 * BUF, *vs = ks + BUF;
+        unsigned char *ks = mine + buf * BUF, *vs = ks + KBUF;
         int t0, end;
         w.tile(t, &t0, &end);
         const bool sink = t < w.n0, partial = t0 + 32 > min(f0.top, end) || (!sink && t0 < f1.low);  // for some row
@@ -578,14 +583,14 @@ __global__ __launch_bounds__((64 * Dims<T, DP>::SW), 1) void attn_split(va_tok_a
             bad = __any(bad);
         }
         f32x16 sc[1];
-        scores<T, DP, 1>(sc, qf, [&](int, int c) { return *(const u32x4*)(ks + ad.k[c]); });
-        Values<T, DP> v0;
+        scores<T, DQ, 1>(sc, qf, [&](int, int c) { return *(const u32x4*)(ks + ad.k[c]); });
+        Values<T, DQ, DV> v0;
         if constexpr (sizeof(T) == 2) v0.read(ad, vs, 0);
         const int from = (sink ? 0 : sp.low) - t0, upto = min(sp.top, end) - t0;
         if (partial) mask<1>(sc, from, upto, lh);
         softmax<1, NV>(r, sc, cexp);
-        add_values<T, DP, 1>(r, sc, v0, ad, vs, lane);
-        if (bad) add_nonfinite<T, DP>(r, kinds[wid], from, upto, 32, lh);
+        add_values<T, DQ, DV, 1>(r, sc, v0, ad, vs, lane);
+        if (bad) add_nonfinite<T, DV>(r, kinds[wid], from, upto, 32, lh);
     }
     // the upper half of the waves into the lower, until one is left
     r.sum += __shfl_xor(r.sum, 32);
@@ -636,9 +641,9 @@ __global__ __launch_bounds__((64 * Dims<T, DP>::SW), 1) void attn_split(va_tok_a
 }
 
 // the shares of 32 rows, in their order: a wave per block of 32 columns
-template <typename T, int DP>
-__global__ __launch_bounds__(64 * (DP / 32)) void attn_join(va_tok_attn_args a, int nrb, int nsplit) {
-    constexpr int NV = DP / 32;
+template <typename T, int DV>
+__global__ __launch_bounds__(64 * (DV / 32)) void attn_join(va_tok_attn_args a, int nrb, int nsplit) {
+    constexpr int NV = DV / 32;
     const int lane = threadIdx.x & 63, v = threadIdx.x >> 6, lc = lane & 31, lh = lane >> 5, G = a.Hq / a.Hk;
     const int rb = blockIdx.x % nrb, unit = blockIdx.x / nrb, hk = unit % a.Hk, b = unit / a.Hk;
     const AttnSeq sq = attn_seq(a, b);
@@ -697,7 +702,10 @@ Plan attn_plan(const va_tok_attn_args& a) {
     return {(int)nrb, (int)max((int64_t)1, min(want, most))};
 }
 
-int64_t part_bytes(const va_tok_attn_args& a) { return (((max(a.D, a.Dv) + 31) / 32) * 16 * 64 + 64) * 4; }
+int padded(int d) { return (d + 31) / 32 * 32; }
+
+// the staged widths of a call: (32, 64) for heads whose keys are half as wide as their values, else the wider for both
+int64_t part_bytes(const va_tok_attn_args& a) { return (padded(max(a.D, a.Dv)) / 2 * 64 + 64) * 4; }
 
 // a kernel's dynamic LDS beyond 64 KiB, once a device
 template <int LDS, typename K>
@@ -709,23 +717,22 @@ hipError_t big_lds(K kernel) {
     return e;
 }
 
-template <typename T, int DP>
+template <typename T, int DQ, int DV>
 hipError_t attn_go(const va_tok_attn_args& a, hipStream_t st, Plan p) {
     const unsigned units = (unsigned)(a.B * a.Hk);
     if (p.nsplit == 0) {
-        constexpr int lds = 4 * Tr<T>::KT * Dims<T, DP>::CS * 16;
-        if (hipError_t e = big_lds<lds>(attn_kernel<T, DP>)) return e;
-        hipLaunchKernelGGL((attn_kernel<T, DP>), dim3(units * p.nrb), dim3(256), lds, st, a, p.nrb);
+        constexpr int lds = 2 * Tr<T>::KT * (Dims<T, DQ>::CS + Dims<T, DV>::CS) * 16;
+        if (hipError_t e = big_lds<lds>(attn_kernel<T, DQ, DV>)) return e;
+        hipLaunchKernelGGL((attn_kernel<T, DQ, DV>), dim3(units * p.nrb), dim3(256), lds, st, a, p.nrb);
         return hipGetLastError();
     }
-    constexpr int lds = Dims<T, DP>::SLDS;
-    hipError_t e = big_lds<lds>(attn_split<T, DP>);
+    using S = Split<T, DQ, DV>;
+    hipError_t e = big_lds<S::LDS>(attn_split<T, DQ, DV>);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((attn_split<T, DP>), dim3(units * p.nrb * p.nsplit), dim3(64 * Dims<T, DP>::SW), lds, st, a, p.nrb,
-                       p.nsplit);
+    hipLaunchKernelGGL((attn_split<T, DQ, DV>), dim3(units * p.nrb * p.nsplit), dim3(64 * S::SW), S::LDS, st, a, p.nrb, p.nsplit);
     e = hipGetLastError();
     if (e == hipSuccess && p.nsplit > 1) {
-        hipLaunchKernelGGL((attn_join<T, DP>), dim3(units * p.nrb), dim3(64 * (DP / 32)), 0, st, a, p.nrb, p.nsplit);
+        hipLaunchKernelGGL((attn_join<T, DV>), dim3(units * p.nrb), dim3(64 * (DV / 32)), 0, st, a, p.nrb, p.nsplit);
         e = hipGetLastError();
     }
     return e;
@@ -733,11 +740,12 @@ hipError_t attn_go(const va_tok_attn_args& a, hipStream_t st, Plan p) {
 
 template <typename T>
 hipError_t attn_type(const va_tok_attn_args& a, hipStream_t st, Plan p) {
-    switch ((max(a.D, a.Dv) + 31) / 32) {
-        case 1: return attn_go<T, 32>(a, st, p);
-        case 2: return attn_go<T, 64>(a, st, p);
-        case 3: return attn_go<T, 96>(a, st, p);
-        default: return attn_go<T, 128>(a, st, p);
+    if (a.D <= 32 && a.Dv > 32 && a.Dv <= 64) return attn_go<T, 32, 64>(a, st, p);
+    switch (padded(max(a.D, a.Dv))) {
+        case 32: return attn_go<T, 32, 32>(a, st, p);
+        case 64: return attn_go<T, 64, 64>(a, st, p);
+        case 96: return attn_go<T, 96, 96>(a, st, p);
+        default: return attn_go<T, 128, 128>(a, st, p);
     }
 }
 

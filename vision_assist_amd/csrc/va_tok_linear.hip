@@ -499,8 +499,8 @@ __global__ __launch_bounds__(512) void linear_few(va_tok_linear_args a, Out o, i
             }
         }
     };
-    // blocks in pairs: the next pair's loads are in flight while this pair is worked on
-    constexpr int U = MB >= 4 || F == F32 ? 1 : 2;
+    // U blocks at a time, the next U's loads in flight while these are worked on: as many as 2 x 88 registers hold
+    constexpr int REGS = (is8(F) ? 4 : 8 * T) + 8 * MB * (F == F32 ? 2 : 1), U = 88 / REGS < 1 ? 1 : 88 / REGS > 4 ? 4 : 88 / REGS;
     Raw cur[U], nxt[U];
     int kb = wid;
 #pragma unroll
