@@ -544,7 +544,7 @@ int va_post_polygons(void* stream, const va_post_args* p, float* polys, int32_t*
 /* One attention layer over the tokens of camera frames -- the layers a transformer block beside the convolutional
  * network needs: a matrix product with its epilogue, the norms and the rotation of queries and keys, attention with a
  * sliding window and first tokens that stay visible.  Forward only, as every layer of this library.  They take
- * VA_DTYPE_BF16 or VA_DTYPE_F32 tensors; sums, norms and softmax statistics are float.  Every pointer is a device
+ * VA_DTYPE_BF16 or VA_DTYPE_F32 tensors of sides up to 2^31 - 1024; sums, norms and softmax statistics are float.  Every pointer is a device
  * pointer of the stream's device; sizes of zero are allowed where noted and launch nothing.  A caller may put them
  * into the op list of va_seg_run (VA_OP_TOK_*). */
 
@@ -582,7 +582,7 @@ int va_tok_linear(void* stream, const va_tok_linear_args* a);
  * (layout 0) or 2 f and 2 f + 1 (layout 1); the angle is formed in float64, so far positions keep their accuracy.
  * Stored once, rounded once.
  * With slots > 0 keys and values go into a stream's cache: token s of sequence b stands at position p = kv_len[b] -
- * q_len[b] + s and is kept in slot p (p < sinks) or sinks + (p - sinks) % (slots - sinks); of tokens that share a slot
+ * min(q_len[b], S) + s and is kept in slot p (p < sinks) or sinks + (p - sinks) % (slots - sinks); of tokens that share a slot
  * the last one is kept.  Tokens s >= q_len[b] are not read, and nothing is written for them.
  * q_out may be q itself and k_out k itself (same strides). */
 typedef struct va_tok_qk_args {
@@ -604,7 +604,7 @@ typedef struct va_tok_qk_args {
 int va_tok_qk(void* stream, const va_tok_qk_args* a);
 
 /* Attention of B x S queries (Hq heads) over `slots` cached keys and values (Hk heads, Hq % Hk == 0; query head h reads
- * key head h / (Hq / Hk)).  Query s of sequence b stands at position i = kv_len[b] - q_len[b] + s; its frame ends at
+ * key head h / (Hq / Hk)).  Query s of sequence b stands at position i = kv_len[b] - min(q_len[b], S) + s; its frame ends at
  * e = (i / frame + 1) * frame (frame 0, with window and sinks 0: no end), and it sees the keys at positions j < min(e, kv_len[b]) with j < sinks
  * or j >= e - window (window 0: no limit): frame 1 is causal attention token by token, frame = tokens of an image lets
  * the tokens of one image see each other.  Position j is held in slot j (j < sinks) or sinks + (j - sinks) %
@@ -616,7 +616,7 @@ int va_tok_qk(void* stream, const va_tok_qk_args* a);
 typedef struct va_tok_attn_args {
     const void *q, *k, *v;      /* [B][S][Hq][D], [B][slots][Hk][D], [B][slots][Hk][Dv]: D, Dv contiguous, % 8 == 0, <= 128 */
     void* o;                    /* [B][S][Hq][Dv] dtype */
-    int64_t q_sb, q_ss, q_sh, k_sb, k_ss, k_sh, v_sb, v_ss, v_sh, o_sb, o_ss, o_sh; /* strides in elements, % 8 == 0 */
+    int64_t q_sb, q_ss, q_sh, k_sb, k_ss, k_sh, v_sb, v_ss, v_sh, o_sb, o_ss, o_sh; /* strides in elements, % 8 == 0; 0 <= k_ss, v_ss < 2^22 */
     const int32_t *q_len, *kv_len; /* [B] or NULL: S; slots */
     float scale;
     int32_t B, S, Hq, Hk, D, Dv, slots, frame, window, sinks, dtype;

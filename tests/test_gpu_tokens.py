@@ -626,3 +626,57 @@ def test_calls_on_another_stream_and_two_at_once(dtype):
         torch.cuda.synchronize()
         for a, b in zip(got + [here], want + [want[0]]):
             assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+# ------------------------------------------------------------------ far ends of the counts
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("S,frame,window", [(1, 1, 0), (1, 1, 90), (3, 1, 90), (160, 1, 90), (160, 32, 64)])
+@pytest.mark.parametrize("slots,sinks", [(300, 4), (333, 0), (352, 32)])
+def test_attend_positions_up_to_the_last_one(dtype, S, frame, window, slots, sinks):
+    """A ring's result depends on positions by their differences: lengths a whole number of rings (and frames) apart agree."""
+    from vision_assist_amd.tokens import attend
+    g = torch.Generator().manual_seed(S + slots)
+    t = DT[dtype]
+    q, k, v = (rnd(g, *s, dtype=t).cuda() for s in ((2, S, 4, 64), (2, slots, 2, 64), (2, slots, 2, 64)))
+    turn = math.lcm(slots - sinks, frame)
+    far = [2 ** 31 - 1, 2 ** 31 - 60]
+    near = [n - (n - 4 * slots) // turn * turn for n in far]
+    out = [attend(q, k, v, frame=frame, window=window, sinks=sinks, kv_len=torch.tensor(n, dtype=torch.int32, device="cuda"))
+           for n in (far, near)]
+    assert torch.equal(*out)
+
+
+def test_qk_lengths_behind_the_call_are_the_calls():
+    """q_len[b] > S counts as S, as it does for attention: the tokens stand at the last S positions."""
+    from vision_assist_amd.tokens import QKNorm, TokenCache
+    g = torch.Generator().manual_seed(3)
+    q, k, v = (rnd(g, 2, 5, 2, 32, dtype=torch.float32).cuda() for _ in range(3))
+    caches = []
+    for n in ([5, 3], [9, 3]):
+        c = TokenCache(2, 16, 2, 32, dtype="f32").advance(5)
+        QKNorm(32).store(q, k, v, None, c, q_len=torch.tensor(n, dtype=torch.int32, device="cuda"))
+        caches.append(c)
+    assert torch.equal(caches[0].k, caches[1].k) and torch.equal(caches[0].v, caches[1].v)
+
+
+@pytest.mark.parametrize("M,K", [(1, 64), (65, 64), (3, 60)])
+def test_linear_offsets_behind_31_bits(M, K):
+    """Channels from 2^26 on: offsets of their packed rows pass 2^31.  Weights of 1 in one column each: copies of x."""
+    from vision_assist_amd.tokens import Linear
+    N = (1 << 26) + 32
+    lin = Linear.__new__(Linear)
+    from vision_assist_amd import _lib
+    lin.lib, lin.device, lin.N, lin.K, lin.dtype, lin.tdtype = _lib.load(), torch.device("cuda", 0), N, K, "bf16", torch.bfloat16
+    w = torch.zeros(2, (N + 63) // 64 * 2, 32, 32, dtype=torch.bfloat16, device="cuda")
+    at = [0, 31, (1 << 25) - 1, 1 << 25, (1 << 25) + 77, (1 << 26) - 1, 1 << 26, N - 1]
+    for i, n in enumerate(at):  # w[n][i] = 1: row n % 32's place, its first eight columns' piece
+        r = next(r for r in range(32) if 16 * (r // 4 % 2) + 4 * (r // 8) + r % 4 == n % 32)
+        w[0, n // 32, r, 8 * (0 ^ (r // 4 % 4)) + i] = 1
+    lin._w, lin._wscale, lin._bias = w, None, None
+    lin._ptrs, lin._ints = (w.data_ptr(), 0, 0), (N, K, w.shape[1] * 32, 64, 1, 0, 0)
+    x = torch.randn(M, K, device="cuda").to(torch.bfloat16)
+    y = lin(x)
+    for i, n in enumerate(at):
+        assert torch.equal(y[:, n], x[:, i]), f"channel {n}"
+    y[:, at] = 0
+    assert not y.any()

@@ -7,7 +7,8 @@ import pytest
 import torch
 
 from vision_assist_amd import _lib
-from vision_assist_amd.tokens import (AttnArgs, LinearArgs, QKArgs, _apart, _interleaved, _own_elements, attend)
+from vision_assist_amd.tokens import (AttnArgs, Linear, LinearArgs, QKArgs, QKNorm, Rotary, TokenCache, _apart, _interleaved,
+                                      _own_elements, attend)
 
 ERR = _lib.VA_ERR_ARG
 P = 4096  # a pointer that is aligned and never read
@@ -133,3 +134,41 @@ def test_attend_refuses_types_and_places():
         attend(q, k, k, kv_len=torch.zeros(3, dtype=torch.int32))
     with pytest.raises(_lib.VaError):  # no GPU tensors: nothing computes on the host
         attend(q, k, k)
+
+
+BIG = 2 ** 31 - 1
+
+
+@pytest.mark.parametrize("call,kw", [(linear, dict(M=BIG)), (linear, dict(Npad=BIG - 63, N=BIG - 100, ldy=BIG)),
+                                     (linear, dict(Kpad=BIG - 63, K=BIG - 100, ldx=BIG)), (attn, dict(slots=BIG)), (attn, dict(k_ss=-8)),
+                                     (attn, dict(v_ss=-64)), (attn, dict(k_ss=1 << 22)), (attn, dict(v_ss=1 << 24)),
+                                     (qk, dict(B=1, slots=4, v=P, v_out=P, Hk=1 << 12, Dv=1 << 19))])
+def test_sides_and_strides_that_the_kernels_do_not_count(call, kw):
+    assert call(**kw) == ERR
+
+
+@pytest.mark.parametrize("call,kw", [(linear, dict(M=1 << 30, N=1 << 30, Npad=1 << 30, ldy=1 << 30)),
+                                     (linear, dict(M=1 << 30, N=1 << 30, Npad=1 << 30, ldy=1 << 30, K=63)),
+                                     (qk, dict(B=1 << 20, S=1 << 20)), (qk, dict(B=1 << 20, S=1 << 20, D=33))])
+def test_more_workgroups_than_a_launch_has(call, kw):
+    rc = call(**{**dict(x=P), **kw} if call is linear else kw)
+    assert rc == _lib.VA_ERR_RANGE
+
+
+def test_more_workgroups_than_a_launch_has_attention():
+    lib = _lib.load()
+    a = AttnArgs(**{**ATTN, "B": 1 << 20, "S": 1 << 20, "ws": P, "ws_bytes": 1 << 62})
+    assert lib.va_tok_attn(None, ctypes.byref(a)) == _lib.VA_ERR_RANGE
+
+
+def test_tensors_whose_addresses_calls_take_are_not_replaced():
+    c = TokenCache.of(torch.zeros(2, 8, 3, 16), torch.zeros(2, 8, 3, 8), sinks=2)
+    for n in ("k", "v", "sinks", "len"):
+        with pytest.raises(AttributeError):
+            setattr(c, n, getattr(c, n))
+    before = c.len.data_ptr()
+    assert c.advance(3).advance(torch.tensor([1, 2])).len.tolist() == [4, 5] and c.len.data_ptr() == before
+    for cls, names in ((Linear, ("w", "wscale", "bias")), (Rotary, ("turns", "axis")), (QKNorm, ("wq", "wk", "rotary"))):
+        for n in names:
+            with pytest.raises(AttributeError):
+                setattr(cls.__new__(cls), n, None)

@@ -20,6 +20,12 @@ typedef __attribute__((ext_vector_type(4))) short s16x4;
 typedef __attribute__((address_space(1))) void gvoid_t;
 typedef __attribute__((address_space(3))) void lvoid_t;
 
+// the largest side of an operand that the kernels' 32-bit counts take, rounded up to a tile
+constexpr int SIDE_MAX = 0x7fffffff - 1023;
+
+// whether a x b workgroups can be launched: a launch counts its threads in 32 bits
+inline bool grid_ok(int64_t a, int64_t b, int threads) { return a <= 0xffffffffll / threads / (b > 1 ? b : 1); }
+
 // consecutive workgroups go to the 8 XCDs in turn: the i-th workgroup of an XCD takes the i-th tile of a contiguous
 // run, so that neighbouring tiles (which read the same operand rows) share that XCD's L2
 __device__ __forceinline__ int xcd_tile(int bid, int ntiles) {

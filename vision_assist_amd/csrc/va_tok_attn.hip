@@ -35,7 +35,7 @@ __device__ __forceinline__ AttnSeq attn_seq(const va_tok_attn_args& a, int b) {
     return q;
 }
 
-// visible positions of the query at position i: [0, min(sinks, top)) and [low, top), low >= sinks; nothing for i < 0
+// visible positions of the query at position i (up to 2^31 - 2: what follows forms differences of positions, no sums): [0, min(sinks, top)) and [low, top), low >= sinks; nothing for i < 0
 __device__ __forceinline__ Span attn_span(const va_tok_attn_args& a, const AttnSeq& q, int i) {
     if (i < 0) return {a.sinks, 0};
     int64_t e = 0x7fffffff;
@@ -432,18 +432,18 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DV <= 64 ? 3 : 2) : (DV <= 6
         const int64_t slot = slot_of(a, t0);
         const T *kt = kb + slot * a.k_ss, *vt = vb + slot * a.v_ss;
         unsigned char *ks = sm + buf * BUF + wid * NK * 1024, *vs = sm + buf * BUF + KBUF + wid * NP * 1024;
-        const bool whole = t0 + KT <= end;  // (uniform) no row is missing
+        const bool whole = end - t0 >= KT;  // (uniform) no row is missing
 #pragma unroll
         for (int j = 0; j < NK; ++j) {
             const int rj = kr + j * (64 / CK), c = lane % CK ^ swz<T, CK>(rj);
-            const int out = whole ? 0 : (int)(t0 + rj >= end);  // (no short cuts: a branch would split the DMA)
+            const int out = whole ? 0 : (int)(rj >= end - t0);  // (no short cuts: a branch would split the DMA)
             dma16(kt, ks + j * 1024, (out | (int)(c * VE >= a.D)) ? TILE_OOB : krow + 16 * c,
                   j * (64 / CK) * (int)a.k_ss * (int)sizeof(T));
         }
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
             const int rj = vr + j * (64 / CV), c = lane % CV ^ swz<T, CV>(rj);
-            const int out = whole ? 0 : (int)(t0 + rj >= end);
+            const int out = whole ? 0 : (int)(rj >= end - t0);
             dma16(vt, vs + j * 1024, (out | (int)(c * VE >= a.Dv)) ? TILE_OOB : vrow + 16 * c,
                   j * (64 / CV) * (int)a.v_ss * (int)sizeof(T));
         }
@@ -452,7 +452,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DV <= 64 ? 3 : 2) : (DV <= 6
     auto partial = [&](int t) {
         int t0, end;
         w.tile(t, &t0, &end);
-        return t0 + KT > min(g0.top, end) || (t >= w.n0 && t0 < g1.low);
+        return min(g0.top, end) - t0 < KT || (t >= w.n0 && t0 < g1.low);
     };
     // this wave's pieces of tile t are there: what is not finite leaves them before the barrier shows them to the others
     auto clean = [&](int t) {
@@ -478,13 +478,13 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DV <= 64 ? 3 : 2) : (DV <= 6
         int t0, end;
         w.tile(t, &t0, &end);
         const bool sink = t < w.n0;
-        if (!idle && t0 < f1.top && (sink || t0 + KT > f0.low)) {
+        if (!idle && t0 < f1.top && (sink || f0.low - t0 < KT)) {
             f32x16 sc[KB];
             scores<T, DQ, KB>(sc, qf, [&](int k, int c) { return *(const u32x4*)(ks + ad.k[c] + k * 32 * CK * 16); });
             Values<T, DQ, DV> v0;
             if constexpr (sizeof(T) == 2) v0.read(ad, vs, 0);
             const int from = (sink ? 0 : sp.low) - t0, upto = min(sp.top, end) - t0;
-            if (t0 + KT > min(f0.top, end) || (!sink && t0 < f1.low)) mask<KB>(sc, from, upto, lh);  // not all see all
+            if (min(f0.top, end) - t0 < KT || (!sink && t0 < f1.low)) mask<KB>(sc, from, upto, lh);  // not all see all
             softmax<KB, NV>(r, sc, cexp);
             add_values<T, DQ, DV, KB>(r, sc, v0, ad, vs, lane);
             if (bad_tile[buf] == t) add_nonfinite<T, DV>(r, kinds[buf], from, upto, KT, lh);
@@ -551,17 +551,17 @@ __global__ __launch_bounds__((64 * Split<T, DQ, DV>::SW), 1) void attn_split(va_
         const int64_t slot = slot_of(a, t0);
         const T *k = kb + slot * a.k_ss, *v = vb + slot * a.v_ss;
         unsigned char* to = mine + buf * BUF;
-        const bool whole = t0 + 32 <= end;
+        const bool whole = end - t0 >= 32;
 #pragma unroll
         for (int j = 0; j < NK; ++j) {
             const int rj = kr + j * (64 / CK), c = lane % CK ^ swz<T, CK>(rj);
-            const int out = whole ? 0 : (int)(t0 + rj >= end);
+            const int out = whole ? 0 : (int)(rj >= end - t0);
             dma16(k, to + j * 1024, (out | (int)(c * VE >= a.D)) ? TILE_OOB : krow + 16 * c, j * (64 / CK) * (int)a.k_ss * (int)sizeof(T));
         }
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
             const int rj = vr + j * (64 / CV), c = lane % CV ^ swz<T, CV>(rj);
-            const int out = whole ? 0 : (int)(t0 + rj >= end);
+            const int out = whole ? 0 : (int)(rj >= end - t0);
             dma16(v, to + KBUF + j * 1024, (out | (int)(c * VE >= a.Dv)) ? TILE_OOB : vrow + 16 * c,
                   j * (64 / CV) * (int)a.v_ss * (int)sizeof(T));
         }
@@ -575,7 +575,7 @@ __global__ __launch_bounds__((64 * Split<T, DQ, DV>::SW), 1) void attn_split(va_
         unsigned char *ks = mine + buf * BUF, *vs = ks + KBUF;
         int t0, end;
         w.tile(t, &t0, &end);
-        const bool sink = t < w.n0, partial = t0 + 32 > min(f0.top, end) || (!sink && t0 < f1.low);  // for some row
+        const bool sink = t < w.n0, partial = min(f0.top, end) - t0 < 32 || (!sink && t0 < f1.low);  // for some row
         bool bad = false;
         if (partial) {
 #pragma unroll
@@ -675,12 +675,12 @@ bool attn_ok(const va_tok_attn_args& a) {
     if (a.B < 0 || a.S < 0 || a.Hk < 1 || a.Hq < a.Hk || a.Hq % a.Hk || a.slots < 0) return false;
     if (a.dtype != VA_DTYPE_BF16 && a.dtype != VA_DTYPE_F32) return false;
     if (a.D < 8 || a.D > 128 || a.D % 8 || a.Dv < 8 || a.Dv > 128 || a.Dv % 8) return false;
-    if (a.frame < 0 || a.window < 0 || a.sinks < 0 || (a.slots && a.sinks >= a.slots)) return false;
+    if (a.frame < 0 || a.window < 0 || a.sinks < 0 || (a.slots && a.sinks >= a.slots) || a.slots > SIDE_MAX) return false;
     if (!a.frame && (a.window || a.sinks)) return false;
     if (!(a.scale > 0.0f) || !(a.scale < INFINITY)) return false;
     if ((int64_t)a.S * (a.Hq / a.Hk) > INT32_MAX - 256) return false;
     const int64_t st = a.q_sb | a.q_ss | a.q_sh | a.k_sb | a.k_ss | a.k_sh | a.v_sb | a.v_ss | a.v_sh | a.o_sb | a.o_ss | a.o_sh;
-    if (st % 8 || a.k_ss >= ROW_MAX || a.v_ss >= ROW_MAX) return false;
+    if (st % 8 || min(a.k_ss, a.v_ss) < 0 || max(a.k_ss, a.v_ss) >= ROW_MAX) return false;
     const bool some = a.B > 0 && a.S > 0;
     if (some && (!a.q || !a.o || (a.slots && (!a.k || !a.v)))) return false;
     return !(((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.o) & 15);
@@ -765,7 +765,7 @@ int va_tok_attn(void* stream, const va_tok_attn_args* ap) {
     const va_tok_attn_args& a = *ap;
     if (a.B == 0 || a.S == 0) return VA_OK;
     const Plan p = attn_plan(a);
-    if ((int64_t)a.B * a.Hk * p.nrb * max(p.nsplit, 1) > INT32_MAX) return VA_ERR_RANGE;
+    if (!grid_ok((int64_t)a.B * a.Hk, p.nrb * max(p.nsplit, 1), 256)) return VA_ERR_RANGE;
     const int64_t need = va_tok_attn_workspace_bytes(ap);
     if (need > 0 && (!a.ws || a.ws_bytes < need || ((uintptr_t)a.ws & 15))) return VA_ERR_ARG;
     const hipError_t e = a.dtype == VA_DTYPE_F32 ? attn_type<float>(a, (hipStream_t)stream, p)

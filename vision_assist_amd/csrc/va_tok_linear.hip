@@ -288,7 +288,7 @@ __global__ __launch_bounds__(256, 2) void linear_tile(va_tok_linear_args a, Out 
     // weights: DMA d of a stage's plane copies its bytes [1024 d, 1024 d + 1024); blocks from channel Npad on are not there
     const unsigned char* wb = (const unsigned char*)a.w + (int64_t)(n0 / 32) * 32 * C::WROW;
     const int64_t wstep = (int64_t)a.Npad * C::WROW, plane = wstep * (a.Kpad / 32);
-    const int wend = (a.Npad - n0) * C::WROW;
+    const int wend = min(a.Npad - n0, C::BN) * C::WROW;
     auto issue_w = [&](int t) {
         unsigned char* to = sm + t % C::NSW * C::WB;
         const unsigned char* from = wb + min(t, nk - 1) * wstep;
@@ -436,7 +436,7 @@ __global__ __launch_bounds__(512) void linear_few(va_tok_linear_args a, Out o, i
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fr = lane & 15, fq = lane >> 4;
     const int n0 = blockIdx.x % ntn * 16, m0 = blockIdx.x / ntn * 16 * MB;
     const int nk = (a.K + 63) / 64;
-    const int wrow = (n0 / 32) * 32 + row_of((n0 & 16) + fr);  // this lane's weight row among a step's
+    const int64_t wrow = (n0 / 32) * 32 + row_of((n0 & 16) + fr);  // this lane's weight row among a step's
     int64_t xrow[MB];
 #pragma unroll
     for (int j = 0; j < MB; ++j) xrow[j] = (int64_t)min(m0 + 16 * j + fr, a.M - 1) * a.ldx;
@@ -530,6 +530,7 @@ __global__ __launch_bounds__(512) void linear_few(va_tok_linear_args a, Out o, i
 
 bool linear_ok(const va_tok_linear_args& a) {
     if (a.M < 0 || a.N <= 0 || a.K <= 0 || !a.w || !a.y || (a.M > 0 && !a.x)) return false;
+    if (a.M > SIDE_MAX || a.Npad > SIDE_MAX || a.Kpad > SIDE_MAX) return false;
     if (a.dtype != VA_DTYPE_BF16 && a.dtype != VA_DTYPE_F32) return false;
     if ((a.w8 != 0 && a.w8 != 1) || (a.w8 && (a.dtype != VA_DTYPE_BF16 || !a.wscale)) || (!a.w8 && a.wscale)) return false;
     if (a.act < VA_ACT_NONE || a.act > VA_ACT_RELU) return false;
@@ -547,13 +548,14 @@ template <Form F, int WN, int WM>
 hipError_t go_tile(const va_tok_linear_args& a, const Out& o, hipStream_t st) {
     using C = TileCfg<F, WN, WM>;
     constexpr int lds = C::LDS;
+    const int ntn = (a.N + C::BN - 1) / C::BN, ntm = (a.M + C::BM - 1) / C::BM;
+    if (!grid_ok(ntn, ntm, 256)) return hipErrorInvalidConfiguration;
     static DevFlag attr;
     if (lds > 65536 && !attr()) {
         const hipError_t e = hipFuncSetAttribute((const void*)linear_tile<F, WN, WM>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         if (e != hipSuccess) return e;
         attr() = true;
     }
-    const int ntn = (a.N + C::BN - 1) / C::BN, ntm = (a.M + C::BM - 1) / C::BM;
     hipLaunchKernelGGL((linear_tile<F, WN, WM>), dim3((unsigned)(ntn * ntm)), dim3(256), lds, st, a, o, ntn, ntm);
     return hipGetLastError();
 }
@@ -561,6 +563,7 @@ hipError_t go_tile(const va_tok_linear_args& a, const Out& o, hipStream_t st) {
 template <Form F, int MB>
 hipError_t go_few(const va_tok_linear_args& a, const Out& o, hipStream_t st) {
     const int ntn = (a.N + 15) / 16, ntm = (a.M + 16 * MB - 1) / (16 * MB);
+    if (!grid_ok(ntn, ntm, 512)) return hipErrorInvalidConfiguration;
     hipLaunchKernelGGL((linear_few<F, MB>), dim3((unsigned)(ntn * ntm)), dim3(512), 0, st, a, o, ntn);
     return hipGetLastError();
 }
@@ -568,6 +571,7 @@ hipError_t go_few(const va_tok_linear_args& a, const Out& o, hipStream_t st) {
 template <Form F>
 hipError_t go_any(const va_tok_linear_args& a, const Out& o, hipStream_t st, int xvec) {
     const int ntn = (a.N + GB - 1) / GB, ntm = (a.M + GB - 1) / GB;
+    if (!grid_ok(ntn, ntm, 256)) return hipErrorInvalidConfiguration;
     hipLaunchKernelGGL(linear_any<F>, dim3((unsigned)(ntn * ntm)), dim3(256), 0, st, a, o, ntn, xvec);
     return hipGetLastError();
 }
@@ -598,7 +602,6 @@ extern "C" int va_tok_linear(void* stream, const va_tok_linear_args* ap) {
     if (!ap || !linear_ok(*ap)) return VA_ERR_ARG;
     const va_tok_linear_args& a = *ap;
     if (a.M == 0) return VA_OK;
-    if ((int64_t)((a.N + 15) / 16) * ((a.M + 15) / 16) > INT32_MAX) return VA_ERR_RANGE;
     const bool f32 = a.dtype == VA_DTYPE_F32;
     const bool f32out = f32 || a.out_f32;
     Out o = {a.wscale, a.bias, a.res, a.y, a.ldr, a.ldy, a.M, a.N, a.act, 0};
@@ -613,5 +616,5 @@ extern "C" int va_tok_linear(void* stream, const va_tok_linear_args* ap) {
     const hipError_t e = f32         ? go<F32>(a, o, st)
                          : a.out_f32 ? (a.w8 ? go<W8F>(a, o, st) : go<BF16F>(a, o, st))
                                      : (a.w8 ? go<W8>(a, o, st) : go<BF16>(a, o, st));
-    return e == hipSuccess ? VA_OK : VA_ERR_HIP;
+    return e == hipSuccess ? VA_OK : e == hipErrorInvalidConfiguration ? VA_ERR_RANGE : VA_ERR_HIP;
 }

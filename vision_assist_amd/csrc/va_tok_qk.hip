@@ -43,7 +43,7 @@ __device__ __forceinline__ void pair_at(int f, int D, int rot, int layout, int* 
 
 // the slot of token s of sequence b, or -1: not kept
 __device__ __forceinline__ int kept_slot(const va_tok_qk_args& a, int b, int s) {
-    const int ql = a.q_len ? a.q_len[b] : a.S, kv = a.kv_len ? a.kv_len[b] : ql, ring = a.slots - a.sinks;
+    const int ql = a.q_len ? min(a.q_len[b], a.S) : a.S, kv = a.kv_len ? a.kv_len[b] : ql, ring = a.slots - a.sinks;
     const int64_t p = (int64_t)kv - ql + s;
     if (p < 0 || p >= kv || (p >= a.sinks && p < (int64_t)kv - ring)) return -1;
     return p < a.sinks ? (int)p : a.sinks + ((int)p - a.sinks) % ring;
@@ -244,7 +244,7 @@ bool qk_ok(const va_tok_qk_args& a) {
     const bool some = a.B > 0 && a.S > 0;
     if (some && ((a.Hq && (!a.q || !a.q_out)) || (a.Hk && (!a.k || !a.k_out)))) return false;
     if (a.slots < 0 || a.sinks < 0 || (a.slots && a.sinks >= a.slots)) return false;
-    if (a.slots && a.Hk && some && (!a.v || !a.v_out || a.Dv < 1)) return false;
+    if (a.slots && a.Hk && some && (!a.v || !a.v_out || a.Dv < 1 || (int64_t)a.Hk * a.Dv > SIDE_MAX)) return false;
     return true;
 }
 
@@ -272,7 +272,7 @@ extern "C" int va_tok_qk(void* stream, const va_tok_qk_args* ap) {
     const dim3 block(64 * QK_WAVES);
     if (!wide_ok(a)) {
         const int64_t blocks = (tokens + QK_WAVES - 1) / QK_WAVES;
-        if (blocks > INT32_MAX) return VA_ERR_RANGE;
+        if (!grid_ok(blocks, 1, 64 * QK_WAVES)) return VA_ERR_RANGE;
         if (f32)
             hipLaunchKernelGGL(qk_any<float>, dim3((unsigned)blocks), block, 0, st, a);
         else
@@ -286,7 +286,7 @@ extern "C" int va_tok_qk(void* stream, const va_tok_qk_args* ap) {
     const int groups = (a.Hq + a.Hk + 64 / lph - 1) / (64 / lph);
     const int parts = (int)max((int64_t)1, min((int64_t)groups, 2048 / tokens));
     const int64_t blocks = (tokens * parts + QK_WAVES - 1) / QK_WAVES;
-    if (blocks > INT32_MAX) return VA_ERR_RANGE;
+    if (!grid_ok(blocks, 1, 64 * QK_WAVES)) return VA_ERR_RANGE;
     const dim3 grid((unsigned)blocks);
     if (f32 && a.layout)
         hipLaunchKernelGGL((qk_wide<float, 2, 1>), grid, block, 0, st, a, lph, parts);

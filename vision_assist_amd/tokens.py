@@ -135,6 +135,11 @@ def _own_elements(out: torch.Tensor) -> None:
         at = s * n
 
 
+def _fixed(name: str) -> property:
+    """A tensor whose address a call takes from the object: it is read, not replaced (its values may change)."""
+    return property(lambda self: self.__dict__["_" + name])
+
+
 _raw_stream, _device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
@@ -178,6 +183,8 @@ class Linear:
     convolutions' are, or given as float8_e4m3fn values with ``scale`` [N]).  bias: [N].  act: None, "silu", "gelu",
     "gelu_tanh" or "relu"."""
 
+    w, wscale, bias = _fixed("w"), _fixed("wscale"), _fixed("bias")
+
     def __init__(self, weight: torch.Tensor, bias: torch.Tensor | None = None, act: str | None = None,
                  dtype: str = "bf16", scale: torch.Tensor | None = None, device=None):
         _need(dtype in ("bf16", "f32", "w8a16"), f"dtype {dtype!r}: bf16, f32 or w8a16")
@@ -205,7 +212,7 @@ class Linear:
             p[:N, :K] = t
             return p
 
-        w, self.wscale = weight.detach().to(self.device), None
+        w, self._wscale = weight.detach().to(self.device), None
         if dtype == "w8a16":
             if scale is None:
                 from .seg import F8_MAX
@@ -213,16 +220,16 @@ class Linear:
                 amax = w.abs().amax(1)
                 scale = torch.where(amax > 0, amax / F8_MAX, torch.ones_like(amax))
                 w = (w / scale[:, None]).clamp(-F8_MAX, F8_MAX).to(torch.float8_e4m3fn)
-            self.wscale = torch.ones(Np, dtype=torch.float32, device=self.device)
-            self.wscale[:N] = scale.detach().to(self.device, torch.float32)
-            self.w = _blocks(padded(w.view(torch.uint8)))
+            self._wscale = torch.ones(Np, dtype=torch.float32, device=self.device)
+            self._wscale[:N] = scale.detach().to(self.device, torch.float32)
+            self._w = _blocks(padded(w.view(torch.uint8)))
         elif dtype == "f32":
-            self.w = torch.stack([_blocks(t) for t in split3_bf16(padded(w.float())).permute(2, 0, 1, 3).reshape(3, Np, Kp)])
+            self._w = torch.stack([_blocks(t) for t in split3_bf16(padded(w.float())).permute(2, 0, 1, 3).reshape(3, Np, Kp)])
         else:
-            self.w = _blocks(padded(w.to(torch.bfloat16)))
-        self.bias = None if bias is None else bias.detach().to(self.device, torch.float32).contiguous()
-        self._ptrs = (self.w.data_ptr(), self.wscale.data_ptr() if self.wscale is not None else 0,
-                      self.bias.data_ptr() if bias is not None else 0)
+            self._w = _blocks(padded(w.to(torch.bfloat16)))
+        self._bias = None if bias is None else bias.detach().to(self.device, torch.float32).contiguous()
+        self._ptrs = (self._w.data_ptr(), self._wscale.data_ptr() if self._wscale is not None else 0,
+                      self._bias.data_ptr() if bias is not None else 0)
         self._ints = (N, K, Np, Kp, VA_DTYPE_F32 if dtype == "f32" else VA_DTYPE_BF16, int(dtype == "w8a16"), ACTS[act])
 
     def args(self, x: torch.Tensor, out: torch.Tensor, residual: torch.Tensor | None = None) -> LinearArgs:
@@ -243,7 +250,7 @@ class Linear:
         float; it may be the residual itself, and must not overlap x."""
         _on(x, self.device, self.tdtype, "x")
         if not _here(self.device, stream):
-            return _elsewhere(self.device, stream, (x, residual, out, self.w), lambda: self(x, residual, out))
+            return _elsewhere(self.device, stream, (x, residual, out, self.w, self.wscale, self.bias), lambda: self(x, residual, out))
         shape = x.shape
         if len(shape) == 0 or shape[-1] != self.K:
             raise _lib.VaError(f"x {tuple(shape)}: [..., {self.K}]")
@@ -300,6 +307,8 @@ class Rotary:
     the n pairs of its axis (freqs "axis").  layout "half": pair f is values f and f + dim / 2; "pairs": 2 f and
     2 f + 1."""
 
+    turns, axis = _fixed("turns"), _fixed("axis")
+
     def __init__(self, dim: int, sections=None, base: float = 10000.0, layout: str = "half", freqs: str = "shared",
                  device=None):
         _need(dim > 0 and dim % 2 == 0, f"dim {dim}: even")
@@ -317,9 +326,9 @@ class Rotary:
         self.device = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
         if self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
-        self.turns = torch.tensor([base ** -v / (2 * math.pi) for v in e], dtype=torch.float64, device=self.device)
-        self.axis = torch.tensor([a for a, n in enumerate(sections) for _ in range(n)], dtype=torch.int32,
-                                 device=self.device)
+        self._turns = torch.tensor([base ** -v / (2 * math.pi) for v in e], dtype=torch.float64, device=self.device)
+        self._axis = torch.tensor([a for a, n in enumerate(sections) for _ in range(n)], dtype=torch.int32,
+                                  device=self.device)
 
 
 class TokenCache:
@@ -327,6 +336,8 @@ class TokenCache:
 
     k [B, slots, heads, D], v [B, slots, heads, Dv], len [B] (int32, on the device): tokens seen so far.  Position p is
     kept in slot p while p < slots; later ones take the slots behind the sinks in turn."""
+
+    k, v, sinks, len = _fixed("k"), _fixed("v"), _fixed("sinks"), _fixed("len")
 
     def __init__(self, B: int, slots: int, heads: int, head_dim: int, v_dim: int | None = None, sinks: int = 0,
                  dtype: str = "bf16", device=None):
@@ -348,7 +359,7 @@ class TokenCache:
         _own_elements(k)
         _own_elements(v)
         _apart(k, v, "the values")
-        self.k, self.v, self.sinks, self.len = k, v, int(sinks), length
+        self._k, self._v, self._sinks, self._len = k, v, int(sinks), length
         self.slots = k.shape[1]
         item = k.element_size()
         (ka, k0, k1, k2, _, kend), (va, v0, v1, v2, _, vend) = _plain(k, item), _plain(v, item)
@@ -363,7 +374,7 @@ class TokenCache:
 
     def advance(self, n) -> "TokenCache":
         """n (an int, or int32 [B] on the device) more tokens of each stream: before they are stored."""
-        self.len += n
+        self._len += n
         return self
 
 
@@ -371,6 +382,8 @@ class QKNorm:
     """x / sqrt(mean(x^2) + eps) * weight for each head of the queries and keys, then ``rotary``, in one pass.
 
     q_weight / k_weight: [head_dim] (None: that norm is left out).  rotary: a Rotary (None: no rotation)."""
+
+    wq, wk, rotary = _fixed("wq"), _fixed("wk"), _fixed("rotary")
 
     def __init__(self, head_dim: int, rotary: Rotary | None = None, q_weight: torch.Tensor | None = None,
                  k_weight: torch.Tensor | None = None, eps: float = 1e-6, device=None):
@@ -385,12 +398,13 @@ class QKNorm:
         if self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
         _need(rotary is None or rotary.device == self.device, "rotary: on another device")
-        self.D, self.rotary = head_dim, rotary
-        self.wq, self.wk = (None if w is None else w.detach().to(self.device, torch.float32).contiguous()
-                            for w in (q_weight, k_weight))
+        self.D, self._rotary = head_dim, rotary
+        self._wq, self._wk = (None if w is None else w.detach().to(self.device, torch.float32).contiguous()
+                              for w in (q_weight, k_weight))
         self.eps = float(eps)
         self._norm = (self.wq.data_ptr() if self.wq is not None else 0, self.wk.data_ptr() if self.wk is not None else 0,
                       self.eps)
+        self._held = (self.wq, self.wk, *(() if rotary is None else (rotary.turns, rotary.axis)))
         self._turn = (0, 0, 0) if rotary is None else (rotary.dim, rotary.turns.data_ptr(), rotary.axis.data_ptr())
         self._rot = (0, 0) if rotary is None else (rotary.axes, LAYOUTS[rotary.layout])
 
@@ -400,7 +414,8 @@ class QKNorm:
         -> (q', k').  pos: int32 [B, S, axes] ([B, S] for one axis; expanded views are fine).  q_out / k_out may be
         q / k themselves."""
         if not _here(self.device, stream):
-            return _elsewhere(self.device, stream, (q, k, pos, q_out, k_out), lambda: self(q, k, pos, q_out, k_out))
+            return _elsewhere(self.device, stream, (q, k, pos, q_out, k_out, *self._held),
+                              lambda: self(q, k, pos, q_out, k_out))
         q, k, pos, turn, B, S, Hq, Hk, item = self._begin(q, k, pos)
         if q_out is None and k_out is None:
             q_out, k_out = q.new_empty(q.shape), k.new_empty(k.shape)
@@ -422,11 +437,11 @@ class QKNorm:
 
     def store(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor | None, cache: TokenCache,
               q_len: torch.Tensor | None = None, q_out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
-        """The same for the last q_len[b] tokens (default S) of cache.len[b]: -> q', with the keys and values in the
+        """The same for the last q_len[b] tokens (S at most, and by default) of cache.len[b]: -> q', with the keys and values in the
         cache.  Rows s >= q_len[b] of q_out are left as they were (zeros where the call makes it); a token whose slot a
         later one of the call takes, or whose position is negative, is not kept."""
         if not _here(self.device, stream):
-            return _elsewhere(self.device, stream, (q, k, v, pos, q_len, q_out, cache.k, cache.v, cache.len),
+            return _elsewhere(self.device, stream, (q, k, v, pos, q_len, q_out, cache.k, cache.v, cache.len, *self._held),
                               lambda: self.store(q, k, v, pos, cache, q_len, q_out))
         q, k, pos, turn, B, S, Hq, Hk, item = self._begin(q, k, pos)
         Dv = cache.v.shape[3]
@@ -536,7 +551,7 @@ def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float | 
     """softmax(scale q k^T) v of q [B, S, Hq, D] over k [B, slots, Hk, D] and v [B, slots, Hk, Dv] (a TokenCache's
     tensors, or a batch of prompts), Hq a multiple of Hk: -> [B, S, Hq, Dv].
 
-    The queries of sequence b are its last q_len[b] (default S) of kv_len[b] (default slots) positions.  A query at
+    The queries of sequence b are its last q_len[b] (S at most, and by default) of kv_len[b] (default slots) positions.  A query at
     position i sees the positions j < e = (i // frame + 1) * frame with j < sinks or j >= e - window (window 0: all of
     them): frame 1 goes token by token, frame = tokens of an image lets one image's tokens see each other, and frame 0
     (with window = sinks = 0) lets every token see every token.  With kv_len[b] > slots the tensors are rings behind
