@@ -5,6 +5,7 @@
 #include <stdint.h>
 
 #include "../../include/va355.h"
+#include "va_dev.h"
 
 namespace tok {
 
@@ -25,6 +26,16 @@ constexpr int SIDE_MAX = 0x7fffffff - 1023;
 
 // whether a x b workgroups can be launched: a launch counts its threads in 32 bits
 inline bool grid_ok(int64_t a, int64_t b, int threads) { return a <= 0xffffffffll / threads / (b > 1 ? b : 1); }
+
+// a kernel's dynamic LDS beyond 64 KiB, once a device
+template <auto KERNEL, int LDS>
+hipError_t big_lds() {
+    static DevFlag attr;
+    if (LDS <= 65536 || attr()) return hipSuccess;
+    const hipError_t e = hipFuncSetAttribute((const void*)KERNEL, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+    if (e == hipSuccess) attr() = true;
+    return e;
+}
 
 // consecutive workgroups go to the 8 XCDs in turn: the i-th workgroup of an XCD takes the i-th tile of a contiguous
 // run, so that neighbouring tiles (which read the same operand rows) share that XCD's L2

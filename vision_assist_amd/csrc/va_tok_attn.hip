@@ -704,30 +704,19 @@ Plan attn_plan(const va_tok_attn_args& a) {
 
 int padded(int d) { return (d + 31) / 32 * 32; }
 
-// the staged widths of a call: (32, 64) for heads whose keys are half as wide as their values, else the wider for both
 int64_t part_bytes(const va_tok_attn_args& a) { return (padded(max(a.D, a.Dv)) / 2 * 64 + 64) * 4; }
-
-// a kernel's dynamic LDS beyond 64 KiB, once a device
-template <int LDS, typename K>
-hipError_t big_lds(K kernel) {
-    static DevFlag attr;
-    if (LDS <= 65536 || attr()) return hipSuccess;
-    const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
-    if (e == hipSuccess) attr() = true;
-    return e;
-}
 
 template <typename T, int DQ, int DV>
 hipError_t attn_go(const va_tok_attn_args& a, hipStream_t st, Plan p) {
     const unsigned units = (unsigned)(a.B * a.Hk);
     if (p.nsplit == 0) {
         constexpr int lds = 2 * Tr<T>::KT * (Dims<T, DQ>::CS + Dims<T, DV>::CS) * 16;
-        if (hipError_t e = big_lds<lds>(attn_kernel<T, DQ, DV>)) return e;
+        if (hipError_t e = big_lds<attn_kernel<T, DQ, DV>, lds>()) return e;
         hipLaunchKernelGGL((attn_kernel<T, DQ, DV>), dim3(units * p.nrb), dim3(256), lds, st, a, p.nrb);
         return hipGetLastError();
     }
     using S = Split<T, DQ, DV>;
-    hipError_t e = big_lds<S::LDS>(attn_split<T, DQ, DV>);
+    hipError_t e = big_lds<attn_split<T, DQ, DV>, S::LDS>();
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL((attn_split<T, DQ, DV>), dim3(units * p.nrb * p.nsplit), dim3(64 * S::SW), S::LDS, st, a, p.nrb, p.nsplit);
     e = hipGetLastError();
@@ -738,6 +727,7 @@ hipError_t attn_go(const va_tok_attn_args& a, hipStream_t st, Plan p) {
     return e;
 }
 
+// heads whose keys are half as wide as their values are staged as they are, others at the wider of both widths
 template <typename T>
 hipError_t attn_type(const va_tok_attn_args& a, hipStream_t st, Plan p) {
     if (a.D <= 32 && a.Dv > 32 && a.Dv <= 64) return attn_go<T, 32, 64>(a, st, p);

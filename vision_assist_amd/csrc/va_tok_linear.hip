@@ -426,104 +426,121 @@ __global__ __launch_bounds__(256, 2) void linear_tile(va_tok_linear_args a, Out 
 }
 
 // ------------------------------------------------------------------ few tiles: K over the waves of a workgroup
-// 16 channels x 16 MB tokens per workgroup; its eight waves take every eighth block of 64 of K, straight from memory into
-// the fragments (weights are read once, the tokens' values come from the L2), and their sums are joined in LDS in the
-// waves' order.  v_mfma_f32_16x16x32_bf16.
+// 16 channels x 16 MB tokens per workgroup; its eight waves take every eighth step of 128 bytes of the tokens' rows, each
+// through two slots of its own in LDS and without a barrier, and their sums are joined in LDS in the waves' order.
+// v_mfma_f32_16x16x32_bf16.
+// Bound by the weights' bytes (32 x 4096 x 4096 over 24 sets of weights: e4m3 9.3 us, bf16 11.0; x 16384: 30.6 and 36.2,
+// 3.7 TB/s; one token, 1024 x 4096: 4.6).  The tokens come by LDS-DMA, eight lanes to a row's 128 bytes: loaded straight
+// into the fragments neighbouring lanes held different rows, so that each lane's 16 bytes was a request of its own, and
+// the tokens, not the weights, took the time (12.9, 14.1; 49.0 and 52.9 us).  Three or four slots: 1 to 9 us slower where
+// workgroups queue, as fewer fit a CU.
+template <Form F, int MB>
+struct FewCfg {
+    static constexpr int NW = 8, XE = F == F32 ? 4 : 2, KS = 128 / XE;  // waves; K of a step
+    static constexpr int NS = 2;                                        // steps in LDS
+    static constexpr int DX = 2 * MB, DW = is8(F) ? 1 : F == F32 ? 3 : 2;  // loads of a step: tokens', weights'
+    static constexpr int XB = DX * 1024, LDS = NW * NS * XB;
+};
 template <Form F, int MB>
 __global__ __launch_bounds__(512) void linear_few(va_tok_linear_args a, Out o, int ntn) {
-    constexpr int T = F == F32 ? 3 : 1, NW = 8;
-    __shared__ f32x4 part[NW][MB][64];
+    using C = FewCfg<F, MB>;
+    constexpr int T = F == F32 ? 3 : 1, NW = C::NW, XE = C::XE, NS = C::NS;
+    extern __shared__ __align__(16) unsigned char sm[];  // a wave: [NS][16 MB tokens][128]; then its sums
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fr = lane & 15, fq = lane >> 4;
     const int n0 = blockIdx.x % ntn * 16, m0 = blockIdx.x / ntn * 16 * MB;
-    const int nk = (a.K + 63) / 64;
-    const int64_t wrow = (n0 / 32) * 32 + row_of((n0 & 16) + fr);  // this lane's weight row among a step's
-    int64_t xrow[MB];
-#pragma unroll
-    for (int j = 0; j < MB; ++j) xrow[j] = (int64_t)min(m0 + 16 * j + fr, a.M - 1) * a.ldx;
+    const int nk = (a.K + C::KS - 1) / C::KS, count = (nk - wid + NW - 1) / NW;  // steps wid, wid + NW, ... are this wave's
+    const int64_t wrow = (n0 / 32) * 32 + row_of((n0 & 16) + fr);                // this lane's weight row among a step's
+    unsigned char* mine = sm + wid * NS * C::XB;
     f32x4 acc[MB];
 #pragma unroll
     for (int j = 0; j < MB; ++j) acc[j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-    struct Raw {
-        u32x4 w[is8(F) ? 1 : 2 * T], x[2][MB][F == F32 ? 2 : 1];
-    };
-    auto load = [&](Raw& r, int kb) {
-        const int k = kb * 64 + 8 * fq;
+    u32x4 w[NS][C::DW];
+    // DMA j takes rows 8 j .. 8 j + 7, lane l row l / 8, place l % 8: piece place ^ (row / 2 % 8)
+    const int l8 = lane >> 3, piece = (lane & 7) ^ (l8 >> 1), xmore = a.M - m0 - l8;
+    const unsigned char* xb = (const unsigned char*)a.x + (int64_t)m0 * a.ldx * XE;
+    const int xoff[2] = {(int)(l8 * a.ldx) * XE + 16 * piece, (int)(l8 * a.ldx) * XE + 16 * (piece ^ 4)};
+    auto issue = [&](int i, int s) {  // (steps past the last one: no tokens, and the last one's weights, which no product uses)
+        const int kb = wid + i * NW, kw = min(kb, nk - 1);
         if constexpr (is8(F)) {  // one 16-byte piece: 16 of K
-            r.w[0] = *(const u32x4*)((const uint8_t*)a.w + ((int64_t)(2 * kb + fq / 2) * (a.Npad / 32)) * 1024 + wrow * 32 +
-                                     16 * ((fq & 1) ^ ((wrow >> 4) & 1)));
-            if (wrow & 8) r.w[0] = (u32x4){r.w[0][2], r.w[0][3], r.w[0][0], r.w[0][1]};
+            w[s][0] = *(const u32x4*)((const uint8_t*)a.w + ((int64_t)(2 * kw + fq / 2) * (a.Npad / 32)) * 1024 + wrow * 32 +
+                                      16 * ((fq & 1) ^ ((wrow >> 4) & 1)));
+        } else if constexpr (F == F32) {
+#pragma unroll
+            for (int t = 0; t < T; ++t)
+                w[s][t] = *(const u32x4*)((const __bf16*)a.w + (int64_t)t * a.Npad * a.Kpad + (int64_t)kw * (a.Npad / 32) * 1024 +
+                                          wrow * 32 + 8 * (fq ^ ((wrow >> 2) & 3)));
         } else {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int t = 0; t < T; ++t)
-                    r.w[h * T + t] = *(const u32x4*)((const __bf16*)a.w + (int64_t)t * a.Npad * a.Kpad +
-                                                     ((int64_t)(2 * kb + h) * (a.Npad / 32)) * 1024 + wrow * 32 +
-                                                     8 * (fq ^ ((wrow >> 2) & 3)));
+                w[s][h] = *(const u32x4*)((const __bf16*)a.w + (int64_t)(2 * kw + h) * (a.Npad / 32) * 1024 + wrow * 32 +
+                                          8 * (fq ^ ((wrow >> 2) & 3)));
         }
+        const int k = kb * C::KS;
+        const bool in[2] = {k + piece * (16 / XE) < a.K, k + (piece ^ 4) * (16 / XE) < a.K};
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int j = 0; j < MB; ++j) {
-                const int kk = is8(F) ? kb * 64 + 16 * fq + 8 * h : k + 32 * h;
-                if constexpr (F == F32) {
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)
-                        r.x[h][j][e] = kk + 4 * e < a.K ? *(const u32x4*)((const float*)a.x + xrow[j] + kk + 4 * e) : (u32x4){0, 0, 0, 0};
-                } else {
-                    r.x[h][j][0] = kk < a.K ? *(const u32x4*)((const __bf16*)a.x + xrow[j] + kk) : (u32x4){0, 0, 0, 0};
-                }
-            }
+        for (int j = 0; j < C::DX; ++j)
+            dma16(xb, mine + s * C::XB + j * 1024, in[j & 1] && 8 * j < xmore ? xoff[j & 1] : LIN_OOB,
+                  (int)(8 * j * a.ldx) * XE + min(kb, nk) * 128);
     };
-    auto mma = [&](const Raw& r) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            bf16x8 w[T];
-#pragma unroll
-            for (int t = 0; t < T; ++t)
-                w[t] = is8(F) ? e4m3x8(make_uint2(r.w[0][2 * h], r.w[0][2 * h + 1])) : (bf16x8)r.w[h * T + t];
+    const int turn = (fr >> 1) & 7;
+    auto mma = [&](int s) {
+        const unsigned char* xs = mine + s * C::XB + fr * 128;
+        if constexpr (F == F32) {
 #pragma unroll
             for (int j = 0; j < MB; ++j) {
+                const f32x4 u = *(const f32x4*)(xs + j * 2048 + 16 * ((2 * fq) ^ turn));
+                const f32x4 v = *(const f32x4*)(xs + j * 2048 + 16 * ((2 * fq + 1) ^ turn));
+                const float e[8] = {u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
                 bf16x8 x[T];
-                if constexpr (F == F32) {
-                    float e[8];
+                split3(e, x);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) e[i] = __uint_as_float(r.x[h][j][i / 4][i % 4]);
-                    split3(e, x);
-                } else {
-                    x[0] = (bf16x8)r.x[h][j][0];
-                }
+                for (int t = 0; t < NTERM; ++t)
+                    acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16((bf16x8)w[s][TERM_W[t]], x[TERM_X[t]], acc[j], 0, 0, 0);
+            }
+        } else {
+            u32x4 r = w[s][0];
+            if (is8(F) && (wrow & 8)) r = (u32x4){r[2], r[3], r[0], r[1]};
 #pragma unroll
-                for (int t = 0; t < (T > 1 ? NTERM : 1); ++t)
-                    acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[T > 1 ? TERM_W[t] : 0], x[T > 1 ? TERM_X[t] : 0], acc[j], 0, 0, 0);
+            for (int h = 0; h < 2; ++h) {
+                bf16x8 wh;
+                if constexpr (is8(F))
+                    wh = e4m3x8(make_uint2(r[2 * h], r[2 * h + 1]));
+                else
+                    wh = (bf16x8)w[s][h];
+                const int pc = is8(F) ? 2 * fq + h : 4 * h + fq;
+#pragma unroll
+                for (int j = 0; j < MB; ++j)
+                    acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wh, *(const bf16x8*)(xs + j * 2048 + 16 * (pc ^ turn)), acc[j], 0, 0, 0);
             }
         }
     };
-    // U blocks at a time, the next U's loads in flight while these are worked on: as many as 2 x 88 registers hold
-    constexpr int REGS = (is8(F) ? 4 : 8 * T) + 8 * MB * (F == F32 ? 2 : 1), U = 88 / REGS < 1 ? 1 : 88 / REGS > 4 ? 4 : 88 / REGS;
-    Raw cur[U], nxt[U];
-    int kb = wid;
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-        if (kb + u * NW < nk) load(cur[u], kb + u * NW);
-    for (; kb < nk; kb += U * NW) {
+    for (int s = 0; s < NS - 1; ++s) issue(s, s);
+    int i = 0;
+    for (; i + NS <= count; i += NS) {
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (kb + (U + u) * NW < nk) load(nxt[u], kb + (U + u) * NW);
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (kb + u * NW < nk) mma(cur[u]);
-#pragma unroll
-        for (int u = 0; u < U; ++u) cur[u] = nxt[u];
+        for (int s = 0; s < NS; ++s) {
+            // the slot that is filled next was read in the step before: those reads are done
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            issue(i + s + NS - 1, (s + NS - 1) % NS);
+            wait_vm<(NS - 1) * (C::DX + C::DW)>();
+            mma(s);
+        }
     }
+    wait_vm<0>();
 #pragma unroll
-    for (int j = 0; j < MB; ++j) part[wid][j][lane] = acc[j];
+    for (int s = 0; s < NS - 1; ++s)
+        if (i + s < count) mma(s);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    f32x4* part = (f32x4*)mine;
+#pragma unroll
+    for (int j = 0; j < MB; ++j) part[j * 64 + lane] = acc[j];
     __syncthreads();
     for (int i = threadIdx.x; i < MB * 64; i += 64 * NW) {
         const int j = i / 64;
-        f32x4 v = part[0][j][lane];
+        f32x4 v = *(const f32x4*)(sm + i * 16);
 #pragma unroll
-        for (int w = 1; w < NW; ++w) v += part[w][j][lane];
+        for (int q = 1; q < NW; ++q) v += *(const f32x4*)(sm + q * NS * C::XB + i * 16);
         finish4<fin(F), fout(F)>(o, m0 + 16 * j + fr, n0 + 4 * fq, v);
     }
 }
@@ -550,12 +567,7 @@ hipError_t go_tile(const va_tok_linear_args& a, const Out& o, hipStream_t st) {
     constexpr int lds = C::LDS;
     const int ntn = (a.N + C::BN - 1) / C::BN, ntm = (a.M + C::BM - 1) / C::BM;
     if (!grid_ok(ntn, ntm, 256)) return hipErrorInvalidConfiguration;
-    static DevFlag attr;
-    if (lds > 65536 && !attr()) {
-        const hipError_t e = hipFuncSetAttribute((const void*)linear_tile<F, WN, WM>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-        if (e != hipSuccess) return e;
-        attr() = true;
-    }
+    if (hipError_t e = big_lds<linear_tile<F, WN, WM>, lds>()) return e;
     hipLaunchKernelGGL((linear_tile<F, WN, WM>), dim3((unsigned)(ntn * ntm)), dim3(256), lds, st, a, o, ntn, ntm);
     return hipGetLastError();
 }
@@ -564,7 +576,9 @@ template <Form F, int MB>
 hipError_t go_few(const va_tok_linear_args& a, const Out& o, hipStream_t st) {
     const int ntn = (a.N + 15) / 16, ntm = (a.M + 16 * MB - 1) / (16 * MB);
     if (!grid_ok(ntn, ntm, 512)) return hipErrorInvalidConfiguration;
-    hipLaunchKernelGGL((linear_few<F, MB>), dim3((unsigned)(ntn * ntm)), dim3(512), 0, st, a, o, ntn);
+    constexpr int lds = FewCfg<F, MB>::LDS;
+    if (hipError_t e = big_lds<linear_few<F, MB>, lds>()) return e;
+    hipLaunchKernelGGL((linear_few<F, MB>), dim3((unsigned)(ntn * ntm)), dim3(512), lds, st, a, o, ntn);
     return hipGetLastError();
 }
 
@@ -584,11 +598,13 @@ hipError_t go(const va_tok_linear_args& a, const Out& o, hipStream_t st) {
     const int64_t t64 = (int64_t)((a.N + 63) / 64) * ((a.M + 63) / 64);
     if (a.M <= 16) return go_few<F, 1>(a, o, st);
     if (a.M <= 32) return go_few<F, 2>(a, o, st);
-    // Measured (us, graph replays, K 512-4096; few | 128 x 64 tiles | 256 x 128): bf16 64 tiles of 64 x 64 20.4 | 30.8,
-    // 56: 4.8 | 7.2, 112: 11.1 | 10.3, 256: 17.9 | 10.5; large tiles 100: 16.0 | 23.9, 208: 25.2 | 25.5, 400: 42.0 | 37.4
-    // (e4m3 208: 28.9 | 33.4, 400: 50.1 | 44.5).  Float, few | 64 x 64 | 128 x 64: 56: 8.3 | 13.3, 112: 25.8 | 23.7,
-    // 208: 25.3 | 30.5, 400: 35.3 | 33.5, 832: 74 | 53
-    if (a.M <= 64 || t64 < 100) return go_few<F, 4>(a, o, st);
+    // Measured (us, graph replays, K 1024; few | tiles): 112 tiles of 64 x 64: bf16 8.5 | 10.4, e4m3 8.7 | 16.0, float
+    // 16.2 | 23.3; 128: 8.6 | 10.2, 8.9 | 16.1, 17.3 | 23.4; 208: 15.4 | 10.6, 15.8 | 16.4, 31.1 | 24.7; 256: 16.1 | 10.7,
+    // 16.2 | 16.3, 31.7 | 25.5
+    if (a.M <= 64 || t64 <= (is8(F) ? 256 : 128)) return go_few<F, 4>(a, o, st);
+    // Tiles of 128 x 64 | of 256 x 128, by the number of large ones: bf16 208 25.2 | 25.5, 400 42.0 | 37.4; e4m3 208
+    // 28.9 | 33.4, 400 50.1 | 44.5.  Float, 64 x 64 | 128 x 64 by the number of small ones: 112 23.7 | -, 208 25 | 30.5, 400
+    // 35.3 | 33.5, 832 74 | 53
     if constexpr (F == F32) {
         return t64 < 320 ? go_tile<F32, 1, 1>(a, o, st) : go_tile<F32, 2, 1>(a, o, st);
     } else {
