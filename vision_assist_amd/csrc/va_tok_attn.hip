@@ -163,7 +163,7 @@ __device__ __forceinline__ void mask(f32x16 (&sc)[KB], int from, int to, int lh)
         }
 }
 
-template <int KB, int NV>
+template <typename T, int KB, int NV>
 __device__ __forceinline__ void softmax(Row<NV>& r, f32x16 (&sc)[KB], float c) {
     float nm = -INFINITY;
 #pragma unroll
@@ -188,9 +188,9 @@ __device__ __forceinline__ void softmax(Row<NV>& r, f32x16 (&sc)[KB], float c) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             sc[k][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[k][i], c, off));
-            part[i % 4] += sc[k][i];
+            if constexpr (sizeof(T) == 4) part[i % 4] += sc[k][i];
         }
-    r.sum += (part[0] + part[1]) + (part[2] + part[3]);
+    if constexpr (sizeof(T) == 4) r.sum += (part[0] + part[1]) + (part[2] + part[3]);
 }
 
 // This lane's LDS addresses in a tile's image, formed once: K of row lane & 31, piece 2 c + lh; V for the reads of block v.
@@ -247,17 +247,27 @@ __device__ __forceinline__ void add_values(Row<DV / 32>& r, const f32x16 (&p)[KB
     constexpr int CS = Dims<T, DV>::CS, NV = DV / 32;
     if constexpr (sizeof(T) == 2) {
         Values<T, DQ, DV> cur = first, next;
+        const bf16x2 one = {(__bf16)1.0f, (__bf16)1.0f};
+        float part[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int st = 0; st < 2 * KB; ++st) {
             if (st + 1 < 2 * KB) next.read(ad, vs, st + 1);
             u32x4 pf;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) pf[e] = pk_bf16(p[st / 2][8 * (st & 1) + 2 * e], p[st / 2][8 * (st & 1) + 2 * e + 1]);
+            for (int e = 0; e < 4; ++e) {
+                const f32x16& w = p[st / 2];
+                const int i = 8 * (st & 1) + 2 * e;
+                const bf16x2 two = {(__bf16)w[i], (__bf16)w[i + 1]};
+                pf[e] = __builtin_bit_cast(unsigned, two);
+                part[e & 1] = __builtin_amdgcn_fdot2_f32_bf16(two, one, part[e & 1], false);
+            }
+            asm volatile("" : "+v"(part[0]), "+v"(part[1]));  // (summed here, beside the MFMAs)
 #pragma unroll
             for (int v = 0; v < NV; ++v)
                 r.acc[v] = __builtin_amdgcn_mfma_f32_32x32x16_bf16((bf16x8)cur.f[v], (bf16x8)pf, r.acc[v], 0, 0, 0);
             cur = next;
         }
+        r.sum += part[0] + part[1];
     } else {
         const int lc = lane & 31, lh = lane >> 5;
 #pragma unroll
@@ -485,7 +495,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DV <= 64 ? 3 : 2) : (DV <= 6
             if constexpr (sizeof(T) == 2) v0.read(ad, vs, 0);
             const int from = (sink ? 0 : sp.low) - t0, upto = min(sp.top, end) - t0;
             if (min(f0.top, end) - t0 < KT || (!sink && t0 < f1.low)) mask<KB>(sc, from, upto, lh);  // not all see all
-            softmax<KB, NV>(r, sc, cexp);
+            softmax<T, KB, NV>(r, sc, cexp);
             add_values<T, DQ, DV, KB>(r, sc, v0, ad, vs, lane);
             if (bad_tile[buf] == t) add_nonfinite<T, DV>(r, kinds[buf], from, upto, KT, lh);
         }
@@ -588,7 +598,7 @@ __global__ __launch_bounds__((64 * Split<T, DQ, DV>::SW), 1) void attn_split(va_
         if constexpr (sizeof(T) == 2) v0.read(ad, vs, 0);
         const int from = (sink ? 0 : sp.low) - t0, upto = min(sp.top, end) - t0;
         if (partial) mask<1>(sc, from, upto, lh);
-        softmax<1, NV>(r, sc, cexp);
+        softmax<T, 1, NV>(r, sc, cexp);
         add_values<T, DQ, DV, 1>(r, sc, v0, ad, vs, lane);
         if (bad) add_nonfinite<T, DV>(r, kinds[wid], from, upto, 32, lh);
     }
