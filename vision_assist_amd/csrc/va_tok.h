@@ -44,6 +44,13 @@ __device__ __forceinline__ int xcd_tile(int bid, int ntiles) {
     return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + j;
 }
 
+// the same in runs of C: an XCD takes every eighth run, so that tiles of unequal work spread over the XCDs
+template <int C>
+__device__ __forceinline__ int xcd_runs(int bid, int ntiles) {
+    const int x = bid % 8, j = bid / 8;
+    return bid < ntiles / (8 * C) * (8 * C) ? (j / C * 8 + x) * C + j % C : bid;
+}
+
 // two floats -> packed bf16 (round to nearest even)
 __device__ __forceinline__ unsigned pk_bf16(float a, float b) {
     return __builtin_bit_cast(unsigned, (bf16x2){(__bf16)a, (__bf16)b});

@@ -407,10 +407,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DV <= 64 ? 3 : 2) : (DV <= 6
     __shared__ int bad_tile[2];  // the tile of a buffer, if values were taken out of it
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), lc = lane & 31, lh = lane >> 5;
     const int G = a.Hq / a.Hk;
-    int bid = xcd_tile(blockIdx.x, gridDim.x);
-    const int tile = ntiles - 1 - bid % ntiles;  // the rows that see most first
-    bid /= ntiles;
-    const int hk = bid % a.Hk, b = bid / a.Hk;
+    // four row blocks of a unit (a sequence's key head) are a run on one XCD; those that see most come first
+    constexpr int RUN = 4;
+    const int at = xcd_runs<RUN>(blockIdx.x, gridDim.x), units = a.B * a.Hk, run = at / (units * RUN);
+    const int in = at - run * units * RUN, width = min(RUN, ntiles - run * RUN);
+    const int unit = in / width, tile = ntiles - 1 - (run * RUN + in % width), hk = unit % a.Hk, b = unit / a.Hk;
     const AttnSeq sq = attn_seq(a, b);
     const int rows = sq.ql * G, r0 = tile * 128;
     if (r0 >= rows) return;
@@ -475,6 +476,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DV <= 64 ? 3 : 2) : (DV <= 6
     };
     if (tid < 2) bad_tile[tid] = -1;
     __syncthreads();
+    __builtin_amdgcn_s_setprio(1);
     if (w.nt > 0) {
         fetch(0, 0);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -495,7 +497,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DV <= 64 ? 3 : 2) : (DV <= 6
             if constexpr (sizeof(T) == 2) v0.read(ad, vs, 0);
             const int from = (sink ? 0 : sp.low) - t0, upto = min(sp.top, end) - t0;
             if (min(f0.top, end) - t0 < KT || (!sink && t0 < f1.low)) mask<KB>(sc, from, upto, lh);  // not all see all
+            __builtin_amdgcn_s_setprio(0);  // (beside the other waves' products, which go first)
             softmax<T, KB, NV>(r, sc, cexp);
+            __builtin_amdgcn_s_setprio(1);
             add_values<T, DQ, DV, KB>(r, sc, v0, ad, vs, lane);
             if (bad_tile[buf] == t) add_nonfinite<T, DV>(r, kinds[buf], from, upto, KT, lh);
         }
