@@ -10,7 +10,6 @@
 namespace tok {
 
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
-typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
 typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
 typedef __attribute__((ext_vector_type(2))) float f32x2;
 typedef __attribute__((ext_vector_type(4))) float f32x4;
@@ -18,7 +17,6 @@ typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef __attribute__((ext_vector_type(2))) unsigned int u32x2;
 typedef __attribute__((ext_vector_type(4))) unsigned int u32x4;
 typedef __attribute__((ext_vector_type(4))) short s16x4;
-typedef __attribute__((address_space(1))) void gvoid_t;
 typedef __attribute__((address_space(3))) void lvoid_t;
 
 // the largest side of an operand that the kernels' 32-bit counts take, rounded up to a tile
@@ -68,8 +66,8 @@ __device__ __forceinline__ bf16x8 e4m3x8(uint2 q) {
 }
 
 // x = h + m + l exactly, each the round-to-nearest bf16 of what remains (x - h and x - h - m are exact in float: the
-// remainders have at most 16 and 8 significant bits).  Six of the nine term products (hh, hm, mh, hl, mm, lh) keep a
-// float product to 2^-26 of |a b|: |m| <= 2^-9 |x|, |l| <= 2^-18 |x|.
+// remainders have at most 16 and 8 significant bits).  |m| <= 2^-8 |x| and |l| <= 2^-16 |x|, so the six term products hh, hm,
+// mh, hl, mm, lh leave out ml, lm and ll: together at most 2^-23 + 2^-32 of |a b|.
 __device__ __forceinline__ void split3(const float (&x)[8], bf16x8 (&t)[3]) {
     unsigned w[3][4];
 #pragma unroll

@@ -7,7 +7,14 @@
 // keys may run in any order, so V^T is read in the order in which the scores lie in the registers.
 //   bf16: v_mfma_f32_32x32x16_bf16, V^T by the transposing LDS read (16 lanes x 8 bytes: 4 keys x 16 columns)
 //   f32:  v_mfma_f32_32x32x2_f32 (exact products), V^T by plain 4-byte reads
-// One pass over the keys with the running maximum and sum of the softmax (base 2: the scale is folded with log2 e).
+// One pass over the keys with the running maximum and sum of the softmax (base 2: the scale is folded with log2 e).  A row's
+// running maximum is only raised where a score passes it by more than 8 (in powers of two): its sums stay below 2^8 times
+// the keys, and few tiles rescale.  bf16: the probabilities are rounded to bf16 for the second product (half a step,
+// 2^-8 of each at most), and the sum is of the rounded ones, which is what the product weighs by.
+//
+// What is not finite in a value that no row of a tile's part sees must not meet a probability of 0 in an MFMA: in tiles
+// that some row does not see whole, such values are replaced by 0 as the tile arrives (take_out) and added afterwards by
+// the rows that do see them (add_nonfinite); whole tiles need neither.
 #include <math.h>
 
 #include "va_dev.h"
@@ -386,8 +393,14 @@ struct Walk {
 
 // ------------------------------------------------------------------ many rows: 128 a workgroup, keys through LDS
 // Tiles of KT keys in two LDS buffers: the next tile is on its way into one by LDS-DMA while the other is worked on, and
-// one wait and barrier a tile publish it.  A tile's slots are consecutive (the walk is cut at the ring's end), so its
+// one wait and barrier a tile publish it.  Tiles of 64 keys (bf16) or 32: the scores of twice as many would not fit the
+// registers of three waves a SIMD at D <= 64, of two at 128.  A tile's slots are consecutive (the walk is cut at the ring's end), so its
 // rows are offsets from one address; rows and pieces that are not there take an offset out of range and load zeros.
+// Bound by the instructions between the products: at D = 128 MFMAs and vector instructions (an exp2 of four issue slots,
+// a multiply-add, half a maximum, half a conversion and half a sum for each score) take half of a SIMD's time each, and two
+// waves overlap them in part.  Measured, bf16: 16 heads over 2 key heads, 8192 tokens, window 4096, D 128: 255 us, 809
+// TFLOP/s; 8 streams, 400 queries over 3200 keys, D 128: 118 us, 708 TFLOP/s; two clips of 6400 tokens, frames of 400, D
+// 64: 137 us, 574 TFLOP/s.  Float (32-bit MFMA, 154 TFLOP/s at most): 16 x 8 heads of 400 x 400, D 32, Dv 64: 53 us, 74 TFLOP/s.
 constexpr int TILE_OOB = 0x7ffffff0;
 
 // (a plain function: the host pass drops the stub of a kernel template that names the builtin)
@@ -407,7 +420,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DV <= 64 ? 3 : 2) : (DV <= 6
     __shared__ int bad_tile[2];  // the tile of a buffer, if values were taken out of it
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), lc = lane & 31, lh = lane >> 5;
     const int G = a.Hq / a.Hk;
-    // four row blocks of a unit (a sequence's key head) are a run on one XCD; those that see most come first
+    // Four row blocks of a unit (a sequence's key head) are a run on one XCD, which share its keys in that L2; those that
+    // see most come first, over all units.  (A contiguous eighth for each XCD, unit after unit: 162 us instead of 136 for
+    // two clips, 288 instead of 255 for a long prompt, as the XCDs' shares differ in work.  Runs of 8, 16: the same.)
     constexpr int RUN = 4;
     const int at = xcd_runs<RUN>(blockIdx.x, gridDim.x), units = a.B * a.Hk, run = at / (units * RUN);
     const int in = at - run * units * RUN, width = min(RUN, ntiles - run * RUN);
@@ -519,7 +534,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DV <= 64 ? 3 : 2) : (DV <= 6
 // A workgroup takes 32 rows and one of nsplit shares of their tiles of 32 keys; its waves walk the share's tiles in
 // turn, each through two buffers of its own in LDS and without a barrier, until their sums are joined.  A tile comes by
 // LDS-DMA while the one before is worked on, whole rows at a time (a load covers complete cache lines: reading each key's
-// row by its own lane instead, 32 lines at a time, ran at 1.7 TB/s).
+// row by its own lane instead, 32 lines at a time, ran at 1.7 TB/s).  Bound by the bytes of the keys and values: 32
+// streams over 6800 slots, 8 key heads of 128: 149 us, 4.3 TB/s (a large copy: 4.9).
 // A share's result: [NV * 16][64] registers as they lie in the wave, then the 32 rows' maxima and sums.
 __device__ __forceinline__ int64_t part_floats(int NV) { return NV * 16 * 64 + 64; }
 
