@@ -174,11 +174,13 @@ __device__ __forceinline__ void grouped_tile(int i, int ntn, int ntm, int* tn, i
 // whole step, so its stage is free and the weights of step t + NSW (after a token stage's last step: the tokens two stages
 // on) are sent into it; and the wait before the barrier has retired what step t + 1 needs -- all but what the barrier
 // before sent -- whose fragments are read next.
+// KG = 2: two groups of four waves with rings of their own take the first and the second half of K, and the second's sums
+// are added to the first's through LDS: two waves a SIMD where there is a workgroup for each CU at most.
 // Two workgroups of 256 x 128 share a CU: the epilogue of one (activations: VALU, stores) runs beside the MFMAs of the
 // other.  (One workgroup of 256 x 256 a CU: slower for want of that; deeper rings: no faster, and one workgroup a CU.)
 // Bound by the MFMAs and the issue around them: 8192^3 in bf16 1198 TFLOP/s (the library's product: 1548); 25600 x 1024 x
 // 4096 with bias and GELU 249 us, 863 TFLOP/s, of which the GELU is some 60 us of vector instructions that the MFMAs of the
-// other workgroup cover in part; float 1603 x 520 x 1000 19.5 us, where 208 workgroups leave each SIMD one wave.
+// other workgroup cover in part; float 1603 x 520 x 1000 with a residual 18.4 us: 208 workgroups, two waves a SIMD.
 constexpr int LIN_OOB = 0x7ffffff0;      // an offset that a descriptor of that many bytes answers with zeros
 constexpr int LIN_ROW = 1 << 21;         // longest rows in values: the offsets of 256 of them stay within 31 bits
 
@@ -193,20 +195,19 @@ __device__ __forceinline__ void wait_vm() {
 
 // eight consecutive channels of a token, through every type and alignment
 template <bool FIN, bool FOUT>
-__device__ __forceinline__ void finish8(const Out& o, int m, int n, float (&r)[8], const float (&scale)[8], const float (&bias)[8]) {
+__device__ __forceinline__ void finish8(const Out& o, int m, int n, float (&r)[8], const float (&scale)[8], const float (&bias)[8],
+                                        const u32x4 (&res)[FIN ? 2 : 1]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) r[i] = __builtin_fmaf(r[i], scale[i], bias[i]);
     activate_n<FOUT>(r, o.act);
     if (o.vec == 2 && n + 7 < o.N) {
         if (o.res) {
-            if (FIN) {
-                const f32x4* q = (const f32x4*)((const float*)o.res + (int64_t)m * o.ldr + n);
+            if constexpr (FIN) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) r[i] += q[i / 4][i % 4];
+                for (int i = 0; i < 8; ++i) r[i] += __uint_as_float(res[i / 4][i % 4]);
             } else {
-                const u32x4 q = *(const u32x4*)((const __bf16*)o.res + (int64_t)m * o.ldr + n);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) r[2 * e] += bf_lo(q[e]), r[2 * e + 1] += bf_hi(q[e]);
+                for (int e = 0; e < 4; ++e) r[2 * e] += bf_lo(res[0][e]), r[2 * e + 1] += bf_hi(res[0][e]);
             }
         }
         if (FOUT) {
@@ -260,17 +261,31 @@ __device__ __forceinline__ void store_tile(const Out& o, const f32x16 (&acc)[WN]
             for (int e = 0; e < 16; e += 4)
                 *(f32x4*)(es + lc * EROW + (32 * i + 16 * lh + e) * 4) =
                     (f32x4){acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]};
-#pragma unroll 2
-        for (int it = 0; it < 32 / RI; ++it) {
-            const int row = it * RI + er, mr = m + 32 * j + row;
-            const f32x4 u = *(const f32x4*)(es + row * EROW + ec * 4), v = *(const f32x4*)(es + row * EROW + ec * 4 + 16);
-            float r[8] = {u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
-            if (mr < o.M && n + ec < o.N) finish8<fin(FF), fout(FF)>(o, mr, n + ec, r, scale, bias);
+        // the residuals of U iterations are on their way before the first store: res may be y, so no load passes a store
+        constexpr int U = 32 / RI < 4 ? 32 / RI : 4, NR = fin(FF) ? 2 : 1;
+#pragma unroll 1
+        for (int it = 0; it < 32 / RI; it += U) {
+            u32x4 res[U][NR];
+            if (o.res && o.vec == 2 && n + ec + 7 < o.N) {
+#pragma unroll
+                for (int t = 0; t < U; ++t) {
+                    const int64_t at = (int64_t)min(m + 32 * j + (it + t) * RI + er, o.M - 1) * o.ldr + n + ec;
+#pragma unroll
+                    for (int q = 0; q < NR; ++q) res[t][q] = *(const u32x4*)((const unsigned char*)o.res + at * (fin(FF) ? 4 : 2) + 16 * q);
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < U; ++t) {
+                const int row = (it + t) * RI + er, mr = m + 32 * j + row;
+                const f32x4 u = *(const f32x4*)(es + row * EROW + ec * 4), v = *(const f32x4*)(es + row * EROW + ec * 4 + 16);
+                float r[8] = {u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
+                if (mr < o.M && n + ec < o.N) finish8<fin(FF), fout(FF)>(o, mr, n + ec, r, scale, bias, res[t]);
+            }
         }
     }
 }
 
-template <Form F, int WN, int WM>
+template <Form F, int WN, int WM, int KG>
 struct TileCfg {
     static constexpr int BN = 64 * WN, BM = 64 * WM, T = F == F32 ? 3 : 1;
     static constexpr int WROW = is8(F) ? 32 : 64, XP = F == F32 ? 1 : 2;        // bytes of a weight row; steps of a token stage
@@ -278,32 +293,35 @@ struct TileCfg {
     static constexpr int NSW = 3 * WB + (F == F32 ? 3 : 2) * XB <= 80 * 1024 ? 3 : 2, NSX = F == F32 ? NSW : 2;
     static constexpr int DW = WB / 4096, DX = XB / 4096;                        // DMAs of a wave
     static constexpr int EROW = (32 * WN + 4) * 4, EPI = 4 * 32 * EROW;         // the epilogue's blocks (store_tile)
-    static constexpr int RING = NSW * WB + NSX * XB, LDS = RING > EPI ? RING : EPI;
-    static_assert(WB % 4096 == 0 && XB % 4096 == 0 && WPL % 1024 == 0 && LDS <= 80 * 1024, "two workgroups a CU");
+    static constexpr int RING = NSW * WB + NSX * XB, LDS = KG * (RING > EPI ? RING : EPI);
+    static_assert(WB % 4096 == 0 && XB % 4096 == 0 && WPL % 1024 == 0 && LDS <= KG * 80 * 1024, "eight waves a CU");
+    static_assert(KG == 1 || 4 * WN * WM * 16 * 64 * 4 <= LDS / 2, "");
 };
 
-template <Form F, int WN, int WM>
-__global__ __launch_bounds__(256, 2) void linear_tile(va_tok_linear_args a, Out o, int ntn, int ntm) {
-    using C = TileCfg<F, WN, WM>;
+template <Form F, int WN, int WM, int KG>
+__global__ __launch_bounds__((256 * KG), 2) void linear_tile(va_tok_linear_args a, Out o, int ntn, int ntm) {
+    using C = TileCfg<F, WN, WM, KG>;
     constexpr int T = C::T, XE = F == F32 ? 4 : 2;
-    extern __shared__ __align__(16) unsigned char sm[];  // [NSW] weights, [NSX] tokens
+    extern __shared__ __align__(16) unsigned char lds[];  // [KG]: [NSW] weights, [NSX] tokens
     int tn, tm;
     grouped_tile<8>(xcd_tile(blockIdx.x, gridDim.x), ntn, ntm, &tn, &tm);
     const int n0 = tn * C::BN, m0 = tm * C::BM;
-    const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lc = lane & 31, lh = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), grp = wave >> 2, wid = wave & 3, lane = threadIdx.x & 63, lc = lane & 31, lh = lane >> 5;
     const int wn = wid & 1, wm = wid >> 1;
-    const int nk = 2 * ((a.K + 63) / 64);
+    const int nk = 2 * ((a.K + 63) / 64), nl = KG == 1 ? nk : 2 * ((nk / 2 + KG - 1) / KG), k0 = grp * nl;  // steps: all, a group's, from
+    unsigned char* sm = lds + grp * (C::LDS / KG);
     // weights: DMA d of a stage's plane copies its bytes [1024 d, 1024 d + 1024); blocks from channel Npad on are not there
     const unsigned char* wb = (const unsigned char*)a.w + (int64_t)(n0 / 32) * 32 * C::WROW;
     const int64_t wstep = (int64_t)a.Npad * C::WROW, plane = wstep * (a.Kpad / 32);
     const int wend = min(a.Npad - n0, C::BN) * C::WROW;
     auto issue_w = [&](int t) {
         unsigned char* to = sm + t % C::NSW * C::WB;
-        const unsigned char* from = wb + min(t, nk - 1) * wstep;
+        const unsigned char* from = wb + min(t + k0, nk - 1) * wstep;
+        const bool on = t < nl && t + k0 < nk;
 #pragma unroll
         for (int j = 0; j < C::DW; ++j) {
             const int d = (wid * C::DW + j) * 1024, in = d % C::WPL;  // uniform
-            dma16(from + (T > 1 ? d / C::WPL * plane : 0), to + d, t < nk && in < wend ? lane * 16 : LIN_OOB, in);
+            dma16(from + (T > 1 ? d / C::WPL * plane : 0), to + d, on && in < wend ? lane * 16 : LIN_OOB, in);
         }
     };
     // tokens: DMA j takes rows 8 (wid DX + j) .. + 7, lane l row l / 8, place l % 8: piece place ^ (row / 2 % 8), so rows of
@@ -315,10 +333,11 @@ __global__ __launch_bounds__(256, 2) void linear_tile(va_tok_linear_args a, Out 
     const int xoff[2] = {(int)(xrow * a.ldx) * XE + 16 * piece, (int)(xrow * a.ldx) * XE + 16 * (piece ^ 4)};
     auto issue_x = [&](int st) {
         unsigned char* to = sm + C::NSW * C::WB + st % C::NSX * C::XB + wid * C::DX * 1024;
-        const bool in[2] = {st * (128 / XE) + piece * (16 / XE) < a.K, st * (128 / XE) + (piece ^ 4) * (16 / XE) < a.K};
+        const int g = st + k0 / C::XP;
+        const bool in[2] = {g * (128 / XE) + piece * (16 / XE) < a.K, g * (128 / XE) + (piece ^ 4) * (16 / XE) < a.K};
 #pragma unroll
         for (int j = 0; j < C::DX; ++j)
-            dma16(xb, to + j * 1024, in[j & 1] && 8 * j < xmore ? xoff[j & 1] : LIN_OOB, (int)(8 * j * a.ldx) * XE + st * 128);
+            dma16(xb, to + j * 1024, in[j & 1] && 8 * j < xmore ? xoff[j & 1] : LIN_OOB, (int)(8 * j * a.ldx) * XE + g * 128);
     };
     f32x16 acc[WN][WM];
 #pragma unroll
@@ -409,7 +428,7 @@ __global__ __launch_bounds__(256, 2) void linear_tile(va_tok_linear_args a, Out 
     Frag f0, f1;
     read(f0, 0, 0);
     split(f0);
-    for (int t2 = 0; t2 < nk; t2 += 2) {
+    for (int t2 = 0; t2 < nl; t2 += 2) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const int t = t2 + u;
@@ -430,6 +449,31 @@ __global__ __launch_bounds__(256, 2) void linear_tile(va_tok_linear_args a, Out 
     }
     wait_vm<0>();
     __syncthreads();
+    if constexpr (KG == 2) {  // the second group's sums into the first's
+        f32x4* part = (f32x4*)(lds + C::LDS / 2) + wid * WN * WM * 4 * 64 + lane;
+        if (grp) {
+#pragma unroll
+            for (int i = 0; i < WN; ++i)
+#pragma unroll
+                for (int j = 0; j < WM; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        part[((i * WM + j) * 4 + e) * 64] =
+                            (f32x4){acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]};
+        }
+        __syncthreads();
+        if (grp) return;
+#pragma unroll
+        for (int i = 0; i < WN; ++i)
+#pragma unroll
+            for (int j = 0; j < WM; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const f32x4 v = part[((i * WM + j) * 4 + e) * 64];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) acc[i][j][4 * e + q] += v[q];
+                }
+    }
     store_tile<F, WN, WM>(o, acc, sm + wid * 32 * C::EROW, m0 + 32 * wm * WM, n0 + 32 * wn * WN, lane);
 }
 
@@ -569,14 +613,14 @@ bool linear_ok(const va_tok_linear_args& a) {
 }  // namespace
 
 namespace {
-template <Form F, int WN, int WM>
+template <Form F, int WN, int WM, int KG>
 hipError_t go_tile(const va_tok_linear_args& a, const Out& o, hipStream_t st) {
-    using C = TileCfg<F, WN, WM>;
+    using C = TileCfg<F, WN, WM, KG>;
     constexpr int lds = C::LDS;
     const int ntn = (a.N + C::BN - 1) / C::BN, ntm = (a.M + C::BM - 1) / C::BM;
-    if (!grid_ok(ntn, ntm, 256)) return hipErrorInvalidConfiguration;
-    if (hipError_t e = big_lds<linear_tile<F, WN, WM>, lds>()) return e;
-    hipLaunchKernelGGL((linear_tile<F, WN, WM>), dim3((unsigned)(ntn * ntm)), dim3(256), lds, st, a, o, ntn, ntm);
+    if (!grid_ok(ntn, ntm, 256 * KG)) return hipErrorInvalidConfiguration;
+    if (hipError_t e = big_lds<linear_tile<F, WN, WM, KG>, lds>()) return e;
+    hipLaunchKernelGGL((linear_tile<F, WN, WM, KG>), dim3((unsigned)(ntn * ntm)), dim3(256 * KG), lds, st, a, o, ntn, ntm);
     return hipGetLastError();
 }
 
@@ -611,14 +655,17 @@ hipError_t go(const va_tok_linear_args& a, const Out& o, hipStream_t st) {
     // 16.2 | 16.3, 31.7 | 25.5
     if (a.M <= 64 || t64 <= (is8(F) ? 256 : 128)) return go_few<F, 4>(a, o, st);
     // Tiles of 128 x 64 | of 256 x 128, by the number of large ones: bf16 208 25.2 | 25.5, 400 42.0 | 37.4; e4m3 208
-    // 28.9 | 33.4, 400 50.1 | 44.5.  Float, 64 x 64 | 128 x 64 by the number of small ones: 112 23.7 | -, 208 25 | 30.5, 400
-    // 35.3 | 33.5, 832 74 | 53
-    if constexpr (F == F32) {
-        return t64 < 320 ? go_tile<F32, 1, 1>(a, o, st) : go_tile<F32, 2, 1>(a, o, st);
-    } else {
+    // 28.9 | 33.4, 400 50.1 | 44.5.
+    // Up to 256 tiles of 128 x 64, a workgroup a CU: one group of four waves | K halved between two, by the number of 64 x 64
+    // (K 1024): float 256 24.3 | 23.5, 400 30.9 | 26.5, 448 31.7 | 27.8, 832 51.9 | 56.4; e4m3 400 16.6 |
+    // 13.1, 448 16.6 | 13.1, 800 19.2 | 19.0; bf16, whose steps are short, 400 11.1 | 10.6, at K 520 8.2 | 8.5: one group.
+    if constexpr (F != F32) {
         const int64_t big = (int64_t)((a.N + 255) / 256) * ((a.M + 127) / 128);
-        return big >= (is8(F) ? 320 : 224) ? go_tile<F, 4, 2>(a, o, st) : go_tile<F, 2, 1>(a, o, st);
+        if (big >= (is8(F) ? 320 : 224)) return go_tile<F, 4, 2, 1>(a, o, st);
     }
+    if constexpr (F == F32 || is8(F))
+        if (t64 <= 512) return go_tile<F, 2, 1, 2>(a, o, st);
+    return go_tile<F, 2, 1, 1>(a, o, st);
 }
 }  // namespace
 
