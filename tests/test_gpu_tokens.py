@@ -680,3 +680,13 @@ def test_linear_offsets_behind_31_bits(M, K):
         assert torch.equal(y[:, n], x[:, i]), f"channel {n}"
     y[:, at] = 0
     assert not y.any()
+
+
+@pytest.mark.parametrize("S", [1, 5, 300])
+def test_attend_keys_that_sequences_share(S):
+    """Keys and values expanded over the sequences (stride 0) are those of copies."""
+    from vision_assist_amd.tokens import attend
+    g = torch.Generator().manual_seed(S)
+    q, k, v = (rnd(g, *s, dtype=torch.bfloat16).cuda() for s in ((3, S, 4, 64), (1, 700, 2, 64), (1, 700, 2, 64)))
+    shared = attend(q, k.expand(3, -1, -1, -1), v.expand(3, -1, -1, -1))
+    assert torch.equal(shared, attend(q, k.repeat(3, 1, 1, 1), v.repeat(3, 1, 1, 1)))
