@@ -9,8 +9,12 @@
 //   f32:  v_mfma_f32_32x32x2_f32 (exact products), V^T by plain 4-byte reads
 // One pass over the keys with the running maximum and sum of the softmax (base 2: the scale is folded with log2 e).  A row's
 // running maximum is only raised where a score passes it by more than 8 (in powers of two): its sums stay below 2^8 times
-// the keys, and few tiles rescale.  bf16: the probabilities are rounded to bf16 for the second product (half a step,
-// 2^-8 of each at most), and the sum is of the rounded ones, which is what the product weighs by.
+// the keys, and few tiles rescale.  bf16, many rows: the probabilities are rounded to bf16 for the second product (half a
+// step, 2^-8 of each at most), and the sum is of the rounded ones, which is what the product weighs by.  Few rows (single
+// tokens over a cache) are bound by the cache's bytes, so there a probability enters as two bf16 terms (2^-16 of it is left
+// out) and the sum is of the floats: 1 % of the time (161.1 us against 159.4 for 32 streams over 6800 slots), and the error
+// against float64 is the output's own rounding (0.0017 instead of 0.0023, relative L2).  For many rows the second term's
+// MFMAs and conversions were 23 to 27 % of the time (116 -> 143 us, 136 -> 168, 254 -> 324).
 //
 // What is not finite in a value that no row of a tile's part sees must not meet a probability of 0 in an MFMA: in tiles
 // that some row does not see whole, such values are replaced by 0 as the tile arrives (take_out) and added afterwards by
@@ -170,7 +174,8 @@ __device__ __forceinline__ void mask(f32x16 (&sc)[KB], int from, int to, int lh)
         }
 }
 
-template <typename T, int KB, int NV>
+// (FSUM: the sum is formed here, of the floats)
+template <typename T, int KB, int NV, bool FSUM>
 __device__ __forceinline__ void softmax(Row<NV>& r, f32x16 (&sc)[KB], float c) {
     float nm = -INFINITY;
 #pragma unroll
@@ -195,9 +200,9 @@ __device__ __forceinline__ void softmax(Row<NV>& r, f32x16 (&sc)[KB], float c) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             sc[k][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[k][i], c, off));
-            if constexpr (sizeof(T) == 4) part[i % 4] += sc[k][i];
+            if constexpr (FSUM) part[i % 4] += sc[k][i];
         }
-    if constexpr (sizeof(T) == 4) r.sum += (part[0] + part[1]) + (part[2] + part[3]);
+    if constexpr (FSUM) r.sum += (part[0] + part[1]) + (part[2] + part[3]);
 }
 
 // This lane's LDS addresses in a tile's image, formed once: K of row lane & 31, piece 2 c + lh; V for the reads of block v.
@@ -247,8 +252,8 @@ struct Values {
 };
 
 // O^T += V^T P^T over the KB blocks of 32 keys of a tile; bf16: first = step 0's values, read before the softmax, and each
-// step's are read beside the MFMAs of the step before
-template <typename T, int DQ, int DV, int KB>
+// step's are read beside the MFMAs of the step before; TWO: the probabilities as two bf16 terms, else their rounded sum too
+template <typename T, int DQ, int DV, int KB, bool TWO>
 __device__ __forceinline__ void add_values(Row<DV / 32>& r, const f32x16 (&p)[KB], const Values<T, DQ, DV>& first,
                                            const Addr<T, DQ, DV>& ad, const unsigned char* vs, int lane) {
     constexpr int CS = Dims<T, DV>::CS, NV = DV / 32;
@@ -259,22 +264,30 @@ __device__ __forceinline__ void add_values(Row<DV / 32>& r, const f32x16 (&p)[KB
 #pragma unroll
         for (int st = 0; st < 2 * KB; ++st) {
             if (st + 1 < 2 * KB) next.read(ad, vs, st + 1);
-            u32x4 pf;
+            u32x4 pf, pl;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const f32x16& w = p[st / 2];
                 const int i = 8 * (st & 1) + 2 * e;
                 const bf16x2 two = {(__bf16)w[i], (__bf16)w[i + 1]};
                 pf[e] = __builtin_bit_cast(unsigned, two);
-                part[e & 1] = __builtin_amdgcn_fdot2_f32_bf16(two, one, part[e & 1], false);
+                if constexpr (TWO)
+                    pl[e] = pk_bf16(w[i] - bf_lo(pf[e]), w[i + 1] - bf_hi(pf[e]));
+                else
+                    part[e & 1] = __builtin_amdgcn_fdot2_f32_bf16(two, one, part[e & 1], false);
             }
-            asm volatile("" : "+v"(part[0]), "+v"(part[1]));  // (summed here, beside the MFMAs)
+            if constexpr (!TWO) asm volatile("" : "+v"(part[0]), "+v"(part[1]));  // (summed here, beside the MFMAs)
 #pragma unroll
             for (int v = 0; v < NV; ++v)
                 r.acc[v] = __builtin_amdgcn_mfma_f32_32x32x16_bf16((bf16x8)cur.f[v], (bf16x8)pf, r.acc[v], 0, 0, 0);
+            if constexpr (TWO) {
+#pragma unroll
+                for (int v = 0; v < NV; ++v)
+                    r.acc[v] = __builtin_amdgcn_mfma_f32_32x32x16_bf16((bf16x8)cur.f[v], (bf16x8)pl, r.acc[v], 0, 0, 0);
+            }
             cur = next;
         }
-        r.sum += part[0] + part[1];
+        if constexpr (!TWO) r.sum += part[0] + part[1];
     } else {
         const int lc = lane & 31, lh = lane >> 5;
 #pragma unroll
@@ -513,9 +526,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DV <= 64 ? 3 : 2) : (DV <= 6
             const int from = (sink ? 0 : sp.low) - t0, upto = min(sp.top, end) - t0;
             if (min(f0.top, end) - t0 < KT || (!sink && t0 < f1.low)) mask<KB>(sc, from, upto, lh);  // not all see all
             __builtin_amdgcn_s_setprio(0);  // (beside the other waves' products, which go first)
-            softmax<T, KB, NV>(r, sc, cexp);
+            softmax<T, KB, NV, sizeof(T) == 4>(r, sc, cexp);
             __builtin_amdgcn_s_setprio(1);
-            add_values<T, DQ, DV, KB>(r, sc, v0, ad, vs, lane);
+            add_values<T, DQ, DV, KB, false>(r, sc, v0, ad, vs, lane);
             if (bad_tile[buf] == t) add_nonfinite<T, DV>(r, kinds[buf], from, upto, KT, lh);
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -618,8 +631,8 @@ __global__ __launch_bounds__((64 * Split<T, DQ, DV>::SW), 1) void attn_split(va_
         if constexpr (sizeof(T) == 2) v0.read(ad, vs, 0);
         const int from = (sink ? 0 : sp.low) - t0, upto = min(sp.top, end) - t0;
         if (partial) mask<1>(sc, from, upto, lh);
-        softmax<T, 1, NV>(r, sc, cexp);
-        add_values<T, DQ, DV, 1>(r, sc, v0, ad, vs, lane);
+        softmax<T, 1, NV, true>(r, sc, cexp);
+        add_values<T, DQ, DV, 1, true>(r, sc, v0, ad, vs, lane);
         if (bad) add_nonfinite<T, DV>(r, kinds[wid], from, upto, 32, lh);
     }
     // the upper half of the waves into the lower, until one is left
