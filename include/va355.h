@@ -563,8 +563,8 @@ typedef struct va_tok_linear_args {
                                holds its row 16 (r / 4 % 2) + 4 (r / 8) + r % 4, whose columns 8 p .. 8 p + 7 stand in
                                place p ^ (r / 4 % 4) of its four (w8: p ^ (r / 8 % 4)).  BF16: bf16;  w8 = 1 (BF16): e4m3 bytes;  F32: bf16 [3] such arrays,
                                the weights' exact terms h, m, l (w = h + m + l, each the round-to-nearest bf16 of what
-                               remains): six exact term products each, float sums, for values below bf16's largest in
-                               size */
+                               remains; a weight from 0x1.ffp127 on has the largest bf16 for h, an infinity is +-1, 0,
+                               +-inf): six exact term products each, float sums */
     const float* wscale;    /* w8: [Npad] scale of each row, else NULL */
     const float* bias;      /* [N] or NULL */
     const void* res;        /* [M][N] dtype, rows ldr elements apart, or NULL */

@@ -28,3 +28,63 @@ def test_attend_few_rows_round_once(B, S, Hq, Hk, D, slots, kv):
     size, _ = attend_ref(q.float(), k, v.abs(), *args)
     tol = tol + 2.0 ** -16 * size + U[t] * want.abs()
     assert float(((got - want).abs() / tol).max()) <= 1
+
+
+# ------------------------------------------------------------------ Linear
+# the float forms: rows few enough to split K over waves, unaligned rows, tiles with K halved between two groups, tiles
+F32_FORMS = [(1, 200, 96), (40, 264, 160), (70, 131, 130), (1300, 264, 576), (2112, 136, 1024)]
+
+
+@pytest.mark.parametrize("M,K,N", F32_FORMS)
+def test_linear_f32_infinities_and_the_largest_values(M, K, N):
+    """What the definition gives: an infinity's row is infinities of the weights' signs (NaN at a weight of 0), and values
+    beyond bf16's largest are values like others.  Those rows' bound is that of test_gpu_tokens.py: (K + 8) 2^-24 sum |x w|."""
+    from vision_assist_amd.tokens import Linear
+    g = torch.Generator().manual_seed(M)
+    big = torch.finfo(torch.float32).max
+    w = rnd(g, N, K, by=K ** -0.5)
+    w[3, K - 1] = 0.0
+    lin = Linear(w, dtype="f32", device="cuda")
+    x = rnd(g, M, K)
+    clean = lin(x.cuda()).cpu()
+    plus, minus, both, large, nan = (i * M // 5 for i in range(5)) if M > 4 else (0,) * 5
+
+    def row(at, i, value):
+        y = x.clone()
+        for j, v in zip(i, value):
+            y[at, j] = v
+        got = lin(y.cuda()).cpu()
+        rest = torch.arange(M) != at
+        assert torch.equal(got[rest], clean[rest])
+        return got[at].double()
+
+    s = torch.sign(w[:, K - 1].double())
+    want = torch.where(s == 0, math.nan, s * math.inf)
+    assert torch.equal(row(plus, [K - 1], [math.inf]).nan_to_num(7.0), want.nan_to_num(7.0))
+    assert torch.equal(row(minus, [K - 1], [-math.inf]).nan_to_num(7.0), (-want).nan_to_num(7.0))
+    s0 = torch.sign(w[:, 0].double())
+    two = torch.where((s == s0) & (s != 0), s * math.inf, math.nan)
+    assert torch.equal(row(both, [0, K - 1], [math.inf, math.inf]).nan_to_num(7.0), two.nan_to_num(7.0))
+    assert row(nan, [K // 2], [math.nan]).isnan().all()
+    got = row(large, [K - 1], [big])
+    y = x.double()[large].clone()
+    y[K - 1] = big
+    cols = w[:, K - 1].abs() <= 0.2  # (sums that stay within the range)
+    mag = y.abs() @ w.double().abs().t()
+    ref = y @ w.double().t()
+    tol = (K + 8) * 2.0 ** -24 * mag + 2.0 ** -24 * ref.abs()
+    assert cols.any() and bool(((got - ref).abs() <= tol)[cols].all())
+
+
+@pytest.mark.parametrize("M,K,N", F32_FORMS)
+def test_linear_f32_infinite_weights(M, K, N):
+    from vision_assist_amd.tokens import Linear
+    g = torch.Generator().manual_seed(N)
+    w = rnd(g, N, K)
+    w[5, 2], w[9, K - 1] = math.inf, -math.inf
+    x = rnd(g, M, K)
+    x[0, 2], x[M // 2, K - 1] = 0.0, math.inf
+    got = Linear(w, dtype="f32", device="cuda")(x.cuda()).double().cpu()
+    ref = x.double() @ w.double().t()
+    assert torch.equal(got.isnan(), ref.isnan()) and torch.equal(got.isinf(), ref.isinf())
+    assert torch.equal(got[got.isinf()], ref[ref.isinf()])

@@ -67,7 +67,9 @@ __device__ __forceinline__ bf16x8 e4m3x8(uint2 q) {
 
 // x = h + m + l exactly, each the round-to-nearest bf16 of what remains (x - h and x - h - m are exact in float: the
 // remainders have at most 16 and 8 significant bits).  |m| <= 2^-8 |x| and |l| <= 2^-16 |x|, so the six term products hh, hm,
-// mh, hl, mm, lh leave out ml, lm and ll: together at most 2^-23 + 2^-32 of |a b|.
+// mh, hl, mm, lh leave out ml, lm and ll: together at most 2^-23 + 2^-32 of |a b|.  A value whose h would be an infinity (an
+// infinity, or from 0x1.ffp127 on) has a NaN for l here, which makes a NaN of every sum that it enters: who finds one forms
+// its sums once more with split3_far.
 __device__ __forceinline__ void split3(const float (&x)[8], bf16x8 (&t)[3]) {
     unsigned w[3][4];
 #pragma unroll
@@ -81,6 +83,21 @@ __device__ __forceinline__ void split3(const float (&x)[8], bf16x8 (&t)[3]) {
     }
 #pragma unroll
     for (int k = 0; k < 3; ++k) t[k] = __builtin_bit_cast(bf16x8, (u32x4){w[k][0], w[k][1], w[k][2], w[k][3]});
+}
+
+// The same for any value.  Beyond bf16's largest, h is that largest one and the remainder is split on.  An infinity is
+// (+-1, 0, +-inf): l meets the other factor's h alone, whose sign is the factor's and which is 0 only where the factor is, and
+// two infinities meet each other's +-1, so products and their sums are the infinities and NaNs that they have to be.
+__device__ __forceinline__ void split3_far(const float (&x)[8], bf16x8 (&t)[3]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float a = x[e];
+        const bool inf = __builtin_isinf(a), far = fabsf(a) >= 0x1.ffp127f;
+        const __bf16 h = (__bf16)(far ? copysignf(inf ? 1.0f : 0x1.fep127f, a) : a);
+        const float r = inf ? 0.0f : a - (float)h;
+        const __bf16 m = (__bf16)r;
+        t[0][e] = h, t[1][e] = m, t[2][e] = (__bf16)(inf ? a : r - (float)m);
+    }
 }
 
 // x Phi(x) = x erfc(-x / sqrt 2) / 2 (the erfc form keeps the left tail's relative accuracy); the tanh form as

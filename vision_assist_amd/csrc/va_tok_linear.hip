@@ -7,6 +7,8 @@
 // three left out come to 2^-23 of a product's size at most -- so a product runs on the bf16 MFMA at a sixth of its rate, 215 TFLOP/s
 // by the bf16 product measured here, where the 32-bit MFMA reaches 154.  e4m3 weights: every e4m3 value is a bf16 value; the
 // row's scale is applied to the sum.
+#include <type_traits>
+
 #include "va_dev.h"
 #include "va_tok.h"
 
@@ -94,7 +96,11 @@ __global__ __launch_bounds__(256) void linear_any(va_tok_linear_args a, Out o, i
     const int wn = wid & 1, wm = wid >> 1;
     const int row = tid >> 2, kq = tid & 3;  // this thread's staged row and 8-value chunk
     const int m = m0 + row;
-    f32x4 acc[2][2] = {};
+    f32x4 acc[2][2];
+    bool far = false;
+again:
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i / 2][i % 2] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
     for (int k0 = 0; k0 < a.Kpad; k0 += GK) {
         const int k = k0 + 8 * kq;
         bf16x8 wt[T], xt[T];
@@ -112,7 +118,10 @@ __global__ __launch_bounds__(256) void linear_any(va_tok_linear_args a, Out o, i
             const float* p = (const float*)a.x + (int64_t)m * a.ldx + k;
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] = m < a.M && k + e < a.K ? p[e] : 0.0f;
-            split3(x, xt);
+            if (far)
+                split3_far(x, xt);
+            else
+                split3(x, xt);
         } else {
             const __bf16* p = (const __bf16*)a.x + (int64_t)m * a.ldx + k;
             if (xvec && m < a.M && k + 8 <= a.K) {
@@ -146,6 +155,11 @@ __global__ __launch_bounds__(256) void linear_any(va_tok_linear_args a, Out o, i
                 for (int j = 0; j < 2; ++j)
                     acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw[TA[t]][i], fx[TB[t]][j], acc[i][j], 0, 0, 0);
     }
+    if constexpr (FF == F32)  // (as in the tiles below: NaN where split3 does not take a value)
+        if (!far && __syncthreads_or(acc[0][0][0] != acc[0][0][0] || acc[0][1][0] != acc[0][1][0])) {
+            far = true;
+            goto again;
+        }
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -176,6 +190,9 @@ __device__ __forceinline__ void grouped_tile(int i, int ntn, int ntm, int* tn, i
 // before sent -- whose fragments are read next.
 // KG = 2: two groups of four waves with rings of their own take the first and the second half of K, and the second's sums
 // are added to the first's through LDS: two waves a SIMD where there is a workgroup for each CU at most.
+// Float: a value that split3 does not take leaves NaN in its token's sums, all channels of them (0 x NaN too), so one sum of
+// each token is looked at, and the tile is formed once more with split3_far if it is one, by a loop of its own (a test of
+// every split value was 4 to 5 % of the time, split3_far in the loop itself 0 to 6 %).
 // Two workgroups of 256 x 128 share a CU: the epilogue of one (activations: VALU, stores) runs beside the MFMAs of the
 // other.  (One workgroup of 256 x 256 a CU: slower for want of that; deeper rings: no faster, and one workgroup a CU.)
 // Bound by the MFMAs and the issue around them: 8192^3 in bf16 1198 TFLOP/s (the library's product: 1548); 25600 x 1024 x
@@ -340,13 +357,14 @@ __global__ __launch_bounds__((256 * KG), 2) void linear_tile(va_tok_linear_args 
             dma16(xb, to + j * 1024, in[j & 1] && 8 * j < xmore ? xoff[j & 1] : LIN_OOB, (int)(8 * j * a.ldx) * XE + g * 128);
     };
     f32x16 acc[WN][WM];
+    auto clear = [&]() {
 #pragma unroll
-    for (int i = 0; i < WN; ++i)
+        for (int i = 0; i < WN; ++i)
 #pragma unroll
-        for (int j = 0; j < WM; ++j)
+            for (int j = 0; j < WM; ++j)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
-
+                for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+    };
     struct Frag {
         bf16x8 w[WN][T], x[WM][T];
         f32x4 raw[F == F32 ? WM : 1][2];
@@ -414,6 +432,7 @@ __global__ __launch_bounds__((256 * KG), 2) void linear_tile(va_tok_linear_args 
             mma(f);
         }
     };
+    clear();
     // in the order in which the steps need them; past the last step they run on, on offsets out of range
     issue_x(0);
     issue_w(0);
@@ -448,7 +467,42 @@ __global__ __launch_bounds__((256 * KG), 2) void linear_tile(va_tok_linear_args 
         }
     }
     wait_vm<0>();
-    __syncthreads();
+    if constexpr (F == F32) {
+        __shared__ int nans[4 * KG];
+        bool nan = false;
+#pragma unroll
+        for (int j = 0; j < WM; ++j) nan |= acc[0][j][0] != acc[0][j][0];
+        nan = __any(nan);
+        if (lane == 0) nans[wave] = nan;
+        __syncthreads();
+        bool far = false;
+#pragma unroll
+        for (int i = 0; i < 4 * KG; ++i) far |= nans[i] != 0;
+        if (far) {  // (the whole workgroup, step by step)
+            clear();
+#pragma unroll 1
+            for (int t = 0; t < nl; ++t) {
+                issue_w(t);
+                issue_x(t);
+                wait_vm<0>();
+                __syncthreads();
+#pragma unroll 1
+                for (int ks = 0; ks < 2; ++ks) {
+                    read(f0, t, ks);
+#pragma unroll
+                    for (int j = 0; j < WM; ++j) {
+                        const f32x4 u = f0.raw[j][0], v = f0.raw[j][1];
+                        const float e[8] = {u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
+                        split3_far(e, f0.x[j]);
+                    }
+                    mma(f0);
+                }
+                __syncthreads();
+            }
+        }
+    } else {
+        __syncthreads();
+    }
     if constexpr (KG == 2) {  // the second group's sums into the first's
         f32x4* part = (f32x4*)(lds + C::LDS / 2) + wid * WN * WM * 4 * 64 + lane;
         if (grp) {
@@ -504,8 +558,10 @@ __global__ __launch_bounds__(512) void linear_few(va_tok_linear_args a, Out o, i
     const int64_t wrow = (n0 / 32) * 32 + row_of((n0 & 16) + fr);                // this lane's weight row among a step's
     unsigned char* mine = sm + wid * NS * C::XB;
     f32x4 acc[MB];
+    auto clear = [&]() {
 #pragma unroll
-    for (int j = 0; j < MB; ++j) acc[j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+        for (int j = 0; j < MB; ++j) acc[j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+    };
     u32x4 w[NS][C::DW];
     // DMA j takes rows 8 j .. 8 j + 7, lane l row l / 8, place l % 8: piece place ^ (row / 2 % 8)
     const int l8 = lane >> 3, piece = (lane & 7) ^ (l8 >> 1), xmore = a.M - m0 - l8;
@@ -535,7 +591,7 @@ __global__ __launch_bounds__(512) void linear_few(va_tok_linear_args a, Out o, i
                   (int)(8 * j * a.ldx) * XE + min(kb, nk) * 128);
     };
     const int turn = (fr >> 1) & 7;
-    auto mma = [&](int s) {
+    auto mma = [&](int s, auto far) {  // (far: with split3_far)
         const unsigned char* xs = mine + s * C::XB + fr * 128;
         if constexpr (F == F32) {
 #pragma unroll
@@ -544,7 +600,10 @@ __global__ __launch_bounds__(512) void linear_few(va_tok_linear_args a, Out o, i
                 const f32x4 v = *(const f32x4*)(xs + j * 2048 + 16 * ((2 * fq + 1) ^ turn));
                 const float e[8] = {u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
                 bf16x8 x[T];
-                split3(e, x);
+                if constexpr (decltype(far)::value)
+                    split3_far(e, x);
+                else
+                    split3(e, x);
 #pragma unroll
                 for (int t = 0; t < NTERM; ++t)
                     acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16((bf16x8)w[s][TERM_W[t]], x[TERM_X[t]], acc[j], 0, 0, 0);
@@ -566,6 +625,7 @@ __global__ __launch_bounds__(512) void linear_few(va_tok_linear_args a, Out o, i
             }
         }
     };
+    clear();
 #pragma unroll
     for (int s = 0; s < NS - 1; ++s) issue(s, s);
     int i = 0;
@@ -576,14 +636,29 @@ __global__ __launch_bounds__(512) void linear_few(va_tok_linear_args a, Out o, i
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             issue(i + s + NS - 1, (s + NS - 1) % NS);
             wait_vm<(NS - 1) * (C::DX + C::DW)>();
-            mma(s);
+            mma(s, std::false_type());
         }
     }
     wait_vm<0>();
 #pragma unroll
     for (int s = 0; s < NS - 1; ++s)
-        if (i + s < count) mma(s);
+        if (i + s < count) mma(s, std::false_type());
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if constexpr (F == F32) {  // (as in the tiles: NaN where split3 does not take a value)
+        bool nan = false;
+#pragma unroll
+        for (int j = 0; j < MB; ++j) nan |= acc[j][0] != acc[j][0];
+        if (__any(nan)) {
+            clear();
+#pragma unroll 1
+            for (i = 0; i < count; ++i) {
+                issue(i, 0);
+                wait_vm<0>();
+                mma(0, std::true_type());
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            }
+        }
+    }
     f32x4* part = (f32x4*)mine;
 #pragma unroll
     for (int j = 0; j < MB; ++j) part[j * 64 + lane] = acc[j];

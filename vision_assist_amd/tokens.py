@@ -175,6 +175,17 @@ def _blocks(w: torch.Tensor) -> torch.Tensor:
     return b[:, :, ch].gather(3, col.reshape(32, 32).expand(b.shape)).contiguous()
 
 
+def _terms(w: torch.Tensor) -> torch.Tensor:
+    """[N, K] float -> its bf16 terms h, m, l [3, N, K], of any value (va355.h va_tok_linear_args.w)."""
+    h, m, l = split3_bf16(w).permute(2, 0, 1, 3).reshape(3, *w.shape)
+    far, inf = w.abs() >= float.fromhex("0x1.ffp127"), w.isinf()
+    h = torch.where(far, torch.where(inf, 1.0, torch.finfo(torch.bfloat16).max).copysign(w).to(h.dtype), h)
+    r = torch.where(far, w - h.float(), 0.0)
+    m = torch.where(inf, 0.0, torch.where(far, r.to(h.dtype), m))
+    l = torch.where(far, torch.where(inf, w, r - m.float()).to(h.dtype), l)
+    return torch.stack([h, m, l])
+
+
 class Linear:
     """y = act(x w^T + bias) + residual, the weights packed once.
 
@@ -224,7 +235,7 @@ class Linear:
             self._wscale[:N] = scale.detach().to(self.device, torch.float32)
             self._w = _blocks(padded(w.view(torch.uint8)))
         elif dtype == "f32":
-            self._w = torch.stack([_blocks(t) for t in split3_bf16(padded(w.float())).permute(2, 0, 1, 3).reshape(3, Np, Kp)])
+            self._w = torch.stack([_blocks(t) for t in _terms(padded(w.float()))])
         else:
             self._w = _blocks(padded(w.to(torch.bfloat16)))
         self._bias = None if bias is None else bias.detach().to(self.device, torch.float32).contiguous()
