@@ -609,7 +609,9 @@ int va_tok_qk(void* stream, const va_tok_qk_args* a);
  * or j >= e - window (window 0: no limit): frame 1 is causal attention token by token, frame = tokens of an image lets
  * the tokens of one image see each other.  Position j is held in slot j (j < sinks) or sinks + (j - sinks) %
  * (slots - sinks); positions that later ones have overwritten are not seen.  A query that sees nothing gets zeros; for
- * s >= q_len[b] nothing is written.  A key that a query does not see has no part in its result, whatever it holds.
+ * s >= q_len[b] nothing is written.  A key that a query does not see has no part in its result, whatever it holds;
+ * a value that is not finite makes its column of every query that sees it an infinity of its sign, or NaN beside NaN or the
+ * other infinity, however small the probability.
  * out = softmax(scale q k) v; when dtype is BF16 and a key head has more than 32 rows of queries (S * Hq / Hk), the
  * probabilities are rounded to bf16 for the second product (else they enter it as two bf16 terms).
  * ws: va_tok_attn_workspace_bytes(a) bytes, written and read within the call only (calls that may run at the same time

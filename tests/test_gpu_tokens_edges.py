@@ -30,6 +30,44 @@ def test_attend_few_rows_round_once(B, S, Hq, Hk, D, slots, kv):
     assert float(((got - want).abs() / tol).max()) <= 1
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("S,Hk,slots,frame,window,sinks,kv", [(1, 2, 3000, 1, 0, 0, 3000), (1, 1, 500, 1, 200, 5, 1900), (5, 2, 200, 1, 0, 0, 200),
+                                                              (200, 2, 200, 1, 0, 0, 200), (260, 1, 260, 20, 80, 9, 260),
+                                                              (70, 2, 400, 1, 250, 3, 1111), (150, 1, 150, 0, 0, 0, 150)])
+def test_attend_infinite_values_whatever_their_probability(dtype, S, Hk, slots, frame, window, sinks, kv):
+    """Scores of some hundreds, so that most probabilities come out 0: a seen infinity is an infinity all the same, NaN and
+    both infinities are NaN, wherever tiles begin; other columns and rows are those of the call without them, bit by bit."""
+    from tests.test_gpu_tokens import visible
+    from vision_assist_amd.tokens import attend
+    g = torch.Generator().manual_seed(S)
+    t, B, D = DT[dtype], 2, 64
+    q, k, v = rnd(g, B, S, 2 * Hk, D, dtype=t, by=60.0), rnd(g, B, slots, Hk, D, dtype=t), rnd(g, B, slots, Hk, D, dtype=t)
+    lens = torch.tensor([kv, kv - 9], dtype=torch.int32, device="cuda")
+    call = lambda v: attend(q.cuda(), k.cuda(), v.cuda(), frame=frame, window=window, sinks=sinks, kv_len=lens).cpu().double()
+    clean = call(v)
+    spots = torch.randperm(slots, generator=g)[:8].tolist()
+    put = [(3, math.inf, spots[0]), (4, -math.inf, spots[1]), (5, math.inf, spots[2]), (5, -math.inf, spots[3]), (6, math.nan, spots[4]),
+           (40, math.inf, spots[5]), (63, -math.inf, spots[6]), (63, -math.inf, spots[7])]
+    bad = v.clone()
+    for col, x, slot in put:
+        bad[:, slot, :, col] = x
+    want = clean.clone()
+    for b, n in enumerate(lens.tolist()):
+        see = visible(S, slots, frame, window, sinks, S, n)
+        for col in {c for c, _, _ in put}:
+            hit = [torch.zeros(S, dtype=torch.bool) for _ in range(2)]
+            for c, x, slot in put:
+                if c == col:
+                    for i, sign in enumerate((1, -1)):
+                        if math.isnan(x) or x * sign > 0:
+                            hit[i] |= see[:, slot]
+            for rows, x in ((hit[0] & ~hit[1], math.inf), (hit[1] & ~hit[0], -math.inf), (hit[0] & hit[1], math.nan)):
+                want[b, rows, :, col] = x
+    got = call(bad)
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(0.5, math.inf, -math.inf), want.nan_to_num(0.5, math.inf, -math.inf))
+    assert not want.isfinite().all()
+
+
 # ------------------------------------------------------------------ Linear
 # the float forms: rows few enough to split K over waves, unaligned rows, tiles with K halved between two groups, tiles
 F32_FORMS = [(1, 200, 96), (40, 264, 160), (70, 131, 130), (1300, 264, 576), (2112, 136, 1024)]

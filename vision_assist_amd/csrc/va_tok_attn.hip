@@ -18,7 +18,9 @@
 //
 // What is not finite in a value that no row of a tile's part sees must not meet a probability of 0 in an MFMA: in tiles
 // that some row does not see whole, such values are replaced by 0 as the tile arrives (take_out) and added afterwards by
-// the rows that do see them (add_nonfinite); whole tiles need neither.
+// the rows that do see them (add_nonfinite); whole tiles need neither.  Every probability of a seen key is positive, so what a
+// row sees of a column alone says which infinity it is or that it is NaN; but a probability, or the factor that rescales a
+// sum, may come out 0, and 0 x inf is NaN.  Results that are not finite are therefore settled by the column's values (settle).
 #include <math.h>
 
 #include "va_dev.h"
@@ -356,6 +358,49 @@ __device__ __forceinline__ void add_nonfinite(Row<DV / 32>& r, const unsigned sh
     }
 }
 
+// What is not finite in a row's NB blocks of columns from block v0 on is what the values that it sees make it: an infinity,
+// or NaN where it sees both or a NaN; not where the scores made the row NaN (sum), nor where finite values passed the range.
+template <typename T, int NB>
+__device__ __forceinline__ void settle(const va_tok_attn_args& a, f32x16 (&x)[NB], float sum, const T* vb, Span sp, int v0, int lh) {
+    float z = 0.0f;
+#pragma unroll
+    for (int v = 0; v < NB; ++v)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) z = __builtin_fmaf(x[v][i], 0.0f, z);
+    if (__builtin_expect(z == z || sum != sum, 1)) return;
+    unsigned plus[NB], minus[NB];
+#pragma unroll
+    for (int v = 0; v < NB; ++v) plus[v] = minus[v] = 0;
+#pragma unroll 1
+    for (int part = 0; part < 2; ++part) {
+        const int end = part ? sp.top : min(a.sinks, sp.top);
+#pragma unroll 1
+        for (int p = part ? sp.low : 0; p < end; ++p) {
+            const T* row = vb + (int64_t)slot_of(a, p) * a.v_ss;
+#pragma unroll
+            for (int v = 0; v < NB; ++v)
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    const int d = 32 * (v0 + v) + key_of(i, lh);
+                    if (d >= a.Dv) continue;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float y = (float)row[d + e];
+                        plus[v] |= (unsigned)!(y < INFINITY) << (i + e);  // (NaN: both)
+                        minus[v] |= (unsigned)!(y > -INFINITY) << (i + e);
+                    }
+                }
+        }
+    }
+#pragma unroll
+    for (int v = 0; v < NB; ++v)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const bool p = plus[v] >> i & 1, m = minus[v] >> i & 1;
+            x[v][i] = p && m ? NAN : p ? INFINITY : m ? -INFINITY : x[v][i];
+        }
+}
+
 // 16 registers of block v -> columns 32 v + key_of(i, lh) of this lane's row
 template <typename T>
 __device__ __forceinline__ void store_block(T* op, const f32x16& x, float by, int v, int lh, int Dv) {
@@ -537,6 +582,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DV <= 64 ? 3 : 2) : (DV <= 6
     }
     const float total = r.sum + __shfl_xor(r.sum, 32);
     if (!there) return;
+    settle<T, NV>(a, r.acc, total, vb, sp, 0, lh);
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
     T* op = (T*)a.o + b * a.o_sb + s * a.o_ss + (int64_t)(hk * G + g) * a.o_sh;
 #pragma unroll
@@ -666,6 +712,7 @@ __global__ __launch_bounds__((64 * Split<T, DQ, DV>::SW), 1) void attn_split(va_
     }
     if (wid || !there) return;
     if (nsplit == 1) {
+        settle<T, NV>(a, r.acc, r.sum, vb, sp, 0, lh);
         const float inv = r.sum == 0.0f ? 0.0f : 1.0f / r.sum;
         T* op = (T*)a.o + b * a.o_sb + s * a.o_ss + (int64_t)(hk * G + g) * a.o_sh;
 #pragma unroll
@@ -698,18 +745,19 @@ __global__ __launch_bounds__(64 * (DV / 32)) void attn_join(va_tok_attn_args a, 
     for (int i = 0; i < nsplit; ++i) mx = fmaxf(mx, ws[i * part_floats(NV) + NV * 16 * 64 + lc]);
     const float base = mx == -INFINITY ? 0.0f : mx;
     float sum = 0.0f;
-    f32x16 acc;
+    f32x16 acc[1];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) acc[j] = 0.0f;
+    for (int j = 0; j < 16; ++j) acc[0][j] = 0.0f;
     for (int i = 0; i < nsplit; ++i) {
         const float* p = ws + i * part_floats(NV);
         const float y = __builtin_amdgcn_exp2f((p[NV * 16 * 64 + lc] - base) * cexp);
         sum += p[NV * 16 * 64 + 32 + lc] * y;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) acc[j] += p[(v * 16 + j) * 64 + lane] * y;
+        for (int j = 0; j < 16; ++j) acc[0][j] += p[(v * 16 + j) * 64 + lane] * y;
     }
+    settle<T, 1>(a, acc, sum, (const T*)a.v + b * a.v_sb + hk * a.v_sh, attn_span(a, sq, sq.first + s), v, lh);
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    store_block<T>((T*)a.o + b * a.o_sb + s * a.o_ss + (int64_t)(hk * G + g) * a.o_sh, acc, inv, v, lh, a.Dv);
+    store_block<T>((T*)a.o + b * a.o_sb + s * a.o_ss + (int64_t)(hk * G + g) * a.o_sh, acc[0], inv, v, lh, a.Dv);
 }
 
 constexpr int64_t ROW_MAX = 1 << 22;  // elements between slots: a tile's offsets stay within 31 bits

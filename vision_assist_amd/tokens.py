@@ -568,7 +568,8 @@ def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float | 
     (with window = sinks = 0) lets every token see every token.  With kv_len[b] > slots the tensors are rings behind
     their first ``sinks`` slots (TokenCache), and overwritten positions are not seen: for S queries over a window to see
     all of it, slots >= sinks + window + S - 1.  A query that sees nothing gets zeros; rows s >= q_len[b] of out are left
-    as they were (zeros where the call makes it).  scale: D ** -0.5 by default, positive.  D and Dv: multiples of 8 up
+    as they were (zeros where the call makes it).  A value that is not finite makes its column of the queries that see it an
+    infinity of its sign, or NaN beside NaN or the other infinity, and has no part in others.  scale: D ** -0.5 by default, positive.  D and Dv: multiples of 8 up
     to 128."""
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
         raise _lib.VaError("q [B, S, Hq, D], k [B, slots, Hk, D], v [B, slots, Hk, Dv]")
