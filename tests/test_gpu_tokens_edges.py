@@ -126,3 +126,20 @@ def test_linear_f32_infinite_weights(M, K, N):
     ref = x.double() @ w.double().t()
     assert torch.equal(got.isnan(), ref.isnan()) and torch.equal(got.isinf(), ref.isinf())
     assert torch.equal(got[got.isinf()], ref[ref.isinf()])
+
+
+def test_layers_refuse_to_lose_a_gradient():
+    from vision_assist_amd import _lib
+    from vision_assist_amd.tokens import Linear, QKNorm, TokenCache
+    lin, norm = Linear(torch.nn.Parameter(torch.randn(64, 64)), device="cuda"), QKNorm(64, device="cuda")
+    t = lambda grad: torch.randn(2, 3, 4, 64, device="cuda", dtype=torch.bfloat16, requires_grad=grad)
+    cache = TokenCache(2, 8, 4, 64).advance(3)
+    x, y = t(True), t(False)
+    calls = [lambda: lin(x), lambda: lin(y, residual=x), lambda: norm(x, y), lambda: norm(y, x), lambda: norm.store(x, y, y, None, cache),
+             lambda: norm.store(y, x, y, None, cache), lambda: norm.store(y, y, x, None, cache)]
+    for call in calls:
+        with pytest.raises(_lib.VaError, match="gradient"):
+            call()
+        with torch.no_grad():
+            call()
+    assert not lin(y).requires_grad

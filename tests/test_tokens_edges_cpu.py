@@ -20,3 +20,14 @@ def test_terms_of_any_weight():
     t = _terms(w).float()
     assert t[:, 0, 0].tolist() == [1, 0, math.inf] and t[:, 0, 1].tolist() == [-1, 0, -math.inf] and t[:, 0, 2].isnan().any()
     assert torch.equal(t[:, :, 3:].double().sum(0), w[:, 3:].double())
+
+
+def test_attend_refuses_to_lose_a_gradient():
+    from vision_assist_amd.tokens import attend
+    for i in range(3):
+        a = [torch.zeros(2, 3, 4, 64), torch.zeros(2, 10, 2, 64), torch.zeros(2, 10, 2, 64)]
+        a[i].requires_grad_()
+        with pytest.raises(_lib.VaError, match="gradient"):
+            attend(*a)
+        with torch.no_grad(), pytest.raises(_lib.VaError, match="on the GPU"):
+            attend(*a)

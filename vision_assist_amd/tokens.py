@@ -10,7 +10,8 @@ the current stream of the tensors' device, or on ``stream``; it does not synchro
 be captured into a graph.  Results are the same from call to call, bit by bit.  With ``stream``, what the call allocates
 belongs to that stream, its inputs are recorded on it, and the caller orders it against the work that made them.
 
-The operators are forward only, as every layer of this package.
+The operators are forward only, as every layer of this package: a tensor that requires a gradient is refused while
+gradients are recorded (weights are copied when a layer is made, and may require one).
 """
 from __future__ import annotations
 
@@ -72,6 +73,15 @@ def _on(t: torch.Tensor, dev: torch.device, dtype, name: str) -> None:
         raise _lib.VaError(f"{name} is on {t.device}, not on {dev}")
     if t.dtype != dtype:
         raise _lib.VaError(f"{name} is {t.dtype}, not {dtype}")
+    if t.requires_grad:
+        _no_grad(name)
+
+
+def _no_grad(name: str) -> None:
+    """Refuses a tensor that requires a gradient where one would be recorded: the result would be cut off from it."""
+    if torch.is_grad_enabled():
+        raise _lib.VaError(f"{name} requires a gradient, and the token operators are forward only: detach() it, or call under "
+                           "torch.no_grad()")
 
 
 def _range(t: torch.Tensor) -> tuple[int, int]:
@@ -596,6 +606,7 @@ def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float | 
     dev, dtype = q.device, q.dtype
     if dtype not in DTYPES:
         raise _lib.VaError(f"q is {dtype}: bfloat16 or float32")
+    _on(q, dev, dtype, "q")
     _on(k, dev, dtype, "k")
     _on(v, dev, dtype, "v")
     if q_len is not None:
