@@ -31,3 +31,26 @@ def test_attend_refuses_to_lose_a_gradient():
             attend(*a)
         with torch.no_grad(), pytest.raises(_lib.VaError, match="on the GPU"):
             attend(*a)
+
+
+@pytest.mark.parametrize("slots,sinks,frame", [(300, 4, 1), (2804, 4, 400), (1000, 0, 0), (77, 76, 25)])
+def test_rebase_sets_large_counts_back_by_rings_and_frames(slots, sinks, frame):
+    from vision_assist_amd.tokens import TokenCache
+    n = [0, 5, slots, 2 ** 30 - 1, 2 ** 30, 2 ** 30 + 12345678, 2 ** 31 - 1]
+    k = torch.zeros(len(n), slots, 1, 8)
+    c = TokenCache.of(k, k.clone(), sinks=sinks, length=torch.tensor(n, dtype=torch.int32))
+    at = c.len.data_ptr()
+    turn = math.lcm(slots - sinks, frame or 1)
+    got = c.rebase(frame).len.tolist()
+    assert c.len.data_ptr() == at and got[:5] == n[:5]
+    assert all((a - b) % turn == 0 and 2 ** 30 <= a < 2 ** 30 + turn for a, b in zip(got[4:], n[4:]))
+    assert c.rebase(frame).len.tolist() == got
+
+
+def test_rebase_refuses():
+    from vision_assist_amd.tokens import TokenCache
+    k = torch.zeros(1, 1009, 1, 8)
+    c = TokenCache.of(k, k.clone())
+    for frame in (-1, 2 ** 20 + 7):
+        with pytest.raises(_lib.VaError):
+            c.rebase(frame)

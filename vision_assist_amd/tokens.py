@@ -356,7 +356,8 @@ class TokenCache:
     """Keys and values of the last tokens of B streams, and of their first ``sinks`` tokens.
 
     k [B, slots, heads, D], v [B, slots, heads, Dv], len [B] (int32, on the device): tokens seen so far.  Position p is
-    kept in slot p while p < slots; later ones take the slots behind the sinks in turn."""
+    kept in slot p while p < slots; later ones take the slots behind the sinks in turn.  (attend reads heads of multiples of
+    8 up to 128 values; QKNorm fills others too.)"""
 
     k, v, sinks, len = _fixed("k"), _fixed("v"), _fixed("sinks"), _fixed("len")
 
@@ -394,8 +395,21 @@ class TokenCache:
         return c
 
     def advance(self, n) -> "TokenCache":
-        """n (an int, or int32 [B] on the device) more tokens of each stream: before they are stored."""
+        """n (an int, or int32 [B] on the device) more tokens of each stream: before they are stored.  The counts are 32 bits
+        and end at 2^31 - 1: a stream that may get there (12 hours of 1600 tokens a frame, 30 frames a second) calls rebase
+        now and then."""
         self._len += n
+        return self
+
+    def rebase(self, frame: int = 1) -> "TokenCache":
+        """Sets counts from 2^30 on back by a whole number of rings and of ``frame`` (attend's) tokens, which changes no
+        result: a ring's slots and what a query sees depend on differences of positions alone.  Others stay.  Called at
+        least every 2^29 tokens (each frame is fine: it works on the device, and may be captured) a stream never ends.
+        The positions of a rotation are the caller's own."""
+        turn = math.lcm(self.slots - self.sinks, max(int(frame), 1))
+        _need(frame >= 0 and turn <= 1 << 29 and self.slots <= 1 << 29,
+              f"frame {frame}: its common multiple with the ring of {self.slots - self.sinks} slots is beyond 2^29")
+        self._len -= torch.div((self._len - (1 << 30)).clamp_(min=0), turn, rounding_mode="floor") * turn
         return self
 
 
