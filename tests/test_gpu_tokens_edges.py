@@ -192,3 +192,23 @@ def test_a_stream_goes_on_past_32_bits(dtype, S, slots, sinks, frame, window):
         assert torch.equal(y, want), i
     assert int(old.len.max()) < 2 ** 31 - 1 and far + steps * S > 2 ** 31
     assert torch.equal(old.k, young.k) and torch.equal(replayed.v, young.v) and torch.equal(old.len, replayed.len)
+
+
+# ------------------------------------------------------------------ QKNorm
+@pytest.mark.parametrize("S,D", [(3000, 64), (1, 64), (500, 66)])
+def test_angles_keep_floats_accuracy(S, D):
+    """Pairs (1, 0) without a norm: the result is the cosine and the sine.  Half steps relative to them: two for each of
+    the sine's or cosine's evaluation (two units in the last place), one of the sum; and the angle's float64 roundings, two
+    here (frequency and product) and two in the reference: 4 x 2^-53 of it."""
+    from vision_assist_amd.tokens import QKNorm, Rotary
+    g = torch.Generator().manual_seed(D)
+    n = D // 2
+    x = torch.zeros(1, S, 1, D)
+    x[..., 0::2] = 1.0
+    pos = torch.randint(0, 1 << 20, (1, S), generator=g, dtype=torch.int32)
+    q, _ = QKNorm(D, Rotary(D, layout="pairs", device="cuda"), device="cuda")(x.cuda(), x.cuda(), pos.cuda())
+    th = pos.double()[0, :, None] * torch.tensor([10000.0 ** (-2 * i / D) for i in range(n)], dtype=torch.float64)
+    got = q[0, :, 0].double().cpu()
+    for part, want in ((got[:, 0::2], torch.cos(th)), (got[:, 1::2], torch.sin(th))):
+        tol = 5 * 2.0 ** -24 * want.abs() + 4 * 2.0 ** -53 * th
+        assert float(((part - want).abs() / (tol + 1e-300)).max()) <= 1

@@ -52,15 +52,20 @@ __device__ __forceinline__ int kept_slot(const va_tok_qk_args& a, int b, int s) 
     return p < a.sinks ? (int)p : a.sinks + ((int)p - a.sinks) % ring;
 }
 
-// cos and sin of the token's angles: whole turns are dropped in float64, so a position of 2^24 keeps 2^-29 of a turn
+// cos and sin of the token's angles: whole turns are dropped in float64, so a position of 2^24 keeps 2^-29 of a turn; what
+// the rest loses as a float (up to 2^-26 of a turn, l in radians) is added to first order for float tensors, which leaves
+// 2^-48
+template <typename T>
 __device__ __forceinline__ void angles(const va_tok_qk_args& a, int b, int s, int lane, float (&cs)[2][QK_PAIRS]) {
     const int32_t* pos = a.pos + b * a.pos_sb + s * a.pos_ss;
     for (int f = lane; f < a.rot / 2; f += 64) {
-        const double t = a.turns[f] * (double)pos[a.axis[f]];
+        double t = a.turns[f] * (double)pos[a.axis[f]];
+        t -= rint(t);
+        const float h = (float)t, l = sizeof(T) == 4 ? 6.2831853f * (float)(t - (double)h) : 0.0f;
         float sn, c;
-        sincospif(2.0f * (float)(t - rint(t)), &sn, &c);
-        cs[0][f] = c;
-        cs[1][f] = sn;
+        sincospif(2.0f * h, &sn, &c);
+        cs[0][f] = sizeof(T) == 4 ? c - l * sn : c;
+        cs[1][f] = sizeof(T) == 4 ? sn + l * c : sn;
     }
 }
 
@@ -73,7 +78,7 @@ __global__ __launch_bounds__(64 * QK_WAVES) void qk_any(va_tok_qk_args a) {
     const int b = (int)(tok / a.S), s = (int)(tok - (int64_t)b * a.S);
     if (b >= a.B || (a.q_len && s >= a.q_len[b])) return;  // (whole waves, and no barrier follows)
     const int slot = a.slots ? kept_slot(a, b, s) : s;
-    angles(a, b, s, lane, cs[wid]);
+    angles<T>(a, b, s, lane, cs[wid]);
     const int npair = (a.D + 1) / 2;
     const float inv_d = 1.0f / (float)a.D;
     int lo[2], hi[2];
@@ -167,7 +172,7 @@ __global__ __launch_bounds__(64 * QK_WAVES) void qk_wide(va_tok_qk_args a, int l
             for (int p = 0; p < P; ++p) w[k][0][p] = g[lo + (L ? 2 * p : p)], w[k][1][p] = g[hi + (L ? 2 * p : p)];
         }
     }
-    angles(a, b, s, lane, cs[wid]);  // (a wave's LDS operations run in order: its own reads need no barrier)
+    angles<T>(a, b, s, lane, cs[wid]);  // (a wave's LDS operations run in order: its own reads need no barrier)
     float c[P], n[P];
 #pragma unroll
     for (int p = 0; p < P; ++p) {
