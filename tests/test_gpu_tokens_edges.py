@@ -212,3 +212,20 @@ def test_angles_keep_floats_accuracy(S, D):
     for part, want in ((got[:, 0::2], torch.cos(th)), (got[:, 1::2], torch.sin(th))):
         tol = 5 * 2.0 ** -24 * want.abs() + 4 * 2.0 ** -53 * th
         assert float(((part - want).abs() / (tol + 1e-300)).max()) <= 1
+
+
+@pytest.mark.parametrize("K", [1, 8])
+def test_gelu_keeps_its_left_tail(K):
+    """bf16: every value from -12 to -2^-7, the activation alone.  The tail's fit is 2.8e-5 of it off, hardware reciprocal,
+    exponential and their arguments (x^2 / 2 up to 72) some 2e-5: 2^-14 together, and the result's half step."""
+    from vision_assist_amd.tokens import Linear
+    bits = torch.arange(0x10000, dtype=torch.int32).to(torch.int16)
+    x = bits.view(torch.bfloat16)
+    x = x[(x >= -12) & (x <= -2.0 ** -7)]
+    w = torch.zeros(1, K)
+    w[0, 0] = 1
+    rows = torch.zeros(len(x), K, dtype=torch.bfloat16)
+    rows[:, 0] = x
+    got = Linear(w, act="gelu", device="cuda")(rows.cuda())[:, 0].double().cpu()
+    want = 0.5 * x.double() * torch.erfc(x.double() * -(0.5 ** 0.5))
+    assert float(((got - want).abs() / ((2.0 ** -8 + 2.0 ** -14) * want.abs())).max()) <= 1
