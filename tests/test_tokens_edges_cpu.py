@@ -54,3 +54,27 @@ def test_rebase_refuses():
     for frame in (-1, 2 ** 20 + 7):
         with pytest.raises(_lib.VaError):
             c.rebase(frame)
+
+
+def layer(N=6, K=4, dtype=torch.bfloat16):
+    """A Linear without weights on the CPU: what its calls check comes before they are read."""
+    from vision_assist_amd.tokens import Linear
+    lin = Linear.__new__(Linear)
+    lin.device, lin.N, lin.K, lin.tdtype = torch.device("cpu"), N, K, dtype
+    lin._ptrs, lin._ints = (4096, 0, 0), (N, K, 64, 64, 1, 0, 0)
+    return lin
+
+
+def test_args_of_an_op_list_are_checked():
+    lin, z = layer(), lambda *s, dtype=torch.bfloat16: torch.zeros(s, dtype=dtype)
+    x, y = z(5, 4), z(5, 6)
+    a = lin.args(x, y, residual=y)
+    assert (a.M, a.N, a.K, a.ldx, a.ldy, a.ldr, a.x, a.y, a.res) == (5, 6, 4, 4, 6, 6, x.data_ptr(), y.data_ptr(), y.data_ptr())
+    wide = z(5, 20)
+    assert lin.args(wide[:, 3:7], wide[:, 10:16]).ldx == 20 and lin.args(x, z(5, 6, dtype=torch.float32)).out_f32 == 1
+    for bad in ((z(5, 3), y), (z(2, 5, 4), y), (z(4, 5).t(), y), (z(1, 4).expand(5, 4), y), (z(5, 4, dtype=torch.float32), y), (x, z(5, 5)),
+                (x, z(4, 6)), (x, z(6, 5).t()), (x, z(5, 6, dtype=torch.float16)), (wide[:, 2:6], wide[:, 4:10]),
+                (x, y, z(5, 5)), (x, y, z(5, 6, dtype=torch.float32)), (x, y, z(1, 6).expand(5, 6)), (x, wide[:, :6], wide[:, 1:7]),
+                (x, z(1, 6).expand(5, 6))):
+        with pytest.raises(_lib.VaError):
+            lin.args(*bad)

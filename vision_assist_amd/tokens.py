@@ -255,7 +255,16 @@ class Linear:
 
     def args(self, x: torch.Tensor, out: torch.Tensor, residual: torch.Tensor | None = None) -> LinearArgs:
         """The va_tok_linear_args of a call on [M, K] rows (for an op list: VA_OP_TOK_LINEAR); they point into these
-        tensors, which the caller keeps."""
+        tensors and this layer's weights, which the caller keeps."""
+        _need(x.dim() == 2 and x.shape[1] == self.K and x.shape[0] <= I32_MAX, f"x {tuple(x.shape)}: [M, {self.K}]")
+        _on(x, self.device, self.tdtype, "x")
+        want = (x.shape[0], self.N)
+        if residual is not None:
+            _on(residual, self.device, self.tdtype, "residual")
+            _need(residual.shape == want, f"residual {tuple(residual.shape)}: {want}")
+        for t, n, what in ((x, self.K, "x"), (residual, self.N, "residual")):
+            _need(t is None or self._rows(t, n) is t, f"{what}: rows apart from each other, of contiguous values")
+        out = self._given(out, want, x, residual)
         return LinearArgs.from_buffer_copy(self._pack(x, out, residual))
 
     def _pack(self, x, out, residual) -> bytes:
