@@ -229,3 +229,16 @@ def test_gelu_keeps_its_left_tail(K):
     got = Linear(w, act="gelu", device="cuda")(rows.cuda())[:, 0].double().cpu()
     want = 0.5 * x.double() * torch.erfc(x.double() * -(0.5 ** 0.5))
     assert float(((got - want).abs() / ((2.0 ** -8 + 2.0 ** -14) * want.abs())).max()) <= 1
+
+
+def test_layers_are_made_on_a_gpu():
+    from vision_assist_amd import _lib
+    from vision_assist_amd.tokens import Linear, QKNorm, Rotary, TokenCache
+    for make in (lambda d: Linear(torch.zeros(8, 8), device=d), lambda d: Rotary(8, device=d), lambda d: QKNorm(8, device=d),
+                 lambda d: TokenCache(1, 4, 1, 8, device=d)):
+        with pytest.raises(_lib.VaError, match="device cpu"):
+            make("cpu")
+    here = torch.device("cuda", torch.cuda.current_device())
+    for d in (None, "cuda", here):
+        assert Linear(torch.zeros(8, 8), device=d).device == QKNorm(8, Rotary(8, device=d), device=d).device == here
+        assert TokenCache(1, 4, 1, 8, device=d).k.device == here

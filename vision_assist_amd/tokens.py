@@ -84,6 +84,13 @@ def _no_grad(name: str) -> None:
                            "torch.no_grad()")
 
 
+def _gpu(device) -> torch.device:
+    """The GPU that a layer is made on (None: the current one)."""
+    d = torch.device("cuda" if device is None else device)
+    _need(d.type == "cuda", f"device {d}: the token operators run on the GPU")
+    return d if d.index is not None else torch.device("cuda", torch.cuda.current_device())
+
+
 def _range(t: torch.Tensor) -> tuple[int, int]:
     """The bytes between a tensor's first and last element (0, 0: it has none)."""
     if t.is_contiguous():
@@ -218,11 +225,7 @@ class Linear:
               "scale: [N], with float8_e4m3fn weights and dtype w8a16 only")
         _need(scale is not None or weight.dtype != torch.float8_e4m3fn, "float8_e4m3fn weights need their scale")
         _lib.require_gpu()
-        if device is None:
-            device = weight.device if weight.device.type == "cuda" else torch.device("cuda", torch.cuda.current_device())
-        self.device = torch.device(device)
-        if self.device.index is None:
-            self.device = torch.device("cuda", torch.cuda.current_device())
+        self.device = _gpu(weight.device if device is None and weight.device.type == "cuda" else device)
         self.lib = _lib.load()
         self.N, self.K, self.dtype = N, K, dtype
         self.tdtype = torch.float32 if dtype == "f32" else torch.bfloat16
@@ -353,9 +356,7 @@ class Rotary:
         else:
             e = [f / n for n in sections for f in range(n)]
         self.dim, self.sections, self.axes, self.layout = dim, sections, len(sections), layout
-        self.device = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
-        if self.device.index is None:
-            self.device = torch.device("cuda", torch.cuda.current_device())
+        self.device = _gpu(device)
         self._turns = torch.tensor([base ** -v / (2 * math.pi) for v in e], dtype=torch.float64, device=self.device)
         self._axis = torch.tensor([a for a, n in enumerate(sections) for _ in range(n)], dtype=torch.int32,
                                   device=self.device)
@@ -375,7 +376,7 @@ class TokenCache:
         _need(dtype in ("bf16", "f32"), f"dtype {dtype!r}: bf16 or f32")
         _need(min(B, slots, heads, head_dim) > 0, "B, slots, heads and head_dim are positive")
         _lib.require_gpu()
-        t, dev = torch.float32 if dtype == "f32" else torch.bfloat16, device if device is not None else "cuda"
+        t, dev = torch.float32 if dtype == "f32" else torch.bfloat16, _gpu(device)
         self._set(torch.zeros(B, slots, heads, head_dim, dtype=t, device=dev),
                   torch.zeros(B, slots, heads, v_dim or head_dim, dtype=t, device=dev), sinks,
                   torch.zeros(B, dtype=torch.int32, device=dev))
@@ -438,9 +439,7 @@ class QKNorm:
             _need(w is None or w.shape == (head_dim,), f"{n}: [{head_dim}]")
         _lib.require_gpu()
         self.lib = _lib.load()
-        self.device = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
-        if self.device.index is None:
-            self.device = torch.device("cuda", torch.cuda.current_device())
+        self.device = _gpu(device)
         _need(rotary is None or rotary.device == self.device, "rotary: on another device")
         self.D, self._rotary = head_dim, rotary
         self._wq, self._wk = (None if w is None else w.detach().to(self.device, torch.float32).contiguous()
