@@ -575,6 +575,14 @@ typedef struct va_tok_linear_args {
     int32_t pad;
 } va_tok_linear_args;
 int va_tok_linear(void* stream, const va_tok_linear_args* a);
+/* The kernel that the sizes, strides and types of a call choose (or VA_ERR_ARG): any rows; few rows or tiles, K over a
+ * workgroup's waves; tiles of 128 x 64; those with K halved between two groups of waves; tiles of 256 x 128. */
+#define VA_TOK_LINEAR_ANY 0
+#define VA_TOK_LINEAR_FEW 1
+#define VA_TOK_LINEAR_TILE 2
+#define VA_TOK_LINEAR_TILE_2K 3
+#define VA_TOK_LINEAR_LARGE 4
+int va_tok_linear_form(const va_tok_linear_args* a);
 
 /* Norm of each head's vector, x / sqrt(mean(x^2) + eps) * weight, then the rotation of its first `rot` values by the
  * token's position on one or more axes (time, height, width), for the Hq query heads and the Hk key heads of B x S

@@ -242,3 +242,61 @@ def test_layers_are_made_on_a_gpu():
     for d in (None, "cuda", here):
         assert Linear(torch.zeros(8, 8), device=d).device == QKNorm(8, Rotary(8, device=d), device=d).device == here
         assert TokenCache(1, 4, 1, 8, device=d).k.device == here
+
+
+ANY, FEW, TILE, TILE_2K, LARGE = range(5)  # VA_TOK_LINEAR_*
+FORMS = [(ANY, "bf16", 130, 131, 201), (ANY, "w8a16", 130, 131, 201), (ANY, "f32", 130, 131, 201),
+         (FEW, "bf16", 9, 1032, 300), (FEW, "bf16", 30, 520, 301), (FEW, "w8a16", 9, 1032, 300), (FEW, "w8a16", 61, 520, 301),
+         (FEW, "f32", 29, 516, 300), (FEW, "bf16", 300, 200, 500),
+         (TILE, "bf16", 1301, 328, 1001), (TILE, "w8a16", 2115, 328, 1044), (TILE, "f32", 2115, 332, 1044),
+         (TILE_2K, "w8a16", 1301, 456, 1001), (TILE_2K, "f32", 1301, 332, 1001), (TILE_2K, "f32", 1301, 64, 580),
+         (LARGE, "bf16", 3700, 328, 2101), (LARGE, "w8a16", 4500, 328, 2101)]
+
+
+@pytest.mark.parametrize("form,dtype,M,K,N", FORMS)
+def test_linear_forms(form, dtype, M, K, N):
+    """Each kernel form over several turns of its ring, at ragged rows, channels and K: every activation, bias, residual,
+    result = residual, float results, and rows of the result that take stores of eight, four and single values.  Bound: float
+    sums (K + 8) 2^-24 sum |x w| with the activations' slope, 2^-14 of a bf16 result for its hardware activation (float: 2^-21),
+    and the result's half step."""
+    import ctypes
+
+    from vision_assist_amd import _lib
+    from vision_assist_amd.tokens import Linear
+    from tests.test_gpu_tokens import act64
+    g = torch.Generator().manual_seed(M + K + N)
+    t = DT[dtype]
+    x, w, b, r = rnd(g, M, K, dtype=t), rnd(g, N, K, by=K ** -0.5), rnd(g, N, by=0.3), rnd(g, M, N, dtype=t)
+    scale = None
+    if dtype == "w8a16":
+        scale = w.abs().amax(1) / 448
+        w = (w / scale[:, None]).to(torch.float8_e4m3fn)
+    elif dtype == "bf16":
+        w = w.to(t)
+    wd = w.double() if scale is None else w.double() * scale.double()[:, None]
+    raw, mag = x.double() @ wd.t(), x.double().abs() @ wd.abs().t()
+    sums = 1.2 * (K + 8) * 2.0 ** -24 * (mag + b.double().abs()) + 2.0 ** -30
+    x, rd = x.cuda(), r.cuda()
+    # (activation, bias, residual, float result, width of the result's rows, first column; None: a tensor of the call's own)
+    calls = [(None, False, False, False, None, 0), ("silu", True, True, False, (N + 15) // 8 * 8, 8), ("gelu", True, False, False, None, 0),
+             ("gelu_tanh", False, True, False, (N + 7) // 4 * 4 // 8 * 8 + 4, 4), ("relu", True, True, False, N + 4 - N % 2, 1),
+             ("gelu", True, True, True, (N + 15) // 8 * 8, 4), ("silu", False, False, True, N | 1, 0), (None, True, True, True, (N + 7) // 4 * 4, 4)]
+    for act, bias, res, f32, width, first in calls:
+        lin = Linear(w, b if bias else None, act=act, dtype=dtype, scale=scale, device="cuda")
+        ot = torch.float32 if f32 else t
+        buf = torch.full((M, N if width is None else width + first), 3.0, dtype=ot, device="cuda")
+        out = buf[:, first:first + N]
+        same = res and ot == t and width is not None  # the result is the residual
+        if same:
+            out.copy_(rd)
+        arg = out if same else rd if res else None
+        assert _lib.load().va_tok_linear_form(ctypes.byref(lin.args(x, out, arg))) == form
+        assert lin(x, residual=arg, out=out) is out
+        y = act64(raw + b.double() if bias else raw, act)
+        want = y + r.double() if res else y
+        got = out.double().cpu()
+        u = U[torch.float32] if f32 or dtype == "f32" else U[torch.bfloat16]
+        tol = sums + (2.0 ** -21 if u < 2.0 ** -20 else 2.0 ** -14) * (y.abs() + want.abs()) + u * (want.abs() + sums)
+        worst = float(((got - want).abs() / tol).max())
+        assert worst <= 1, (act, bias, res, f32, width, first, worst)
+        assert (buf[:, :first] == 3).all() and (buf[:, first + N:] == 3).all()

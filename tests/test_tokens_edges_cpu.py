@@ -78,3 +78,15 @@ def test_args_of_an_op_list_are_checked():
                 (x, z(1, 6).expand(5, 6))):
         with pytest.raises(_lib.VaError):
             lin.args(*bad)
+
+
+def test_the_form_of_a_call():
+    import ctypes
+
+    from vision_assist_amd.tokens import LinearArgs
+    lib, a = _lib.load(), dict(x=4096, w=4096, y=4096, ldx=64, ldy=64, N=64, K=64, Npad=64, Kpad=64, dtype=1)
+    form = lambda **kw: lib.va_tok_linear_form(ctypes.byref(LinearArgs(**{**a, **kw})))
+    assert lib.va_tok_linear_form(None) == form(M=-1) == form(dtype=3) == _lib.VA_ERR_ARG
+    assert form(M=1) == form(M=64) == form(M=1, dtype=2) == 1 and form(M=1, x=4098) == form(M=1, K=63) == 0
+    assert form(M=20000) == form(M=1 << 20, dtype=2) == 2 and form(M=20000, dtype=2) == 3
+    assert form(M=1 << 20) == form(M=1 << 20, w8=1, wscale=4096) == 4

@@ -87,6 +87,7 @@ SIGNATURES = [
     ("va_post_polygons", I32, [P, P, P, P, I32]),
     ("va_letterbox", I32, [P, P, I32, I32, I32, P, I32, I32, I32, I32, I32, I32]),
     ("va_tok_linear", I32, [P, P]),
+    ("va_tok_linear_form", I32, [P]),
     ("va_tok_qk", I32, [P, P]),
     ("va_tok_attn_workspace_bytes", I64, [P]),
     ("va_tok_attn", I32, [P, P]),

@@ -718,17 +718,14 @@ hipError_t go_any(const va_tok_linear_args& a, const Out& o, hipStream_t st, int
 }
 
 template <Form F>
-hipError_t go(const va_tok_linear_args& a, const Out& o, hipStream_t st) {
+int form_of(const va_tok_linear_args& a) {
     constexpr int E = F == F32 ? 4 : 8;
-    const int xvec = a.ldx % 8 == 0 && !((uintptr_t)a.x & 15);
-    if (a.K % E || a.ldx % E || ((uintptr_t)a.x & 15) || a.ldx > LIN_ROW || a.Kpad > LIN_ROW) return go_any<F>(a, o, st, xvec);
+    if (a.K % E || a.ldx % E || ((uintptr_t)a.x & 15) || a.ldx > LIN_ROW || a.Kpad > LIN_ROW) return VA_TOK_LINEAR_ANY;
     const int64_t t64 = (int64_t)((a.N + 63) / 64) * ((a.M + 63) / 64);
-    if (a.M <= 16) return go_few<F, 1>(a, o, st);
-    if (a.M <= 32) return go_few<F, 2>(a, o, st);
     // Measured (us, graph replays, K 1024; few | tiles): 112 tiles of 64 x 64: bf16 8.5 | 10.4, e4m3 8.7 | 16.0, float
     // 16.2 | 23.3; 128: 8.6 | 10.2, 8.9 | 16.1, 17.3 | 23.4; 208: 15.4 | 10.6, 15.8 | 16.4, 31.1 | 24.7; 256: 16.1 | 10.7,
     // 16.2 | 16.3, 31.7 | 25.5
-    if (a.M <= 64 || t64 <= (is8(F) ? 256 : 128)) return go_few<F, 4>(a, o, st);
+    if (a.M <= 64 || t64 <= (is8(F) ? 256 : 128)) return VA_TOK_LINEAR_FEW;
     // Tiles of 128 x 64 | of 256 x 128, by the number of large ones: bf16 208 25.2 | 25.5, 400 42.0 | 37.4; e4m3 208
     // 28.9 | 33.4, 400 50.1 | 44.5.
     // Up to 256 tiles of 128 x 64, a workgroup a CU: one group of four waves | K halved between two, by the number of 64 x 64
@@ -736,11 +733,25 @@ hipError_t go(const va_tok_linear_args& a, const Out& o, hipStream_t st) {
     // 13.1, 448 16.6 | 13.1, 800 19.2 | 19.0; bf16, whose steps are short, 400 11.1 | 10.6, at K 520 8.2 | 8.5: one group.
     if constexpr (F != F32) {
         const int64_t big = (int64_t)((a.N + 255) / 256) * ((a.M + 127) / 128);
-        if (big >= (is8(F) ? 320 : 224)) return go_tile<F, 4, 2, 1>(a, o, st);
+        if (big >= (is8(F) ? 320 : 224)) return VA_TOK_LINEAR_LARGE;
     }
-    if constexpr (F == F32 || is8(F))
-        if (t64 <= 512) return go_tile<F, 2, 1, 2>(a, o, st);
-    return go_tile<F, 2, 1, 1>(a, o, st);
+    return (F == F32 || is8(F)) && t64 <= 512 ? VA_TOK_LINEAR_TILE_2K : VA_TOK_LINEAR_TILE;
+}
+
+template <Form F>
+hipError_t go(const va_tok_linear_args& a, const Out& o, hipStream_t st) {
+    switch (form_of<F>(a)) {
+        case VA_TOK_LINEAR_FEW:
+            return a.M <= 16 ? go_few<F, 1>(a, o, st) : a.M <= 32 ? go_few<F, 2>(a, o, st) : go_few<F, 4>(a, o, st);
+        case VA_TOK_LINEAR_TILE: return go_tile<F, 2, 1, 1>(a, o, st);
+        case VA_TOK_LINEAR_TILE_2K:
+            if constexpr (F == F32 || is8(F)) return go_tile<F, 2, 1, 2>(a, o, st);
+            break;
+        case VA_TOK_LINEAR_LARGE:
+            if constexpr (F != F32) return go_tile<F, 4, 2, 1>(a, o, st);
+            break;
+    }
+    return go_any<F>(a, o, st, a.ldx % 8 == 0 && !((uintptr_t)a.x & 15));
 }
 }  // namespace
 
@@ -763,4 +774,11 @@ extern "C" int va_tok_linear(void* stream, const va_tok_linear_args* ap) {
                          : a.out_f32 ? (a.w8 ? go<W8F>(a, o, st) : go<BF16F>(a, o, st))
                                      : (a.w8 ? go<W8>(a, o, st) : go<BF16>(a, o, st));
     return e == hipSuccess ? VA_OK : e == hipErrorInvalidConfiguration ? VA_ERR_RANGE : VA_ERR_HIP;
+}
+
+extern "C" int va_tok_linear_form(const va_tok_linear_args* ap) {
+    if (!ap || !linear_ok(*ap)) return VA_ERR_ARG;
+    const va_tok_linear_args& a = *ap;
+    if (a.dtype == VA_DTYPE_F32) return form_of<F32>(a);
+    return a.w8 ? form_of<W8>(a) : form_of<BF16>(a);
 }
