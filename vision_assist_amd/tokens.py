@@ -194,8 +194,11 @@ def _blocks(w: torch.Tensor) -> torch.Tensor:
 
 def _terms(w: torch.Tensor) -> torch.Tensor:
     """[N, K] float -> its bf16 terms h, m, l [3, N, K], of any value (va355.h va_tok_linear_args.w)."""
-    h, m, l = split3_bf16(w).permute(2, 0, 1, 3).reshape(3, *w.shape)
-    far, inf = w.abs() >= float.fromhex("0x1.ffp127"), w.isinf()
+    t = split3_bf16(w).permute(2, 0, 1, 3).reshape(3, *w.shape)
+    far = w.abs() >= float.fromhex("0x1.ffp127")
+    if not far.any():
+        return t
+    (h, m, l), inf = t, w.isinf()
     h = torch.where(far, torch.where(inf, 1.0, torch.finfo(torch.bfloat16).max).copysign(w).to(h.dtype), h)
     r = torch.where(far, w - h.float(), 0.0)
     m = torch.where(inf, 0.0, torch.where(far, r.to(h.dtype), m))
