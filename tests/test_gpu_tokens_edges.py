@@ -300,3 +300,17 @@ def test_linear_forms(form, dtype, M, K, N):
         worst = float(((got - want).abs() / tol).max())
         assert worst <= 1, (act, bias, res, f32, width, first, worst)
         assert (buf[:, :first] == 3).all() and (buf[:, first + N:] == 3).all()
+
+
+def test_layers_keep_their_own_weights():
+    """What a layer was made of may change afterwards, all of it or none: the layer is what it was."""
+    from vision_assist_amd.tokens import Linear, QKNorm
+    g = torch.Generator().manual_seed(7)
+    w, b, n = rnd(g, 96, 64).cuda(), rnd(g, 96).cuda(), 1 + rnd(g, 64).cuda()
+    x = rnd(g, 2, 5, 3, 64, dtype=torch.float32).cuda()
+    layers = [Linear(w, b, dtype="f32"), Linear(w, b, dtype="w8a16"), QKNorm(64, q_weight=n, k_weight=n)]
+    calls = [lambda: layers[0](x), lambda: layers[1](x.bfloat16()), lambda: torch.stack(layers[2](x, x))]
+    want = [c() for c in calls]
+    for t in (w, b, n):
+        t.add_(1)
+    assert all(torch.equal(c(), y) for c, y in zip(calls, want))

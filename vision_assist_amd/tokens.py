@@ -91,6 +91,11 @@ def _gpu(device) -> torch.device:
     return d if d.index is not None else torch.device("cuda", torch.cuda.current_device())
 
 
+def _floats(t: torch.Tensor | None, dev: torch.device) -> torch.Tensor | None:
+    """A layer's own copy of a vector, as its weights are one: the caller's may change later."""
+    return None if t is None else t.detach().to(dev, torch.float32, copy=True, memory_format=torch.contiguous_format)
+
+
 def _range(t: torch.Tensor) -> tuple[int, int]:
     """The bytes between a tensor's first and last element (0, 0: it has none)."""
     if t.is_contiguous():
@@ -254,7 +259,7 @@ class Linear:
             self._w = torch.stack([_blocks(t) for t in _terms(padded(w.float()))])
         else:
             self._w = _blocks(padded(w.to(torch.bfloat16)))
-        self._bias = None if bias is None else bias.detach().to(self.device, torch.float32).contiguous()
+        self._bias = _floats(bias, self.device)
         self._ptrs = (self._w.data_ptr(), self._wscale.data_ptr() if self._wscale is not None else 0,
                       self._bias.data_ptr() if bias is not None else 0)
         self._ints = (N, K, Np, Kp, VA_DTYPE_F32 if dtype == "f32" else VA_DTYPE_BF16, int(dtype == "w8a16"), ACTS[act])
@@ -445,8 +450,7 @@ class QKNorm:
         self.device = _gpu(device)
         _need(rotary is None or rotary.device == self.device, "rotary: on another device")
         self.D, self._rotary = head_dim, rotary
-        self._wq, self._wk = (None if w is None else w.detach().to(self.device, torch.float32).contiguous()
-                              for w in (q_weight, k_weight))
+        self._wq, self._wk = _floats(q_weight, self.device), _floats(k_weight, self.device)
         self.eps = float(eps)
         self._norm = (self.wq.data_ptr() if self.wq is not None else 0, self.wk.data_ptr() if self.wk is not None else 0,
                       self.eps)
