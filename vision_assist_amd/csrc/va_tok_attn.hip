@@ -12,7 +12,7 @@
 // the keys, and few tiles rescale.  bf16, many rows: the probabilities are rounded to bf16 for the second product (half a
 // step, 2^-8 of each at most), and the sum is of the rounded ones, which is what the product weighs by.  Few rows (single
 // tokens over a cache) are bound by the cache's bytes, so there a probability enters as two bf16 terms (2^-16 of it is left
-// out) and the sum is of the floats: 1 % of the time (161.1 us against 159.4 for 32 streams over 6800 slots), and the error
+// out) and the sum is of the floats: 1 % of the time (161.1 us against 159.4 for 32 streams over 6800 slots, graph replays), and the error
 // against float64 is the output's own rounding (0.0017 instead of 0.0023, relative L2).  For many rows the second term's
 // MFMAs and conversions were 23 to 27 % of the time (116 -> 143 us, 136 -> 168, 254 -> 324).
 //
@@ -456,9 +456,9 @@ struct Walk {
 // rows are offsets from one address; rows and pieces that are not there take an offset out of range and load zeros.
 // Bound by the instructions between the products: at D = 128 MFMAs and vector instructions (an exp2 of four issue slots,
 // a multiply-add, half a maximum, half a conversion and half a sum for each score) take half of a SIMD's time each, and two
-// waves overlap them in part.  Measured, bf16: 16 heads over 2 key heads, 8192 tokens, window 4096, D 128: 255 us, 809
-// TFLOP/s; 8 streams, 400 queries over 3200 keys, D 128: 118 us, 708 TFLOP/s; two clips of 6400 tokens, frames of 400, D
-// 64: 137 us, 574 TFLOP/s.  Float (32-bit MFMA, 154 TFLOP/s at most): 16 x 8 heads of 400 x 400, D 32, Dv 64: 53 us, 74 TFLOP/s.
+// waves overlap them in part.  Measured, bf16: 16 heads over 2 key heads, 8192 tokens, window 4096, D 128: 258 us, 799
+// TFLOP/s; 8 streams, 400 queries over 3200 keys, D 128: 119 us, 704 TFLOP/s; two clips of 6400 tokens, frames of 400, D
+// 64: 138 us, 570 TFLOP/s.  One such stream alone is 56 workgroups for 256 CUs, each of which walks all keys: 92 us.  Float (32-bit MFMA, 154 TFLOP/s at most): 16 x 8 heads of 400 x 400, D 32, Dv 64: 53 us, 74 TFLOP/s.
 constexpr int TILE_OOB = 0x7ffffff0;
 
 // (a plain function: the host pass drops the stub of a kernel template that names the builtin)
@@ -594,7 +594,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DV <= 64 ? 3 : 2) : (DV <= 6
 // turn, each through two buffers of its own in LDS and without a barrier, until their sums are joined.  A tile comes by
 // LDS-DMA while the one before is worked on, whole rows at a time (a load covers complete cache lines: reading each key's
 // row by its own lane instead, 32 lines at a time, ran at 1.7 TB/s).  Bound by the bytes of the keys and values: 32
-// streams over 6800 slots, 8 key heads of 128: 149 us, 4.3 TB/s (a large copy: 4.9).
+// streams over 6800 slots, 8 key heads of 128: 153 us, 4.2 TB/s (a large copy: 4.8).
 // A share's result: [NV * 16][64] registers as they lie in the wave, then the 32 rows' maxima and sums.
 __device__ __forceinline__ int64_t part_floats(int NV) { return NV * 16 * 64 + 64; }
 

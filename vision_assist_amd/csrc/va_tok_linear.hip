@@ -4,8 +4,8 @@
 // accumulator registers are consecutive channels of one token: the epilogue stores them as vectors.
 //
 // float: x = h + m + l exactly in three bf16 terms (so are the weights), and six of the nine term products are kept -- the
-// three left out come to 2^-23 of a product's size at most -- so a product runs on the bf16 MFMA at a sixth of its rate, 215 TFLOP/s
-// by the bf16 product measured here, where the 32-bit MFMA reaches 154.  e4m3 weights: every e4m3 value is a bf16 value; the
+// three left out come to 2^-23 of a product's size at most -- so a product runs on the bf16 MFMA at a sixth of its rate, 245 TFLOP/s
+// by the library's large bf16 product (1467), where the 32-bit MFMA reaches 154.  e4m3 weights: every e4m3 value is a bf16 value; the
 // row's scale is applied to the sum.
 #include <type_traits>
 
@@ -194,10 +194,12 @@ __device__ __forceinline__ void grouped_tile(int i, int ntn, int ntm, int* tn, i
 // each token is looked at, and the tile is formed once more with split3_far if it is one, by a loop of its own (a test of
 // every split value was 4 to 5 % of the time, split3_far in the loop itself 0 to 6 %).
 // Two workgroups of 256 x 128 share a CU: the epilogue of one (activations: VALU, stores) runs beside the MFMAs of the
-// other.  (One workgroup of 256 x 256 a CU: slower for want of that; deeper rings: no faster, and one workgroup a CU.)
-// Bound by the MFMAs and the issue around them: 8192^3 in bf16 1198 TFLOP/s (the library's product: 1548); 25600 x 1024 x
-// 4096 with bias and GELU 249 us, 863 TFLOP/s, of which the GELU is some 60 us of vector instructions that the MFMAs of the
-// other workgroup cover in part; float 1603 x 520 x 1000 with a residual 18.4 us: 208 workgroups, two waves a SIMD.
+// other.  (One workgroup of 256 x 256 a CU, without that: 1222 TFLOP/s where this form had 1198 at 8192^3, but 334 us
+// instead of 304 with GELU at 25600 x 1024 x 4096; deeper rings: no faster, and one workgroup a CU.)
+// Bound by the MFMAs and the issue around them, on one GPU: 8192^3 in bf16 1157 TFLOP/s (the library's product: 1467); 25600 x
+// 1024 x 4096 216 us, 995 TFLOP/s (the library's: 184 us), with bias and GELU 241 to 254 us, whose vector instructions the
+// MFMAs of the other workgroup cover in part; with e4m3 weights, which both waves that read a fragment convert, 262 us, with
+// GELU 302; float 1603 x 520 x 1000 with a residual 18.7 us: 208 workgroups, two waves a SIMD.
 constexpr int LIN_OOB = 0x7ffffff0;      // an offset that a descriptor of that many bytes answers with zeros
 constexpr int LIN_ROW = 1 << 21;         // longest rows in values: the offsets of 256 of them stay within 31 bits
 
@@ -535,8 +537,10 @@ __global__ __launch_bounds__((256 * KG), 2) void linear_tile(va_tok_linear_args 
 // 16 channels x 16 MB tokens per workgroup; its eight waves take every eighth step of 128 bytes of the tokens' rows, each
 // through two slots of its own in LDS and without a barrier, and their sums are joined in LDS in the waves' order.
 // v_mfma_f32_16x16x32_bf16.
-// Bound by the weights' bytes (32 x 4096 x 4096 over 24 sets of weights: e4m3 9.3 us, bf16 11.0; x 16384: 30.6 and 36.2,
-// 3.7 TB/s; one token, 1024 x 4096: 4.6).  The tokens come by LDS-DMA, eight lanes to a row's 128 bytes: loaded straight
+// 32 x 4096 x 4096 over 24 sets of weights: bf16 11.0 us, e4m3 9.3; x 16384: 36.2 and 30.6 us.  bf16 is bound by the weights'
+// bytes, 3.7 TB/s; e4m3, at 2.2 TB/s of weights, by the tokens: 16 channels are 64 KB of e4m3 weights and read 256 KB of
+// tokens through L2 and LDS, so half the bytes saves 15 % of the time.  One token, 1024 x 4096: 4.3.  Float weights are 6
+// bytes a value: 32 x 4096 x 4096 22 us, 4.6 TB/s of them.  The tokens come by LDS-DMA, eight lanes to a row's 128 bytes: loaded straight
 // into the fragments neighbouring lanes held different rows, so that each lane's 16 bytes was a request of its own, and
 // the tokens, not the weights, took the time (12.9, 14.1; 49.0 and 52.9 us).  Three or four slots: 1 to 9 us slower where
 // workgroups queue, as fewer fit a CU.

@@ -5,8 +5,8 @@
 // token turns by the same angles -- then its heads, several at a time.  A lane holds P pairs (lo, hi) of a head, so the
 // rotation needs no exchange; the mean of squares is one butterfly over the head's lanes.
 //
-// Bound by memory: the tensors are read and written once.  8 x 1600 tokens, 12 + 12 heads of 64, three axes, bf16: 21.9 us,
-// 3.6 TB/s (a large copy: 4.9); one token of 64 streams into their caches: 7 us, a launch and two dependent loads.
+// Bound by memory: the tensors are read and written once.  8 x 1600 tokens, 12 + 12 heads of 64, three axes, bf16: 21.7 us,
+// 3.6 TB/s (a large copy: 4.8); one token of 64 streams into their caches: 7 us, a launch and two dependent loads.
 #include "va_tok.h"
 
 namespace {
