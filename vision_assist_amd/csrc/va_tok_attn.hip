@@ -368,28 +368,48 @@ __device__ __forceinline__ void settle(const va_tok_attn_args& a, f32x16 (&x)[NB
 #pragma unroll
         for (int i = 0; i < 16; ++i) z = __builtin_fmaf(x[v][i], 0.0f, z);
     if (__builtin_expect(z == z || sum != sum, 1)) return;
-    unsigned plus[NB], minus[NB];
+    // U keys at a time, so that their loads run together, until every such column has shown that it is NaN
+    constexpr int U = NB == 1 ? 8 : NB == 2 ? 4 : 2;
+    unsigned plus[NB], minus[NB], open[NB];
 #pragma unroll
-    for (int v = 0; v < NB; ++v) plus[v] = minus[v] = 0;
+    for (int v = 0; v < NB; ++v) {
+        plus[v] = minus[v] = open[v] = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) open[v] |= (unsigned)!(fabsf(x[v][i]) < INFINITY) << i;
+    }
+    bool more = true;
 #pragma unroll 1
     for (int part = 0; part < 2; ++part) {
         const int end = part ? sp.top : min(a.sinks, sp.top);
 #pragma unroll 1
-        for (int p = part ? sp.low : 0; p < end; ++p) {
-            const T* row = vb + (int64_t)slot_of(a, p) * a.v_ss;
+        for (int p = part ? sp.low : 0; p < end && more; p += min(U, end - p)) {
+            const T* row[U];  // (the last one's again where there are fewer)
 #pragma unroll
-            for (int v = 0; v < NB; ++v)
+            for (int u = 0; u < U; ++u) row[u] = vb + (int64_t)slot_of(a, p + min(u, end - 1 - p)) * a.v_ss;
 #pragma unroll
-                for (int i = 0; i < 16; i += 4) {
-                    const int d = 32 * (v0 + v) + key_of(i, lh);
-                    if (d >= a.Dv) continue;
+            for (int u = 0; u < U; ++u)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float y = (float)row[d + e];
-                        plus[v] |= (unsigned)!(y < INFINITY) << (i + e);  // (NaN: both)
-                        minus[v] |= (unsigned)!(y > -INFINITY) << (i + e);
+                for (int v = 0; v < NB; ++v)
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) {
+                        const int d = min(32 * (v0 + v) + key_of(i, lh), a.Dv - 4);  // (columns from Dv on are not stored)
+                        float four[4];
+                        if constexpr (sizeof(T) == 2) {
+                            const u32x2 y = *(const u32x2*)(row[u] + d);
+                            four[0] = bf_lo(y[0]), four[1] = bf_hi(y[0]), four[2] = bf_lo(y[1]), four[3] = bf_hi(y[1]);
+                        } else {
+                            const f32x4 y = *(const f32x4*)(row[u] + d);
+                            four[0] = y[0], four[1] = y[1], four[2] = y[2], four[3] = y[3];
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            plus[v] |= (unsigned)!(four[e] < INFINITY) << (i + e);  // (NaN: both)
+                            minus[v] |= (unsigned)!(four[e] > -INFINITY) << (i + e);
+                        }
                     }
-                }
+            more = false;
+#pragma unroll
+            for (int v = 0; v < NB; ++v) more |= (open[v] & ~(plus[v] & minus[v])) != 0;
         }
     }
 #pragma unroll
