@@ -12,9 +12,9 @@
 // the keys, and few tiles rescale.  bf16, many rows: the probabilities are rounded to bf16 for the second product (half a
 // step, 2^-8 of each at most), and the sum is of the rounded ones, which is what the product weighs by.  Few rows (single
 // tokens over a cache) are bound by the cache's bytes, so there a probability enters as two bf16 terms (2^-16 of it is left
-// out) and the sum is of the floats: 1 % of the time (161.1 us against 159.4 for 32 streams over 6800 slots, graph replays), and the error
-// against float64 is the output's own rounding (0.0017 instead of 0.0023, relative L2).  For many rows the second term's
-// MFMAs and conversions were 23 to 27 % of the time (116 -> 143 us, 136 -> 168, 254 -> 324).
+// out) and the sum is of the floats: 1 % of the time (161.1 us against 159.4 for 32 streams over 6800 slots, graph
+// replays), and the error against float64 is the output's own rounding (0.0017 instead of 0.0023, relative L2).  For many
+// rows the second term's MFMAs and conversions were 23 to 27 % of the time (116 -> 143 us, 136 -> 168, 254 -> 324).
 //
 // What is not finite in a value that no row of a tile's part sees must not meet a probability of 0 in an MFMA: in tiles
 // that some row does not see whole, such values are replaced by 0 as the tile arrives (take_out) and added afterwards by
@@ -478,7 +478,9 @@ struct Walk {
 // a multiply-add, half a maximum, half a conversion and half a sum for each score) take half of a SIMD's time each, and two
 // waves overlap them in part.  Measured, bf16: 16 heads over 2 key heads, 8192 tokens, window 4096, D 128: 258 us, 799
 // TFLOP/s; 8 streams, 400 queries over 3200 keys, D 128: 119 us, 704 TFLOP/s; two clips of 6400 tokens, frames of 400, D
-// 64: 138 us, 570 TFLOP/s.  One such stream alone is 56 workgroups for 256 CUs, each of which walks all keys: 92 us.  Float (32-bit MFMA, 154 TFLOP/s at most): 16 x 8 heads of 400 x 400, D 32, Dv 64: 53 us, 74 TFLOP/s.
+// 64: 138 us, 570 TFLOP/s.  One stream's 400 queries alone (16 over 8 heads) are 56 workgroups for 256 CUs, each of which
+// walks all keys: 92 us.  Float (32-bit MFMA, 154 TFLOP/s at most): 16 x 8 heads of 400 x 400, D 32, Dv 64: 53 us, 74
+// TFLOP/s.
 constexpr int TILE_OOB = 0x7ffffff0;
 
 // (a plain function: the host pass drops the stub of a kernel template that names the builtin)

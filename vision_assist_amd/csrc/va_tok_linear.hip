@@ -540,10 +540,10 @@ __global__ __launch_bounds__((256 * KG), 2) void linear_tile(va_tok_linear_args 
 // 32 x 4096 x 4096 over 24 sets of weights: bf16 11.0 us, e4m3 9.3; x 16384: 36.2 and 30.6 us.  bf16 is bound by the weights'
 // bytes, 3.7 TB/s; e4m3, at 2.2 TB/s of weights, by the tokens: 16 channels are 64 KB of e4m3 weights and read 256 KB of
 // tokens through L2 and LDS, so half the bytes saves 15 % of the time.  One token, 1024 x 4096: 4.3.  Float weights are 6
-// bytes a value: 32 x 4096 x 4096 22 us, 4.6 TB/s of them.  The tokens come by LDS-DMA, eight lanes to a row's 128 bytes: loaded straight
-// into the fragments neighbouring lanes held different rows, so that each lane's 16 bytes was a request of its own, and
-// the tokens, not the weights, took the time (12.9, 14.1; 49.0 and 52.9 us).  Three or four slots: 1 to 9 us slower where
-// workgroups queue, as fewer fit a CU.
+// bytes a value: 32 x 4096 x 4096 22 us, 4.6 TB/s of them.
+// The tokens come by LDS-DMA, eight lanes to a row's 128 bytes: loaded straight into the fragments neighbouring lanes held
+// different rows, so that each lane's 16 bytes was a request of its own, and the tokens, not the weights, took the time
+// (12.9, 14.1; 49.0 and 52.9 us).  Three or four slots: 1 to 9 us slower where workgroups queue, as fewer fit a CU.
 template <Form F, int MB>
 struct FewCfg {
     static constexpr int NW = 8, XE = F == F32 ? 4 : 2, KS = 128 / XE;  // waves; K of a step
